@@ -3,7 +3,8 @@
 The public names are those of ``diffrast`` (``src/diffrast/__init__.py:21-41``): switching is
 changing the import (``import diffrast_b200 as dr``, or ``diffrast_b200.torch``). ``to_clip`` (the
 world-to-clip transform of diffrast's examples), ``antialias_mse`` (antialias with a fused
-squared-error loss) and ``lambert`` (shading from interpolated normals) are additions.
+squared-error loss), ``lambert`` (shading from interpolated normals), and ``group_norm`` and
+``dropout`` (the feature images of a learned shader) are additions.
 """
 
 from diffrast_b200.backends import get_backend_name, set_backend
@@ -20,6 +21,8 @@ from diffrast_b200.ops import (
     antialias,
     antialias_construct_topology_hash,
     antialias_mse,
+    dropout,
+    group_norm,
     interpolate,
     lambert,
     rasterize,
@@ -43,8 +46,10 @@ __all__ = [
     "antialias",
     "antialias_construct_topology_hash",
     "antialias_mse",
+    "dropout",
     "get_backend_name",
     "get_log_level",
+    "group_norm",
     "install_as_diffrast",
     "install_as_nvdiffrast",
     "interpolate",

@@ -705,6 +705,49 @@ class Lambert(torch.autograd.Function):
         return grad_color, grad_normal, None, None
 
 
+class GroupNorm(torch.autograd.Function):
+    """Group normalisation with an activation and dropout of a feature image. ``drop`` comes
+    without its seed tensor, which is an input of its own: saved like the others, a seed that was
+    changed in place between the passes is reported instead of giving another mask."""
+
+    @staticmethod
+    def forward(ctx, x: Tensor, weight: Tensor | None, bias: Tensor | None, seed: Tensor | None,
+                groups: int, eps: float, activation: int, drop: K.Drop):
+        y, stats = K.group_norm_fwd(x, groups, weight, bias, eps, activation,
+                                    drop._replace(seed=seed))
+        ctx.save_for_backward(*(_saveable(t) for t in (x, weight, bias, seed, stats)))
+        ctx.groups, ctx.activation, ctx.drop = groups, activation, drop
+        return y
+
+    @staticmethod
+    @first_order("group_norm")
+    def backward(ctx, grad_out):
+        x, weight, bias, seed, stats = ctx.saved_tensors
+        grads = K.group_norm_bwd(x, grad_out, ctx.groups, weight, bias, stats, ctx.activation,
+                                 ctx.drop._replace(seed=seed), ctx.needs_input_grad[:3])
+        return *grads, None, None, None, None, None
+
+
+class Dropout(torch.autograd.Function):
+    """``residual + dropout(x)``; ``drop`` and ``seed`` as for :class:`GroupNorm`."""
+
+    @staticmethod
+    def forward(ctx, x: Tensor, residual: Tensor | None, seed: Tensor | None, drop: K.Drop):
+        ctx.save_for_backward(_saveable(seed))
+        ctx.drop = drop
+        return K.dropout(x, residual, drop._replace(seed=seed))
+
+    @staticmethod
+    @first_order("dropout")
+    def backward(ctx, grad_out):
+        (seed,) = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        grad_x = None
+        if need[0]:
+            grad_x = K.dropout(grad_out.contiguous(), None, ctx.drop._replace(seed=seed))
+        return grad_x, grad_out if need[1] else None, None, None
+
+
 class ToClip(torch.autograd.Function):
     """World-to-clip transform of shared positions by per-view matrices."""
 

@@ -764,6 +764,114 @@ def antialias_mse_bwd(color, rast, pos3, tri, opposite, residual, loss_grad, sca
     return grad_color, grad_pos
 
 
+class Drop(NamedTuple):
+    """Dropout of a call: ``threshold`` in 2**-16 (0: none), the seed as a device word or a
+    number, and the layer."""
+
+    threshold: int
+    seed: Tensor | None
+    value: int
+    layer: int
+
+
+def feature_rows(t: Tensor) -> tuple[Tensor, int]:
+    """``t`` (``[..., channels]``) with its pixel stride in elements, copied only when its pixels
+    are not equally spaced rows of contiguous channels."""
+    channels = t.shape[-1]
+    if t.is_contiguous():
+        return t, channels
+    row = span = None
+    uniform = t.stride(-1) == 1 or channels == 1
+    for size, stride in zip(t.shape[-2::-1], t.stride()[-2::-1]):
+        if size == 1:
+            continue
+        if row is None:
+            row = stride
+            uniform = uniform and row >= channels
+        elif stride != span:
+            uniform = False
+        span = stride * size
+    if not uniform:
+        return t.contiguous(), channels
+    return t, channels if row is None else row
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_workspace_bytes(batch, pixels, channels, groups, dtype, backward) -> int:
+    return N.lib().dr_group_norm_workspace_bytes(batch, pixels, channels, groups, dtype, backward)
+
+
+def _param(t: Tensor | None, channels: int) -> tuple[int | None, int, int]:
+    """Pointer, type and rows of a group norm's weight or bias (contiguous, or None)."""
+    if t is None:
+        return None, 0, 1
+    return t.data_ptr(), N.FEATURE_DTYPES[t.dtype], t.numel() // channels
+
+
+@timed("group_norm_fwd")
+def group_norm_fwd(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None, eps: float,
+                   activation: int, drop: Drop) -> tuple[Tensor, Tensor]:
+    """``(y, stats)``: the normalised image and ``[2, batch, groups]`` means and reciprocal
+    standard deviations. ``x`` is ``[batch, ..., channels]`` and not empty."""
+    x, stride = feature_rows(x)
+    batch, channels = x.shape[0], x.shape[-1]
+    pixels = x.numel() // (batch * channels)
+    dtype = N.FEATURE_DTYPES[x.dtype]
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty((2, batch, groups), dtype=torch.float32, device=x.device)
+    work = _scratch(_norm_workspace_bytes(batch, pixels, channels, groups, dtype, 0), x.device)
+    mean = stats.data_ptr()
+    N.check(
+        N.lib().dr_group_norm_fwd(x.data_ptr(), stride, dtype, batch, pixels, channels, groups,
+                                  *_param(weight, channels), *_param(bias, channels), eps,
+                                  activation, drop.threshold, N.ptr(drop.seed), drop.value,
+                                  drop.layer, y.data_ptr(), mean, mean + 4 * batch * groups,
+                                  work.data_ptr(), work.numel(), N.stream(x.device)),
+        "dr_group_norm_fwd",
+    )  # fmt: skip
+    return y, stats
+
+
+@timed("group_norm_bwd")
+def group_norm_bwd(x: Tensor, grad_y: Tensor, groups: int, weight: Tensor | None,
+                   bias: Tensor | None, stats: Tensor, activation: int, drop: Drop,
+                   need: tuple[bool, bool, bool]) -> tuple[Tensor | None, ...]:
+    """Gradients of x (contiguous), weight and bias, None where not needed."""
+    x, stride = feature_rows(x)
+    grad_y, grad_stride = feature_rows(grad_y)
+    batch, channels = x.shape[0], x.shape[-1]
+    pixels = x.numel() // (batch * channels)
+    dtype = N.FEATURE_DTYPES[x.dtype]
+    grad_x = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
+    grad_w = torch.empty_like(weight) if need[1] else None
+    grad_b = torch.empty_like(bias) if need[2] else None
+    work = _scratch(_norm_workspace_bytes(batch, pixels, channels, groups, dtype, 1), x.device)
+    mean = stats.data_ptr()
+    N.check(
+        N.lib().dr_group_norm_bwd(x.data_ptr(), stride, grad_y.data_ptr(), grad_stride, dtype,
+                                  batch, pixels, channels, groups, *_param(weight, channels),
+                                  *_param(bias, channels), mean, mean + 4 * batch * groups,
+                                  activation, drop.threshold, N.ptr(drop.seed), drop.value,
+                                  drop.layer, N.ptr(grad_x), N.ptr(grad_w), N.ptr(grad_b),
+                                  work.data_ptr(), work.numel(), N.stream(x.device)),
+        "dr_group_norm_bwd",
+    )  # fmt: skip
+    return grad_x, grad_w, grad_b
+
+
+@timed("dropout")
+def dropout(x: Tensor, residual: Tensor | None, drop: Drop) -> Tensor:
+    """``residual + dropout(x)`` of contiguous tensors (also the gradient of x, without residual)."""
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    N.check(
+        N.lib().dr_dropout(x.data_ptr(), N.ptr(residual), x.numel(), N.FEATURE_DTYPES[x.dtype],
+                           drop.threshold, N.ptr(drop.seed), drop.value, drop.layer, y.data_ptr(),
+                           N.stream(x.device)),
+        "dr_dropout",
+    )  # fmt: skip
+    return y
+
+
 def capture_overflowed(device: torch.device) -> bool:
     """Whether a captured visibility pass on ``device`` exceeded its capacities since the last
     call (synchronizes); if so, the capacities for later captures are doubled."""

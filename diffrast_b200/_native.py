@@ -10,7 +10,17 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import (
+    POINTER,
+    c_char_p,
+    c_float,
+    c_int,
+    c_int32,
+    c_int64,
+    c_size_t,
+    c_uint32,
+    c_void_p,
+)
 from pathlib import Path
 
 import torch
@@ -25,6 +35,9 @@ LIBRARY = LIBDIR / ("libdiffrast_b200_checked.so" if CHECKED else "libdiffrast_b
 FILTER_MODES = ("nearest", "linear", "linear-mipmap-nearest", "linear-mipmap-linear")
 BOUNDARY_MODES = ("wrap", "clamp", "zero", "cube")
 MAX_LEVELS = 32
+# Element types and activations of the feature-image operators, in the C ABI's numbering.
+FEATURE_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+ACTIVATIONS = ("none", "relu", "silu")
 
 _P = c_void_p
 _SIGNATURES = {
@@ -143,6 +156,24 @@ _SIGNATURES = {
         c_int,
         [_P, _P, c_int64, _P, c_int64, c_float, c_int64, c_int32, c_int32, c_int32, _P, _P, _P,
          _P],
+    ),
+    "dr_dropout": (
+        c_int, [_P, _P, c_int64, c_int32, c_int32, _P, c_int64, c_uint32, _P, _P]
+    ),
+    "dr_group_norm_workspace_bytes": (
+        c_size_t, [c_int64, c_int64, c_int32, c_int32, c_int32, c_int32]
+    ),
+    "dr_group_norm_fwd": (
+        c_int,
+        [_P, c_int64, c_int32, c_int64, c_int64, c_int32, c_int32, _P, c_int32, c_int64, _P,
+         c_int32, c_int64, c_float, c_int32, c_int32, _P, c_int64, c_uint32, _P, _P, _P, _P,
+         c_size_t, _P],
+    ),
+    "dr_group_norm_bwd": (
+        c_int,
+        [_P, c_int64, _P, c_int64, c_int32, c_int64, c_int64, c_int32, c_int32, _P, c_int32,
+         c_int64, _P, c_int32, c_int64, _P, _P, c_int32, c_int32, _P, c_int64, c_uint32, _P, _P,
+         _P, _P, c_size_t, _P],
     ),
     "dr_zero": (c_int, [_P, c_size_t, _P]),
     "dr_checked_build": (c_int, []),

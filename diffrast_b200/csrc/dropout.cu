@@ -1,0 +1,117 @@
+// Dropout of a contiguous tensor, with an optional residual:
+//
+//   y = residual + (kept ? x * 65536 / (65536 - threshold) : 0)
+//
+// and its gradient, which is the same pass over the output's gradient without the residual: the
+// mask comes from philox.cuh again and is never stored.
+#include <cstdint>
+
+#include "philox.cuh"
+#include "vector.cuh"
+
+namespace dr {
+namespace {
+
+constexpr int kThreads = 256;
+
+// One thread for the eight elements of a counter: their loads are issued first, and the rounds of
+// the generator run while they are under way. `Wide` tensors are read and written in 16-byte
+// words; the others, whose address is not a multiple of 16, and the last elements one by one.
+template <typename T, bool Wide, bool Residual>
+__global__ void __launch_bounds__(kThreads) dropout_kernel(
+    const T* __restrict__ x, const T* __restrict__ residual, long long count, DropKey key,
+    T* __restrict__ y) {
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T));  // elements of a 16-byte word
+  constexpr int kWords = 8 / kPer;
+  const long long first = (blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x) * 8;
+  if (first >= count) return;
+  const unsigned long long seed = load_seed(key);
+  float v[8], r[8];
+  if (Wide && first + 8 <= count) {
+    uint4 a[kWords], b[kWords];
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      a[k] = __ldcs(reinterpret_cast<const uint4*>(x + first) + k);
+      if (Residual) b[k] = __ldcs(reinterpret_cast<const uint4*>(residual + first) + k);
+    }
+    float part[kPer];
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      unpack<T, kPer>(a[k], part);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) v[k * kPer + j] = part[j];
+      if (Residual) {
+        unpack<T, kPer>(b[k], part);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) r[k * kPer + j] = part[j];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = first + j < count ? to_float(x[first + j]) : 0.0f;
+      if (Residual) r[j] = first + j < count ? to_float(residual[first + j]) : 0.0f;
+    }
+  }
+  apply_dropout<8>(v, first, key, seed);
+  if (Residual) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += r[j];
+  }
+  if (Wide && first + 8 <= count) {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      float part[kPer];
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) part[j] = v[k * kPer + j];
+      __stcs(reinterpret_cast<uint4*>(y + first) + k, pack<T, kPer>(part));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (first + j < count) y[first + j] = from_float<T>(v[j]);
+  }
+}
+
+template <typename T>
+int run(const void* x, const void* residual, long long count, const DropKey& key, void* y,
+        cudaStream_t stream) {
+  const bool wide = aligned_to(x, 16) && aligned_to(y, 16) &&
+                    (residual == nullptr || aligned_to(residual, 16));
+  const unsigned int blocks = blocks_for((count + 7) / 8, kThreads);
+  auto launch = [&](auto kernel) {
+    kernel<<<blocks, kThreads, 0, stream>>>(static_cast<const T*>(x),
+                                            static_cast<const T*>(residual), count, key,
+                                            static_cast<T*>(y));
+  };
+  if (residual != nullptr)
+    wide ? launch(dropout_kernel<T, true, true>) : launch(dropout_kernel<T, false, true>);
+  else
+    wide ? launch(dropout_kernel<T, true, false>) : launch(dropout_kernel<T, false, false>);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace dr
+
+using namespace dr;
+
+extern "C" int dr_dropout(const void* x, const void* residual, int64_t count, int32_t dtype,
+                          int32_t threshold, const int64_t* seed, int64_t seed_value,
+                          uint32_t layer, void* y, void* stream) {
+  if (count < 0 || !known_dtype(dtype) || threshold < 0 || threshold > 65535)
+    return DR_ERR_INVALID_ARGUMENT;
+  if (count == 0) return DR_OK;
+  if (x == nullptr || y == nullptr) return DR_ERR_INVALID_ARGUMENT;
+  // One block for 2048 elements, at most 2^31 - 1 blocks.
+  if (count > 2048LL * 0x7FFFFFFF) return DR_ERR_TOO_LARGE;
+  const DropKey key = drop_key(seed, seed_value, layer, threshold);
+  switch (dtype) {
+    case DR_FLOAT32:
+      return run<float>(x, residual, count, key, y, as_stream(stream));
+    case DR_FLOAT16:
+      return run<__half>(x, residual, count, key, y, as_stream(stream));
+    default:
+      return run<__nv_bfloat16>(x, residual, count, key, y, as_stream(stream));
+  }
+}

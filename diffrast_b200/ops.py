@@ -18,6 +18,7 @@ from torch import Tensor
 
 from diffrast_b200 import _functions as F
 from diffrast_b200 import _kernels as K
+from diffrast_b200 import _native as N
 from diffrast_b200._cache import TensorCache
 from diffrast_b200.backends import require_cuda
 from diffrast_b200.context import RasterizeContext
@@ -25,12 +26,14 @@ from diffrast_b200.topology import TopologyHash, topology_for
 
 FilterMode = Literal["auto", "nearest", "linear", "linear-mipmap-nearest", "linear-mipmap-linear"]
 BoundaryMode = Literal["wrap", "clamp", "zero", "cube"]
+Activation = Literal["none", "relu", "silu"]
 FILTER_MODES = get_args(FilterMode)
 BOUNDARY_MODES = get_args(BoundaryMode)
 _MODE_INDEX = {name: i for i, name in enumerate(FILTER_MODES[1:])}
 _BOUNDARY_INDEX = {name: i for i, name in enumerate(BOUNDARY_MODES)}
 
 EMPTY_KEY = (1 << 63) - 1
+MAX_NORM_CHANNELS = 1 << 16
 
 
 # ---------------------------------------------------------------------------------------------
@@ -611,7 +614,7 @@ def antialias_construct_topology_hash(tri: Tensor) -> TopologyHash:
 
 
 # ---------------------------------------------------------------------------------------------
-# world-to-clip transform
+# shading and the world-to-clip transform
 # ---------------------------------------------------------------------------------------------
 
 
@@ -652,6 +655,179 @@ def lambert(color: Tensor, normal: Tensor, light_dir: Tensor, ambient: float = 0
     with torch.cuda.device(color.device):
         return F.Lambert.apply(color.contiguous(), normal, light.detach().contiguous(),
                                float(ambient))
+
+
+def group_norm(
+    x: Tensor,
+    groups: int,
+    weight: Tensor | None = None,
+    bias: Tensor | None = None,
+    *,
+    eps: float = 1e-5,
+    activation: Activation = "none",
+    dropout: float = 0.0,
+    seed: int | Tensor | None = None,
+    layer: int = 0,
+) -> Tensor:
+    """Group normalisation of a channels-last feature image, with the activation and dropout that
+    follow it in a learned shader, in one operator each way.
+
+    ``x`` is ``[batch, height, width, channels]`` (any ``[batch, ..., channels]``) in float32,
+    float16 or bfloat16, such as the features a :func:`texture` lookup samples; a channel slice of
+    a wider image (``out[..., 2:34]``) is read in place. Each view's channels are normalised in
+    ``groups`` runs of ``channels / groups`` over all its pixels (biased variance, ``eps`` added
+    to it), scaled by ``weight`` and shifted by ``bias`` (``[channels]``, or ``[batch, channels]``
+    for a modulation of each view; float32 or ``x``'s type; ``None`` for ones and zeros), passed
+    through ``activation`` (``"none"``, ``"relu"`` or ``"silu"``) and dropped out with probability
+    ``dropout`` as :func:`dropout` does with the same ``seed`` and ``layer``. Returns a contiguous
+    image of ``x``'s type. Statistics and sums are held in float32, and the same inputs give the
+    same bits, gradients included.
+
+    Differentiable in ``x``, ``weight`` and ``bias``; the backward pass computes activation and
+    mask again from ``x``. A group with NaN or infinite values is NaN throughout. Not part of
+    diffrast's API.
+    """
+    channels = _check_features(x, "x")
+    if isinstance(groups, bool) or not isinstance(groups, int):
+        raise TypeError(f"groups must be an int, got {groups!r}.")
+    if groups < 1 or channels % groups:
+        raise ValueError(f"groups must divide the {channels} channels of x, got {groups}.")
+    if channels > MAX_NORM_CHANNELS:
+        raise ValueError(f"group_norm takes at most {MAX_NORM_CHANNELS} channels, got {channels}.")
+    weight = _check_norm_param(weight, "weight", x)
+    bias = _check_norm_param(bias, "bias", x)
+    if activation not in N.ACTIVATIONS:
+        options = ", ".join(repr(a) for a in N.ACTIVATIONS)
+        raise ValueError(f"Unknown activation {activation!r}; expected one of {options}.")
+    if not isinstance(eps, SupportsFloat) or not 0.0 <= float(eps) < float("inf"):
+        raise ValueError(f"eps must be a finite number of at least 0, got {eps!r}.")
+    drop, seed = _check_dropout(dropout, seed, layer, x)
+    require_cuda(x.device)
+    args = (groups, float(eps), N.ACTIVATIONS.index(activation), drop)
+    if x.numel() == 0:
+        return _empty_like(x, weight, bias)
+    with torch.cuda.device(x.device):
+        if _wants_grad(x, weight, bias):
+            return F.GroupNorm.apply(x, weight, bias, seed, *args)
+        return K.group_norm_fwd(x, groups, weight, bias, *args[1:3], drop._replace(seed=seed))[0]
+
+
+def dropout(
+    x: Tensor,
+    p: float,
+    seed: int | Tensor,
+    *,
+    layer: int = 0,
+    residual: Tensor | None = None,
+) -> Tensor:
+    """Drop elements of ``x`` (float32, float16 or bfloat16, any shape) with probability ``p`` and
+    scale the others by the reciprocal of the probability to be kept, plus ``residual`` (``x``'s
+    shape and type) if given: the skip connection that dropout usually ends in.
+
+    The mask is a function of ``seed``, ``layer`` and the element's index in contiguous order
+    (Philox4x32-10), drawn again by the backward pass and never stored. ``seed`` is an int or a
+    CUDA int64 tensor of one element, which a training step captured in a CUDA graph changes
+    between replays; a seed tensor must not change between a forward pass and its backward pass.
+    Calls of one step are told apart by ``layer`` (below 2**32). ``p`` in ``[0, 1)`` is rounded to
+    a multiple of 2**-16 (at most 65535 of them), and the scale is that of the rounded
+    probability. A dropped element is 0 whatever its value. Differentiable in ``x`` and
+    ``residual``. Not part of diffrast's API.
+    """
+    _check_features(x, "x", ndim=0)
+    if seed is None:
+        raise TypeError("seed must be an int or an int64 tensor of one element, got None.")
+    drop, seed = _check_dropout(p, seed, layer, x, name="p")
+    if residual is not None:
+        if not isinstance(residual, Tensor):
+            raise TypeError(f"residual must be a torch.Tensor, got {type(residual).__name__}.")
+        if residual.dtype != x.dtype:
+            raise TypeError(f"residual must be {x.dtype} like x, got {residual.dtype}.")
+        if residual.shape != x.shape:
+            raise ValueError(
+                f"residual must match x, got {tuple(residual.shape)} and {tuple(x.shape)}."
+            )
+        _check_devices(x=x, residual=residual)
+    require_cuda(x.device)
+    if x.numel() == 0:
+        return _empty_like(x, residual)
+    x = x.contiguous()
+    residual = None if residual is None else residual.contiguous()
+    with torch.cuda.device(x.device):
+        if _wants_grad(x, residual):
+            return F.Dropout.apply(x, residual, seed, drop)
+        return K.dropout(x, residual, drop._replace(seed=seed))
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _empty_like(x: Tensor, *inputs) -> Tensor:
+    """The empty result of an operator of an empty ``x``, with a gradient (of zeros) to its
+    inputs."""
+    out = x.clone()
+    for t in inputs:
+        if t is not None:
+            out = out + 0.0 * t.sum().to(x.dtype)
+    return out
+
+
+def _check_features(x, name: str, ndim: int = 2) -> int:
+    """Validate a feature tensor; returns its channels (of a tensor with dimensions)."""
+    if not isinstance(x, Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(x).__name__}.")
+    if x.dtype not in N.FEATURE_DTYPES:
+        raise TypeError(f"{name} must be torch.float32, float16 or bfloat16, got {x.dtype}.")
+    if x.ndim < ndim:
+        raise ValueError(f"{name} must have shape [batch, ..., channels], got {tuple(x.shape)}.")
+    channels = x.shape[-1] if x.ndim else 1
+    if ndim and channels == 0:
+        raise ValueError(f"{name} must have channels, got shape {tuple(x.shape)}.")
+    return channels
+
+
+def _check_norm_param(t, name: str, x: Tensor) -> Tensor | None:
+    if t is None:
+        return None
+    if not isinstance(t, Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}.")
+    if t.dtype not in (torch.float32, x.dtype):
+        raise TypeError(f"{name} must be torch.float32 or {x.dtype} like x, got {t.dtype}.")
+    batch, channels = x.shape[0], x.shape[-1]
+    if tuple(t.shape) not in ((channels,), (batch, channels)):
+        raise ValueError(
+            f"{name} must have shape [channels] or [batch, channels], ({channels},) or "
+            f"({batch}, {channels}) here, got {tuple(t.shape)}."
+        )
+    _check_devices(**{"x": x, name: t})
+    return t.contiguous()
+
+
+def _check_dropout(p, seed, layer, x: Tensor, name: str = "dropout"):
+    """Validate dropout arguments; returns ``(drop, seed tensor)``, the :class:`K.Drop` without
+    its seed tensor."""
+    if isinstance(p, bool) or not isinstance(p, SupportsFloat) or not 0.0 <= float(p) < 1.0:
+        raise ValueError(f"{name} must be a probability in [0, 1), got {p!r}.")
+    if isinstance(layer, bool) or not isinstance(layer, int) or not 0 <= layer < 1 << 32:
+        raise ValueError(f"layer must be an int in [0, 2**32), got {layer!r}.")
+    threshold = min(65535, int(float(p) * 65536 + 0.5))
+    if isinstance(seed, Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1:
+            raise TypeError(
+                "seed must be an int or an int64 tensor of one element, got "
+                f"{seed.dtype} of shape {tuple(seed.shape)}."
+            )
+        _check_devices(x=x, seed=seed)
+        return K.Drop(threshold, None, 0, layer), seed
+    if seed is None:
+        if threshold:
+            raise ValueError("seed is required with dropout.")
+        return K.Drop(0, None, 0, layer), None
+    if isinstance(seed, bool) or not isinstance(seed, int):
+        raise TypeError(f"seed must be an int or an int64 tensor of one element, got {seed!r}.")
+    if not 0 <= seed < 1 << 63:
+        raise ValueError(f"seed must be in [0, 2**63), got {seed}.")
+    return K.Drop(threshold, None, seed, layer), None
 
 
 def to_clip(positions: Tensor, matrix: Tensor) -> Tensor:

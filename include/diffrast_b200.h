@@ -44,6 +44,14 @@ extern "C" {
 #define DR_BOUNDARY_CUBE 3
 /* Most mip levels a lookup may use (a 2**31-texel-wide texture has 32). */
 #define DR_MAX_LEVELS 32
+/* Element types of the feature-image operators (group norm, dropout). */
+#define DR_FLOAT32 0
+#define DR_FLOAT16 1
+#define DR_BFLOAT16 2
+/* Activations of dr_group_norm_fwd. */
+#define DR_ACTIVATION_NONE 0
+#define DR_ACTIVATION_RELU 1
+#define DR_ACTIVATION_SILU 2
 
 int dr_version(void);
 const char* dr_status_string(int status);
@@ -472,6 +480,57 @@ int dr_lambert_bwd(const float* color, const float* normal, int64_t normal_strid
                    const float* light, int64_t light_batch, float ambient, int64_t batch,
                    int32_t height, int32_t width, int32_t channels, const float* grad_out,
                    float* grad_color, float* grad_normal, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Feature images of a learned shader (no counterpart in the reference): group normalisation with
+ * an activation, and dropout. `dtype` is DR_FLOAT32, DR_FLOAT16 or DR_BFLOAT16; arithmetic,
+ * statistics and sums are float32 and results are rounded once.
+ *
+ * Dropout masks are functions of (seed, layer, element) and never stored: element e of an image
+ * (its index in contiguous order) takes 16 bits of the Philox4x32-10 block with key = seed and
+ * counter (e / 8 low, e / 8 high, layer, 0): bits 16 (e % 2) and up of word (e % 8) / 2. It is
+ * dropped (0, whatever its value) when they are below drop_threshold (0..65535; 0 drops nothing)
+ * and scaled by 65536 / (65536 - drop_threshold) otherwise. The seed is read from the device
+ * word `seed`, or is seed_value when seed is NULL.
+ * ------------------------------------------------------------------------------------------- */
+
+/* y = (residual, or 0 if NULL) + dropout(x), `count` contiguous elements each; y overlaps
+ * neither. The gradient of x is the same call on the output's gradient without the residual. */
+int dr_dropout(const void* x, const void* residual, int64_t count, int32_t dtype,
+               int32_t drop_threshold, const int64_t* seed, int64_t seed_value, uint32_t layer,
+               void* y, void* stream);
+
+/* Group normalisation of x [batch, pixels, channels], pixels x_stride elements apart (>= channels:
+ * a channel slice is read in place) and views pixels * x_stride: over each view's pixels and each
+ * run of channels / groups channels (groups divides channels, at most 65536),
+ *   y = dropout(act((x - mean) * rstd * weight + bias)),  rstd = 1 / sqrt(variance + eps).
+ * weight and bias have their own dtype and are [weight_batch, channels] with weight_batch 1 or
+ * batch, or NULL (ones, zeros). y [batch, pixels, channels] is contiguous; mean and rstd
+ * [batch, groups] are kept for the backward pass. workspace: dr_group_norm_workspace_bytes(...,
+ * backward 0). */
+size_t dr_group_norm_workspace_bytes(int64_t batch, int64_t pixels, int32_t channels,
+                                     int32_t groups, int32_t dtype, int32_t backward);
+int dr_group_norm_fwd(const void* x, int64_t x_stride, int32_t dtype, int64_t batch,
+                      int64_t pixels, int32_t channels, int32_t groups, const void* weight,
+                      int32_t weight_dtype, int64_t weight_batch, const void* bias,
+                      int32_t bias_dtype, int64_t bias_batch, float eps, int32_t activation,
+                      int32_t drop_threshold, const int64_t* seed, int64_t seed_value,
+                      uint32_t layer, void* y, float* mean, float* rstd, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* Gradients of dr_group_norm_fwd from grad_y (pixels grad_stride elements apart): grad_x
+ * (contiguous, dtype), grad_weight and grad_bias (shape and dtype of weight and bias; written,
+ * summed over views where those are shared). Any may be NULL. With batch or pixels 0 nothing is
+ * written. The same inputs give the same bits. workspace:
+ * dr_group_norm_workspace_bytes(..., backward 1). */
+int dr_group_norm_bwd(const void* x, int64_t x_stride, const void* grad_y, int64_t grad_stride,
+                      int32_t dtype, int64_t batch, int64_t pixels, int32_t channels,
+                      int32_t groups, const void* weight, int32_t weight_dtype,
+                      int64_t weight_batch, const void* bias, int32_t bias_dtype,
+                      int64_t bias_batch, const float* mean, const float* rstd,
+                      int32_t activation, int32_t drop_threshold, const int64_t* seed,
+                      int64_t seed_value, uint32_t layer, void* grad_x, void* grad_weight,
+                      void* grad_bias, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
