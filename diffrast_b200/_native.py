@@ -10,17 +10,7 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
-from ctypes import (
-    POINTER,
-    c_char_p,
-    c_float,
-    c_int,
-    c_int32,
-    c_int64,
-    c_size_t,
-    c_uint32,
-    c_void_p,
-)
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 import torch
@@ -158,7 +148,7 @@ _SIGNATURES = {
          _P],
     ),
     "dr_dropout": (
-        c_int, [_P, _P, c_int64, c_int32, c_int32, _P, c_int64, c_uint32, _P, _P]
+        c_int, [_P, _P, c_int64, c_int32, c_int32, _P, c_int64, c_int64, _P, _P]
     ),
     "dr_group_norm_workspace_bytes": (
         c_size_t, [c_int64, c_int64, c_int32, c_int32, c_int32, c_int32]
@@ -166,13 +156,13 @@ _SIGNATURES = {
     "dr_group_norm_fwd": (
         c_int,
         [_P, c_int64, c_int32, c_int64, c_int64, c_int32, c_int32, _P, c_int32, c_int64, _P,
-         c_int32, c_int64, c_float, c_int32, c_int32, _P, c_int64, c_uint32, _P, _P, _P, _P,
+         c_int32, c_int64, c_float, c_int32, c_int32, _P, c_int64, c_int64, _P, _P, _P, _P,
          c_size_t, _P],
     ),
     "dr_group_norm_bwd": (
         c_int,
         [_P, c_int64, _P, c_int64, c_int32, c_int64, c_int64, c_int32, c_int32, _P, c_int32,
-         c_int64, _P, c_int32, c_int64, _P, _P, c_int32, c_int32, _P, c_int64, c_uint32, _P, _P,
+         c_int64, _P, c_int32, c_int64, _P, _P, c_int32, c_int32, _P, c_int64, c_int64, _P, _P,
          _P, _P, c_size_t, _P],
     ),
     "dr_zero": (c_int, [_P, c_size_t, _P]),

@@ -98,8 +98,8 @@ using namespace dr;
 
 extern "C" int dr_dropout(const void* x, const void* residual, int64_t count, int32_t dtype,
                           int32_t threshold, const int64_t* seed, int64_t seed_value,
-                          uint32_t layer, void* y, void* stream) {
-  if (count < 0 || !known_dtype(dtype) || threshold < 0 || threshold > 65535)
+                          int64_t layer, void* y, void* stream) {
+  if (count < 0 || !known_dtype(dtype) || bad_drop(threshold, layer))
     return DR_ERR_INVALID_ARGUMENT;
   if (count == 0) return DR_OK;
   if (x == nullptr || y == nullptr) return DR_ERR_INVALID_ARGUMENT;

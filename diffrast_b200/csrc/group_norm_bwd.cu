@@ -273,13 +273,13 @@ extern "C" int dr_group_norm_bwd(const void* x, int64_t x_stride, const void* gr
                                  int32_t weight_dtype, int64_t weight_batch, const void* bias,
                                  int32_t bias_dtype, int64_t bias_batch, const float* mean,
                                  const float* rstd, int32_t activation, int32_t drop_threshold,
-                                 const int64_t* seed, int64_t seed_value, uint32_t layer,
+                                 const int64_t* seed, int64_t seed_value, int64_t layer,
                                  void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
                                  size_t workspace_bytes, void* stream) {
   if (bad_norm_sizes(batch, pixels, channels, groups, dtype) || x_stride < channels ||
       grad_stride < channels || bad_norm_param(weight, weight_dtype, weight_batch, batch) ||
       bad_norm_param(bias, bias_dtype, bias_batch, batch) || activation < DR_ACTIVATION_NONE ||
-      activation > DR_ACTIVATION_SILU || drop_threshold < 0 || drop_threshold > 65535 ||
+      activation > DR_ACTIVATION_SILU || bad_drop(drop_threshold, layer) ||
       (grad_weight != nullptr && weight == nullptr) || (grad_bias != nullptr && bias == nullptr))
     return DR_ERR_INVALID_ARGUMENT;
   if (batch == 0 || pixels == 0) return DR_OK;

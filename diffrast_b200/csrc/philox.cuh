@@ -20,17 +20,21 @@
 namespace dr {
 
 struct DropKey {
-  const long long* seed;    // one device word, or NULL
-  unsigned long long value; // the seed when `seed` is NULL
+  const long long* seed;     // one device word, or NULL
+  unsigned long long value;  // the seed when `seed` is NULL
   unsigned int layer;
-  unsigned int threshold;   // 0: nothing is dropped
+  unsigned int threshold;    // 0: nothing is dropped
   float scale;
 };
 
-inline DropKey drop_key(const int64_t* seed, int64_t seed_value, uint32_t layer,
+inline bool bad_drop(int32_t threshold, int64_t layer) {
+  return threshold < 0 || threshold > 65535 || layer < 0 || layer > 0xFFFFFFFFLL;
+}
+
+inline DropKey drop_key(const int64_t* seed, int64_t seed_value, int64_t layer,
                         int32_t threshold) {
   return {reinterpret_cast<const long long*>(seed), static_cast<unsigned long long>(seed_value),
-          layer, static_cast<unsigned int>(threshold),
+          static_cast<unsigned int>(layer), static_cast<unsigned int>(threshold),
           static_cast<float>(65536.0 / (65536 - threshold))};
 }
 

@@ -491,13 +491,13 @@ int dr_lambert_bwd(const float* color, const float* normal, int64_t normal_strid
  * counter (e / 8 low, e / 8 high, layer, 0): bits 16 (e % 2) and up of word (e % 8) / 2. It is
  * dropped (0, whatever its value) when they are below drop_threshold (0..65535; 0 drops nothing)
  * and scaled by 65536 / (65536 - drop_threshold) otherwise. The seed is read from the device
- * word `seed`, or is seed_value when seed is NULL.
+ * word `seed`, or is seed_value when seed is NULL; the layer is below 2^32.
  * ------------------------------------------------------------------------------------------- */
 
 /* y = (residual, or 0 if NULL) + dropout(x), `count` contiguous elements each; y overlaps
  * neither. The gradient of x is the same call on the output's gradient without the residual. */
 int dr_dropout(const void* x, const void* residual, int64_t count, int32_t dtype,
-               int32_t drop_threshold, const int64_t* seed, int64_t seed_value, uint32_t layer,
+               int32_t drop_threshold, const int64_t* seed, int64_t seed_value, int64_t layer,
                void* y, void* stream);
 
 /* Group normalisation of x [batch, pixels, channels], pixels x_stride elements apart (>= channels:
@@ -515,7 +515,7 @@ int dr_group_norm_fwd(const void* x, int64_t x_stride, int32_t dtype, int64_t ba
                       int32_t weight_dtype, int64_t weight_batch, const void* bias,
                       int32_t bias_dtype, int64_t bias_batch, float eps, int32_t activation,
                       int32_t drop_threshold, const int64_t* seed, int64_t seed_value,
-                      uint32_t layer, void* y, float* mean, float* rstd, void* workspace,
+                      int64_t layer, void* y, float* mean, float* rstd, void* workspace,
                       size_t workspace_bytes, void* stream);
 
 /* Gradients of dr_group_norm_fwd from grad_y (pixels grad_stride elements apart): grad_x
@@ -529,7 +529,7 @@ int dr_group_norm_bwd(const void* x, int64_t x_stride, const void* grad_y, int64
                       int64_t weight_batch, const void* bias, int32_t bias_dtype,
                       int64_t bias_batch, const float* mean, const float* rstd,
                       int32_t activation, int32_t drop_threshold, const int64_t* seed,
-                      int64_t seed_value, uint32_t layer, void* grad_x, void* grad_weight,
+                      int64_t seed_value, int64_t layer, void* grad_x, void* grad_weight,
                       void* grad_bias, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -109,7 +109,7 @@ def test_c_abi_refuses_before_any_cuda_call():
     bad, small = 10001, 10002
     common = [dict(dtype=3), dict(dtype=-1), dict(batch=-1), dict(pixels=-1), dict(channels=0),
               dict(groups=0), dict(groups=3), dict(x_stride=7), dict(act=3), dict(act=-1),
-              dict(drop=-1), dict(drop=65536), dict(w=16, wb=3), dict(b=16, bd=4), dict(x=None),
+              dict(drop=-1), dict(drop=65536), dict(layer=-1), dict(layer=1 << 32), dict(w=16, wb=3), dict(b=16, bd=4), dict(x=None),
               dict(mean=None), dict(rstd=None), dict(channels=1 << 17, x_stride=1 << 17)]
     for change in common + [dict(y=None)]:
         assert fwd(lib, **change) == bad, change
