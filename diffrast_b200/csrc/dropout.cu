@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(
   const long long first = (blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x) * 8;
   if (first >= count) return;
   const unsigned long long seed = load_seed(key);
-  float v[8], r[8];
+  Pairs<8> v, r;
   if (Wide && first + 8 <= count) {
     uint4 a[kWords], b[kWords];
 #pragma unroll
@@ -34,42 +34,41 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(
       a[k] = __ldcs(reinterpret_cast<const uint4*>(x + first) + k);
       if (Residual) b[k] = __ldcs(reinterpret_cast<const uint4*>(residual + first) + k);
     }
-    float part[kPer];
 #pragma unroll
     for (int k = 0; k < kWords; ++k) {
-      unpack<T, kPer>(a[k], part);
+      const Pairs<kPer> part = load_pairs<T, kPer>(a[k]);
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) v[k * kPer + j] = part[j];
+      for (int j = 0; j < kPer / 2; ++j) v.p[k * (kPer / 2) + j] = part.p[j];
       if (Residual) {
-        unpack<T, kPer>(b[k], part);
+        const Pairs<kPer> skip = load_pairs<T, kPer>(b[k]);
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) r[k * kPer + j] = part[j];
+        for (int j = 0; j < kPer / 2; ++j) r.p[k * (kPer / 2) + j] = skip.p[j];
       }
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      v[j] = first + j < count ? to_float(x[first + j]) : 0.0f;
-      if (Residual) r[j] = first + j < count ? to_float(residual[first + j]) : 0.0f;
+      v.set(j, first + j < count ? to_float(x[first + j]) : 0.0f);
+      if (Residual) r.set(j, first + j < count ? to_float(residual[first + j]) : 0.0f);
     }
   }
   apply_dropout<8>(v, first, key, seed);
   if (Residual) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] += r[j];
+    for (int j = 0; j < 4; ++j) v.p[j] = add2(v.p[j], r.p[j]);
   }
   if (Wide && first + 8 <= count) {
 #pragma unroll
     for (int k = 0; k < kWords; ++k) {
-      float part[kPer];
+      Pairs<kPer> part;
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) part[j] = v[k * kPer + j];
-      __stcs(reinterpret_cast<uint4*>(y + first) + k, pack<T, kPer>(part));
+      for (int j = 0; j < kPer / 2; ++j) part.p[j] = v.p[k * (kPer / 2) + j];
+      __stcs(reinterpret_cast<uint4*>(y + first) + k, pack_pairs<T, kPer>(part));
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (first + j < count) y[first + j] = from_float<T>(v[j]);
+      if (first + j < count) y[first + j] = from_float<T>(v.get(j));
   }
 }
 

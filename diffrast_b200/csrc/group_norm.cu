@@ -5,170 +5,292 @@
 namespace dr {
 namespace {
 
-constexpr int kUnroll = 4;  // vectors a thread has under way
-
-// Reads the rows first, first + step, ... below `end` of a column of vectors, kUnroll of them at a
-// time, and gives each to `use(vector, row)`.
-template <typename T, int V, typename Use>
+// Reads the rows first, first + step, ... below `end` of a column of vectors, kNormUnroll of them
+// at a time, and gives each to `use(vector)` in order. `Last`: nothing will read them again.
+template <typename T, int V, bool Last, typename Use>
 __device__ __forceinline__ void for_rows(const T* __restrict__ x, long long stride, int first,
                                          int step, int end, Use use) {
   using P = Packed<T, V>;
-  for (int row = first; row < end; row += kUnroll * step) {
-    P p[kUnroll];
+  auto load = [](const T* at) {
+    return Last ? __ldcs(reinterpret_cast<const P*>(at)) : *reinterpret_cast<const P*>(at);
+  };
+  x += first * stride;
+  stride *= step;
+  int left = end - first;
+  for (; left > (kNormUnroll - 1) * step; left -= kNormUnroll * step) {
+    P p[kNormUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (row + u * step < end)
-        p[u] = *reinterpret_cast<const P*>(x + (row + u * step) * stride);
+    for (int u = 0; u < kNormUnroll; ++u) {
+      p[u] = load(x);
+      x += stride;
+    }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (row + u * step < end) use(p[u], row + u * step);
+    for (int u = 0; u < kNormUnroll; ++u) use(load_pairs<T, V>(p[u]));
+  }
+  if (left > 0) {
+    P p[kNormUnroll - 1];
+#pragma unroll
+    for (int u = 0; u < kNormUnroll - 1; ++u)
+      if (left > u * step) p[u] = load(x + u * stride);
+#pragma unroll
+    for (int u = 0; u < kNormUnroll - 1; ++u)
+      if (left > u * step) use(load_pairs<T, V>(p[u]));
   }
 }
 
-// Statistics of one chunk of rows in one tile of columns: per-thread moments per channel, joined
-// over the block's rows, then over the channels (and folded pixels) of each group.
-// parts [batch][groups][chunks * group_tiles] of (mean, squared deviations).
-template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads) norm_stats_kernel(const T* __restrict__ x,
-                                                                  NormShape s,
-                                                                  float2* __restrict__ parts) {
+// Joins the threads' moments of a block's rows into those of the tile's groups: within a thread
+// over the neighbouring channels of a group, then over the rows, then over a group's columns (and
+// folded pixels).
+template <int V, typename Done>
+__device__ __forceinline__ void join_block(Moments<V>& moments, const TileThread& t,
+                                           const NormShape& s, const NormTile& tile, int rows,
+                                           Done done) {
   __shared__ float2 entry[kNormThreads * V];
-  __shared__ float2 channel[kNormThreads * V];
-  long long block = blockIdx.x;
-  const int chunk = static_cast<int>(block % s.chunks);
-  block /= s.chunks;
-  const int tile_index = static_cast<int>(block % s.tiles);
-  const long long view = block / s.tiles;
-  const NormTile tile = norm_tile(s, V, tile_index);
-  const int lanes = kNormThreads / tile.cols;
-  const int col = threadIdx.x % tile.cols, lane = threadIdx.x / tile.cols;
-  const long long row0 = chunk * s.chunk_rows;
-  const int rows = static_cast<int>(min(s.chunk_rows, s.rows - row0));
-  const int width = tile.cols * V;
-  if (lane < lanes) {
-    Moments<V> moments;
-    const T* base = x + (view * s.rows + row0) * s.x_row + (tile.col + col) * V;
-    for_rows<T, V>(base, s.x_row, lane, lanes, rows, [&](const Packed<T, V>& p, int) {
-      float v[V];
-      unpack<T, V>(p, v);
+  __shared__ float2 column[kNormThreads * V / 2];
+  __shared__ float counts[kNormThreads];  // rows of each line of entries
+  const int d = s.group_channels;
+  // Channels folded within a thread: all that its vector has of a group, where vectors do not
+  // straddle groups.
+  int q = d % V == 0 ? V : V % d == 0 ? d : 1;
+  const int per = V / q, width = tile.cols * per;
+  const int mine = t.active && t.lane < rows ? (rows - t.lane + t.lanes - 1) / t.lanes : 0;
+  int lines = t.lanes, line = t.lane;
+  bool write = t.active;
+  float n = static_cast<float>(mine);
+  if (tile.cols < 32 && 32 % tile.cols == 0) {
+    // A tile's columns divide the warp: its rows are joined first.
+    moments.move_pivot(threadIdx.x % tile.cols, n);
+    for (int d = tile.cols; d < 32; d *= 2) {
+      moments.add_lane(d);
+      n += __shfl_xor_sync(0xFFFFFFFFu, n, d);
+    }
+    lines = kNormThreads / 32;
+    line = threadIdx.x / 32;
+    write = threadIdx.x % 32 < tile.cols;
+  }
+  if (write && t.col == 0) counts[line] = n;
+  if (write) {
+    const float inverse = n > 0.0f ? 1.0f / n : 0.0f;
+    float2* to = entry + (line * tile.cols + t.col) * per;
+    auto fold = [&](auto count) {
+      constexpr int Q = decltype(count)::value;
+#pragma unroll
+      for (int j = 0; j < V / Q; ++j)
+        to[j] = n > 0.0f ? fold_channels<Q>(moments, j * Q, n, inverse) : both(0.0f);
+    };
+    if (q == V) {
+      fold(std::integral_constant<int, V>());
+    } else if constexpr (V > 1) {
+      if (q == 1) fold(std::integral_constant<int, 1>());
+      if constexpr (V > 2) {
+        if (q == 2) fold(std::integral_constant<int, 2>());
+      }
+      if constexpr (V > 4) {
+        if (q == 4) fold(std::integral_constant<int, 4>());
+      }
+    }
+  }
+  __syncthreads();
+  const int members = (s.pieces > 1 ? tile.cols * V : s.fold * d) / q;  // columns of a group
+  const float weight = static_cast<float>(q);
+  if (members == 1) {
+    join_moments(
+        width, lines,
+        [&](int item, int i, float2& v) {
+          v = entry[i * width + item];
+          return weight * counts[i];
+        },
+        done);
+    return;
+  }
+  const float2* from = entry;
+  if (lines > 1) {
+    join_moments(
+        width, lines,
+        [&](int item, int i, float2& v) {
+          v = entry[i * width + item];
+          return weight * counts[i];
+        },
+        [&](int item, float mean, float squares) { column[item] = make_float2(mean, squares); });
+    __syncthreads();
+    from = column;
+  }
+  const int span = s.fold > 1 ? d / q : members;  // neighbouring columns of a group
+  join_moments(
+      tile.groups, members,
+      [&](int item, int i, float2& v) {
+        const int f = s.fold > 1 ? i / span : 0;
+        v = from[f * (s.channels / q) + item * span + i - f * span];
+        return weight * static_cast<float>(rows);
+      },
+      done);
+}
+
+// First pass: the statistics of one chunk of rows in one tile of columns.
+// parts [batch][groups][pieces][chunks].
+template <typename T, int V>
+__global__ void __launch_bounds__(kNormThreads, 4) norm_stats_kernel(const T* __restrict__ x,
+                                                                     NormShape s, int view0,
+                                                                     float2* __restrict__ parts) {
+  let_next_kernel_start();
+  const NormBlock b = norm_block(s, V, view0, blockIdx.x);
+  const TileThread t(b.tile.cols);
+  Moments<V> moments;
+  bool first = true;
+#pragma unroll
+  for (int j = 0; j < Pairs<V>::kCount; ++j)
+    moments.pivot.p[j] = moments.sum.p[j] = moments.square.p[j] = both(0.0f);
+  if (t.active)
+    for_rows<T, V, false>(x + b.first * s.x_row + (b.tile.col + t.col) * V, s.x_row, t.lane,
+                          t.lanes, b.rows, [&](const Pairs<V>& v) {
+      if (first) moments.start(v);
+      first = false;
       moments.add(v);
     });
-#pragma unroll
-    for (int j = 0; j < V; ++j) entry[lane * width + col * V + j] = moments.get(j);
-  }
-  __syncthreads();
-  join_moments(
-      width, lanes, kNormThreads,
-      [&](int item, int i, float2& v) {
-        v = entry[i * width + item];
-        return static_cast<float>((rows - i + lanes - 1) / lanes);
-      },
-      [&](int item, float mean, float squares) { channel[item] = make_float2(mean, squares); });
-  __syncthreads();
-  const int d = s.group_tiles > 1 ? width : s.group_channels;
-  const int part_count = s.chunks * s.group_tiles;
-  join_moments(
-      tile.groups, s.fold * d, kNormThreads,
-      [&](int item, int i, float2& v) {
-        const int f = i / d;
-        v = channel[f * s.channels + item * d + i - f * d];
-        return static_cast<float>(rows);
-      },
-      [&](int item, float mean, float squares) {
-        const long long at = (view * s.groups + tile.group + item) * part_count;
-        const int piece = s.group_tiles > 1 ? tile_index % s.group_tiles : 0;
-        parts[at + chunk * s.group_tiles + piece] = make_float2(mean, squares);
-      });
+  join_block<V>(moments, t, s, b.tile, b.rows, [&](int item, float mean, float squares) {
+    const long long group = static_cast<long long>(b.view) * s.groups + b.tile.group + item;
+    parts[(group * s.pieces + b.piece) * s.chunks + b.chunk] = make_float2(mean, squares);
+  });
+  wait_for_kernel_before();
 }
 
-// Joins the chunks' statistics: one warp for each view and group.
+// Sums over a block, for all of its threads.
+__device__ __forceinline__ float block_sum(float v, float* shared) {
+  v = lane_sum(v, 32);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = v;
+  __syncthreads();
+  float total = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kNormThreads / 32; ++i) total += shared[i];
+  return total;
+}
+
+// Joins the parts of one view and group: kJoin of them for each thread at a time, kept in registers
+// between the sum that gives their mean and the sum of squares about it; then with those before.
+constexpr int kJoin = 4;
+
 template <int V>
-__global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const float2* __restrict__ parts,
-                                                                 NormShape s, float eps,
+__global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const float2* parts,
+                                                                 NormShape s, int view0, float eps,
                                                                  float* __restrict__ mean,
                                                                  float* __restrict__ rstd) {
-  constexpr int kWarps = kNormThreads / 32;
-  const long long first = blockIdx.x * static_cast<long long>(kWarps);
-  const long long total = s.batch * s.groups;
-  const int part_count = s.chunks * s.group_tiles;
-  join_moments(
-      static_cast<int>(min(static_cast<long long>(kWarps), total - first)), part_count, kNormThreads,
-      [&](int item, int i, float2& v) {
-        v = parts[(first + item) * part_count + i];
-        const int chunk = i / s.group_tiles, piece = i - chunk * s.group_tiles;
-        const int rows = static_cast<int>(min(s.chunk_rows, s.rows - chunk * s.chunk_rows));
-        const int width = s.group_tiles > 1 ? min(s.tile_cols, s.group_cols - piece * s.tile_cols) * V
-                                            : s.group_channels * s.fold;
-        return static_cast<float>(rows) * static_cast<float>(width);
-      },
-      [&](int item, float m, float squares) {
-        const float count = static_cast<float>(s.pixels) * static_cast<float>(s.group_channels);
-        mean[first + item] = m;
-        rstd[first + item] = rsqrtf(variance_of(m, squares, count) + eps);
-      });
+  __shared__ float shared[kNormThreads / 32];
+  let_next_kernel_start();
+  wait_for_kernel_before();
+  const long long group = static_cast<long long>(view0) * s.groups + blockIdx.x;
+  const int count = s.pieces * s.chunks;
+  parts += group * count;
+  const float2 pivot = parts[0];
+  float all = 0.0f, all_mean = 0.0f, all_squares = 0.0f;
+  for (int base = 0; base < count; base += kJoin * kNormThreads) {
+    float2 v[kJoin];
+    float n[kJoin];
+    float total_n = 0.0f, total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kJoin; ++k) {
+      const int i = base + k * kNormThreads + threadIdx.x;
+      v[k] = pivot;
+      n[k] = 0.0f;
+      if (i < count) {
+        v[k] = parts[i];
+        const int piece = s.pieces > 1 ? i / s.chunks : 0, chunk = i - piece * s.chunks;
+        const long long rows = min(static_cast<long long>(s.chunk_rows),
+                                   s.rows - static_cast<long long>(chunk) * s.chunk_rows);
+        const int width = s.pieces > 1
+                              ? min(s.tile_cols, s.group_cols - piece * s.tile_cols) * V
+                              : s.group_channels * s.fold;
+        n[k] = static_cast<float>(rows) * static_cast<float>(width);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kJoin; ++k) {
+      total_n += n[k];
+      total = fmaf(n[k], v[k].x - pivot.x, total);
+    }
+    total_n = block_sum(total_n, shared);
+    total = block_sum(total, shared);
+    const float m = total / total_n;  // about the pivot
+    float squares = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kJoin; ++k) {
+      const float d = v[k].x - pivot.x - m;
+      squares += n[k] > 0.0f ? fmaf(n[k] * d, d, v[k].y) : 0.0f;
+    }
+    squares = block_sum(squares, shared);
+    const float sum_n = all + total_n, d = m - all_mean;
+    all_squares += squares + d * d * (all * (total_n / sum_n));
+    all_mean += d * (total_n / sum_n);
+    all = sum_n;
+  }
+  if (threadIdx.x == 0) {
+    const float m = pivot.x + all_mean;
+    const float values = static_cast<float>(s.pixels) * static_cast<float>(s.group_channels);
+    mean[group] = m;
+    rstd[group] = rsqrtf(variance_of(m, all_squares, values) + eps);
+  }
 }
 
-// Normalise, scale, activate and drop: one chunk of rows in one tile of columns.
+// Second pass: normalise, scale, activate and drop one chunk of rows in one tile of columns. Blocks
+// run from the end of the views to their start: what the first pass read last is still in L2.
 template <typename T, int V, bool Silu, bool Drop>
-__global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(
-    const T* __restrict__ x, NormShape s, NormParam weight, NormParam bias, float bound,
-    DropKey key, const float* __restrict__ mean, const float* __restrict__ rstd,
-    T* __restrict__ y) {
-  long long block = blockIdx.x;
-  const int chunk = static_cast<int>(block % s.chunks);
-  block /= s.chunks;
-  const NormTile tile = norm_tile(s, V, static_cast<int>(block % s.tiles));
-  const long long view = block / s.tiles;
-  const int lanes = kNormThreads / tile.cols;
-  const int col = threadIdx.x % tile.cols, lane = threadIdx.x / tile.cols;
-  if (lane >= lanes) return;
-  const long long row0 = chunk * s.chunk_rows;
-  const int rows = static_cast<int>(min(s.chunk_rows, s.rows - row0));
-  float m[V], a[V], b[V];
+__global__ void __launch_bounds__(kNormThreads, 4) norm_apply_kernel(
+    const T* __restrict__ x, NormShape s, int view0, NormParam weight, NormParam bias, float bound,
+    DropKey key, const float* mean, const float* rstd, T* __restrict__ y) {
+  let_next_kernel_start();
+  const NormBlock b = norm_block(s, V, view0, gridDim.x - 1 - blockIdx.x);
+  const TileThread t(b.tile.cols);
+  wait_for_kernel_before();
+  if (!t.active) return;
+  const int col = (b.tile.col + t.col) * V;
+  Pairs<V> m, a, c;  // z = (x + m) a + c
+  if (V == 1) m.p[0].y = a.p[0].y = c.p[0].y = 0.0f;
+  ChannelWalk walk(s, col);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int c = ((tile.col + col) * V + j) % s.channels;
-    const long long group = view * s.groups + c / s.group_channels;
-    const float w = weight.data ? load_param(weight.data, weight.dtype, view * weight.view + c) : 1.0f;
-    m[j] = mean[group];
-    a[j] = rstd[group] * w;
-    b[j] = bias.data ? load_param(bias.data, bias.dtype, view * bias.view + c) : 0.0f;
+    const long long group = static_cast<long long>(b.view) * s.groups + walk.group;
+    m.set(j, -mean[group]);
+    a.set(j, rstd[group] * load_scale(weight, b.view, walk.channel));
+    c.set(j, load_shift(bias, b.view, walk.channel));
+    walk.next();
   }
   const unsigned long long seed = Drop ? load_seed(key) : 0;
   const long long out_row = static_cast<long long>(s.channels) * s.fold;
-  const long long offset = (view * s.rows + row0) * out_row + (tile.col + col) * V;
-  const T* base = x + (view * s.rows + row0) * s.x_row + (tile.col + col) * V;
-  for_rows<T, V>(base, s.x_row, lane, lanes, rows, [&](const Packed<T, V>& p, int row) {
-    float v[V];
-    unpack<T, V>(p, v);
+  long long at = (b.first + t.lane) * out_row + col;
+  const long long step = t.lanes * out_row;
+  for_rows<T, V, true>(x + b.first * s.x_row + col, s.x_row, t.lane, t.lanes, b.rows,
+                       [&](const Pairs<V>& v) {
+    Pairs<V> z;
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = activate<Silu>(fmaf(v[j] - m[j], a[j], b[j]), bound);
-    const long long at = offset + row * out_row;
-    if (Drop) apply_dropout<V>(v, at, key, seed);
-    *reinterpret_cast<Packed<T, V>*>(y + at) = pack<T, V>(v);
+    for (int j = 0; j < Pairs<V>::kCount; ++j)
+      z.p[j] = activate<Silu>(fma2(add2(v.p[j], m.p[j]), a.p[j], c.p[j]), bound);
+    if (Drop) apply_dropout<V>(z, at, key, seed);
+    __stcs(reinterpret_cast<Packed<T, V>*>(y + at), pack_pairs<T, V>(z));
+    at += step;
   });
 }
 
-template <typename T, int V>
-int run(const void* x, const NormShape& s, const NormParam& weight, const NormParam& bias,
-        float eps, int activation, const DropKey& key, void* y, float* mean, float* rstd,
-        float2* parts, cudaStream_t stream) {
+template <typename T, int V, bool Silu, bool Drop>
+int passes(const void* x, const NormShape& s, int dtype, const NormParam& weight,
+           const NormParam& bias, float eps, float bound, const DropKey& key, void* y, float* mean,
+           float* rstd, float2* parts, cudaStream_t stream) {
   const T* in = static_cast<const T*>(x);
   T* out = static_cast<T*>(y);
-  const unsigned int blocks = static_cast<unsigned int>(s.batch * s.tiles * s.chunks);
-  norm_stats_kernel<T, V><<<blocks, kNormThreads, 0, stream>>>(in, s, parts);
-  norm_join_kernel<V><<<blocks_for(s.batch * s.groups, kNormThreads / 32), kNormThreads, 0,
-                        stream>>>(parts, s, eps, mean, rstd);
-  const float bound = norm_bound(activation);
-  auto launch = [&](auto kernel) {
-    kernel<<<blocks, kNormThreads, 0, stream>>>(in, s, weight, bias, bound, key, mean, rstd, out);
-  };
-  const bool drop = key.threshold != 0;
-  if (activation == DR_ACTIVATION_SILU)
-    drop ? launch(norm_apply_kernel<T, V, true, true>) : launch(norm_apply_kernel<T, V, true, false>);
-  else
-    drop ? launch(norm_apply_kernel<T, V, false, true>)
-         : launch(norm_apply_kernel<T, V, false, false>);
+  const int most = views_at_once(s, dtype, 1);
+  for (int view0 = 0; view0 < s.batch; view0 += most) {
+    const int views = static_cast<int>(std::min<long long>(most, s.batch - view0));
+    const unsigned int blocks = static_cast<unsigned int>(views) * s.tiles * s.chunks;
+    const unsigned int groups = static_cast<unsigned int>(views) * s.groups;
+    cudaError_t err = launch_kernel(norm_stats_kernel<T, V>, blocks, kNormThreads, stream,
+                                    view0 > 0, in, s, view0, parts);
+    if (err == cudaSuccess)
+      err = launch_kernel(norm_join_kernel<V>, groups, kNormThreads, stream, true, parts, s, view0,
+                          eps, mean, rstd);
+    if (err == cudaSuccess)
+      err = launch_kernel(norm_apply_kernel<T, V, Silu, Drop>, blocks, kNormThreads, stream, true,
+                          in, s, view0, weight, bias, bound, key, mean, rstd, out);
+    if (err != cudaSuccess) return static_cast<int>(err);
+  }
   return launch_status();
 }
 
@@ -201,17 +323,19 @@ extern "C" int dr_group_norm_fwd(const void* x, int64_t x_stride, int32_t dtype,
     return DR_ERR_INVALID_ARGUMENT;
   NormShape s;
   NormVector v = choose_vector(pixels, channels, dtype, x_stride, channels, {x, y});
-  if (!cut_norm(s, v, batch, pixels, channels, groups, dtype, x_stride, channels,
-                norm_chunk_bytes(batch, pixels, channels, dtype)))
+  if (batch > kMaxNormBlocks ||
+      !plan_passes(s, v, batch, pixels, channels, groups, dtype, x_stride, channels))
     return DR_ERR_TOO_LARGE;
-  if (workspace == nullptr || workspace_bytes < norm_forward_bytes(s))
+  if (workspace == nullptr || workspace_bytes < norm_space(s, false).total)
     return DR_ERR_WORKSPACE_TOO_SMALL;
   const NormParam w{weight, weight_dtype, weight_batch > 1 ? channels : 0};
   const NormParam b{bias, bias_dtype, bias_batch > 1 ? channels : 0};
   const DropKey key = drop_key(seed, seed_value, layer, drop_threshold);
-  auto* parts = static_cast<float2*>(workspace);
-  return with_vector(dtype, v.vec, [&](auto type, auto width) {
-    return run<typename decltype(type)::type, decltype(width)::value>(
-        x, s, w, b, eps, activation, key, y, mean, rstd, parts, as_stream(stream));
+  const float bound = norm_bound(activation);
+  return with_variant(dtype, v.vec, activation, drop_threshold, [&](auto k) {
+    using K = decltype(k);
+    return passes<typename K::Type, K::kVec, K::kSilu, K::kDrop>(
+        x, s, dtype, w, b, eps, bound, key, y, mean, rstd, static_cast<float2*>(workspace),
+        as_stream(stream));
   });
 }

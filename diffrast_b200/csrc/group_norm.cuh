@@ -28,7 +28,7 @@ namespace dr {
 
 constexpr int kNormThreads = 256;
 
-// How the views are cut up (made by plan_norm).
+// How the views are cut up (made by cut_norm).
 struct NormShape {
   long long batch;
   long long rows;       // rows of a view: pixels / fold
@@ -37,10 +37,10 @@ struct NormShape {
   int fold;
   int cols;             // vectors in a row
   int tile_cols;        // vectors in a tile of columns (the last tile may have fewer)
-  int tiles;            // tiles in a row
-  int group_tiles;      // tiles a group is cut into (1: tiles hold whole groups)
-  int group_cols;       // vectors of a group that is cut into tiles
-  long long chunk_rows; // rows of one block's work
+  int tiles;            // of a row; whole groups each, unless groups are cut
+  int pieces;           // tiles that a group is cut into, or 1
+  int group_cols;       // vectors of a group that is cut
+  int chunk_rows;       // rows of one block's work
   int chunks;           // of a view
   // Elements between the rows of x and of the output's gradient.
   long long x_row, grad_row;
@@ -53,34 +53,73 @@ struct NormParam {
 };
 
 struct NormTile {
-  int col, cols;       // first vector and vectors
-  int group, groups;   // first group and groups (partly covered when groups are cut)
+  int col, cols;      // first vector and vectors
+  int group, groups;  // first group and groups (the one group when it is cut)
 };
 
-__host__ __device__ inline NormTile norm_tile(const NormShape& s, int vec, int tile) {
-  NormTile t;
-  if (s.group_tiles > 1) {
-    const int g = tile / s.group_tiles, part = tile - g * s.group_tiles;
-    t.col = g * s.group_cols + part * s.tile_cols;
-    t.cols = min(s.tile_cols, s.group_cols - part * s.tile_cols);
-    t.group = g, t.groups = 1;
+// Work of one block: a chunk of rows in a tile of columns.
+struct NormBlock {
+  int view, chunk, piece;
+  NormTile tile;
+  int rows;
+  long long first;  // first row, counted over the views
+};
+
+__device__ __forceinline__ NormBlock norm_block(const NormShape& s, int vec, int view0,
+                                                unsigned int index) {
+  NormBlock b;
+  const unsigned int rest = index / s.chunks;
+  b.chunk = static_cast<int>(index - rest * s.chunks);
+  const unsigned int view = rest / s.tiles;
+  const int tile = static_cast<int>(rest - view * s.tiles);
+  b.view = view0 + static_cast<int>(view);
+  b.piece = 0;
+  if (s.pieces > 1) {
+    b.tile.group = tile / s.pieces;
+    b.piece = tile - b.tile.group * s.pieces;
+    b.tile.col = b.tile.group * s.group_cols + b.piece * s.tile_cols;
+    b.tile.cols = min(s.tile_cols, s.group_cols - b.piece * s.tile_cols);
+    b.tile.groups = 1;
   } else {
-    t.col = tile * s.tile_cols;
-    t.cols = min(s.tile_cols, s.cols - t.col);
-    if (s.fold > 1) {
-      t.group = 0, t.groups = s.groups;
-    } else {
-      t.group = t.col * vec / s.group_channels;
-      t.groups = t.cols * vec / s.group_channels;
-    }
+    b.tile.col = tile * s.tile_cols;
+    b.tile.cols = min(s.tile_cols, s.cols - b.tile.col);
+    b.tile.group = s.fold > 1 ? 0 : b.tile.col * vec / s.group_channels;
+    b.tile.groups = s.fold > 1 ? s.groups : b.tile.cols * vec / s.group_channels;
   }
-  return t;
+  const long long row0 = static_cast<long long>(b.chunk) * s.chunk_rows;
+  b.rows = static_cast<int>(min(static_cast<long long>(s.chunk_rows), s.rows - row0));
+  b.first = b.view * s.rows + row0;
+  return b;
 }
+
+// The channels of a thread's vector one after the other, with their groups: one division for all.
+struct ChannelWalk {
+  int channel, group, rest, channels, size;
+
+  __device__ __forceinline__ ChannelWalk(const NormShape& s, int first)
+      : channels(s.channels), size(s.group_channels) {
+    channel = s.fold > 1 ? first % channels : first;
+    group = channel / size;
+    rest = channel - group * size;
+  }
+  __device__ __forceinline__ void next() {
+    ++channel;
+    if (++rest == size) rest = 0, ++group;
+    if (channel == channels) channel = 0, group = 0;
+  }
+};
 
 __device__ __forceinline__ float load_param(const void* data, int dtype, long long i) {
   if (dtype == DR_FLOAT32) return __ldg(static_cast<const float*>(data) + i);
   if (dtype == DR_FLOAT16) return __half2float(__ldg(static_cast<const __half*>(data) + i));
   return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(data) + i));
+}
+
+__device__ __forceinline__ float load_scale(const NormParam& w, long long view, int channel) {
+  return w.data ? load_param(w.data, w.dtype, view * w.view + channel) : 1.0f;
+}
+__device__ __forceinline__ float load_shift(const NormParam& b, long long view, int channel) {
+  return b.data ? load_param(b.data, b.dtype, view * b.view + channel) : 0.0f;
 }
 
 __device__ __forceinline__ void store_param(void* data, int dtype, long long i, float v) {
@@ -92,65 +131,129 @@ __device__ __forceinline__ void store_param(void* data, int dtype, long long i, 
     static_cast<__nv_bfloat16*>(data)[i] = __float2bfloat16_rn(v);
 }
 
-// 1 / (1 + exp(-z)), from the hardware's exponential and reciprocal (each within two units in the
-// last place of float32). For z below -88 the exponential is infinite and the result 0.
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// 1 / (1 + exp(-z)), from the hardware's exponential (of 2) and reciprocal, each within two units
+// in the last place of float32. For z below -88 the exponential is infinite and the result 0.
+__device__ __forceinline__ float2 sigmoid2(float2 z) {
+  const float2 t = mul2(z, both(-1.4426950408889634f));
+  float2 e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  e = add2(e, both(1.0f));
+  float2 s;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(e.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(e.y));
+  return s;
+}
 
 // The activations: SiLU, or a clamp from below that is the identity with bound -infinity and ReLU
 // with bound 0. The comparisons are written so that NaN passes, as it does through both.
 template <bool Silu>
-__device__ __forceinline__ float activate(float z, float bound) {
-  if (Silu) return z * sigmoid(z);
-  return z <= bound ? bound : z;
+__device__ __forceinline__ float2 activate(float2 z, float bound) {
+  if (Silu) return mul2(z, sigmoid2(z));
+  return make_float2(z.x <= bound ? bound : z.x, z.y <= bound ? bound : z.y);
 }
 
-// The derivative at z: s (1 + z (1 - s)) for SiLU. ReLU's is 0 at 0.
+// q times the derivative at z: s (1 + z (1 - s)) for SiLU. ReLU's is 0 at 0.
 template <bool Silu>
-__device__ __forceinline__ float activate_grad(float z, float bound) {
+__device__ __forceinline__ float2 activate_grad(float2 q, float2 z, float bound) {
   if (Silu) {
-    const float s = sigmoid(z);
-    return s * fmaf(z, 1.0f - s, 1.0f);
+    const float2 s = sigmoid2(z);
+    const float2 t = fma2(make_float2(-s.x, -s.y), z, z);
+    return mul2(q, fma2(s, t, s));
   }
-  return z <= bound ? 0.0f : 1.0f;
+  return make_float2(z.x <= bound ? 0.0f : q.x, z.y <= bound ? 0.0f : q.y);
 }
 
 // Running moments of V channels. Values are summed as differences from the thread's first value
 // k: with n values, sum (x - k)^2 is at most n times their sum of squared deviations from their
 // mean (k is one of them), so rounding grows by no more than n, whatever the offset of the data.
-// Blocks give a thread at most kMomentRows rows.
-constexpr int kMomentRows = 256;
+// Blocks give a thread at most kMomentRows rows; a warp's threads that share a column are joined
+// about the first one's pivot, which multiplies that number by the rows that a warp holds.
+constexpr int kMomentRows = 64;
 
 template <int V>
 struct Moments {
-  float pivot[V], sum[V], square[V];
-  int count = 0;
+  Pairs<V> pivot, sum, square;  // the pivot is kept negated
 
-  __device__ __forceinline__ void add(const float (&v)[V]) {
-    if (count == 0) {
+  __device__ __forceinline__ void start(const Pairs<V>& v) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) pivot[j] = v[j], sum[j] = 0.0f, square[j] = 0.0f;
+    for (int j = 0; j < Pairs<V>::kCount; ++j) {
+      pivot.p[j] = make_float2(-v.p[j].x, -v.p[j].y);
+      sum.p[j] = square.p[j] = both(0.0f);
     }
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float d = v[j] - pivot[j];
-      sum[j] += d;
-      square[j] = fmaf(d, d, square[j]);
-    }
-    ++count;
   }
 
-  // (mean, sum of squared deviations) of channel j.
-  __device__ __forceinline__ float2 get(int j) const {
-    if (count == 0) return make_float2(0.0f, 0.0f);
-    const float n = static_cast<float>(count);
-    const float offset = sum[j] / n;
+  __device__ __forceinline__ void add(const Pairs<V>& v) {
+#pragma unroll
+    for (int j = 0; j < Pairs<V>::kCount; ++j) {
+      const float2 d = add2(v.p[j], pivot.p[j]);
+      sum.p[j] = add2(sum.p[j], d);
+      square.p[j] = fma2(d, d, square.p[j]);
+    }
+  }
+
+  // Moves to the pivots of a lane of the warp: sum (x - l) = sum (x - k) + n (k - l) and
+  // sum (x - l)^2 = sum (x - k)^2 + (k - l) (2 sum (x - k) + n (k - l)). Without values (n = 0)
+  // the sums stay zero.
+  __device__ __forceinline__ void move_pivot(int from_lane, float n) {
+#pragma unroll
+    for (int j = 0; j < Pairs<V>::kCount; ++j) {
+      float2 l;
+      l.x = __shfl_sync(0xFFFFFFFFu, pivot.p[j].x, from_lane);
+      l.y = V > 1 ? __shfl_sync(0xFFFFFFFFu, pivot.p[j].y, from_lane) : 0.0f;
+      const float2 d = n > 0.0f ? make_float2(l.x - pivot.p[j].x, l.y - pivot.p[j].y) : both(0.0f);
+      const float2 nd = mul2(both(n), d);
+      square.p[j] = fma2(d, fma2(both(2.0f), sum.p[j], nd), square.p[j]);
+      sum.p[j] = add2(sum.p[j], nd);
+      pivot.p[j] = l;
+    }
+  }
+
+  // Adds the sums of the lane at this distance, about the same pivots.
+  __device__ __forceinline__ void add_lane(int distance) {
+#pragma unroll
+    for (int j = 0; j < Pairs<V>::kCount; ++j) {
+      float2 a, b = both(0.0f);
+      a.x = __shfl_xor_sync(0xFFFFFFFFu, sum.p[j].x, distance);
+      b.x = __shfl_xor_sync(0xFFFFFFFFu, square.p[j].x, distance);
+      a.y = V > 1 ? __shfl_xor_sync(0xFFFFFFFFu, sum.p[j].y, distance) : 0.0f;
+      b.y = V > 1 ? __shfl_xor_sync(0xFFFFFFFFu, square.p[j].y, distance) : 0.0f;
+      sum.p[j] = add2(sum.p[j], a);
+      square.p[j] = add2(square.p[j], b);
+    }
+  }
+
+  // (mean, sum of squared deviations) of channel j over n values.
+  __device__ __forceinline__ float2 get(int j, float n, float inverse) const {
+    const float offset = sum.get(j) * inverse;
     // An overflown or NaN sum of squares stays what it is.
-    const float squares = square[j] < __int_as_float(0x7f800000)
-                              ? fmaxf(0.0f, fmaf(-sum[j], offset, square[j]))
-                              : square[j];
-    return make_float2(pivot[j] + offset, squares);
+    const float total = square.get(j);
+    const float squares = total < __int_as_float(0x7f800000)
+                              ? fmaxf(0.0f, fmaf(-n * offset, offset, total))
+                              : total;
+    return make_float2(offset - pivot.get(j), squares);
   }
 };
+
+// Moments of Q neighbouring channels of a thread, n values each, as one part of n Q values.
+template <int Q, int V>
+__device__ __forceinline__ float2 fold_channels(const Moments<V>& m, int first, float n,
+                                                float inverse) {
+  float2 part[Q];
+  float mean = 0.0f;
+#pragma unroll
+  for (int j = 0; j < Q; ++j) part[j] = m.get(first + j, n, inverse);
+#pragma unroll
+  for (int j = 0; j < Q; ++j) mean += part[j].x - part[0].x;
+  mean = fmaf(mean, 1.0f / Q, part[0].x);
+  float squares = 0.0f;
+#pragma unroll
+  for (int j = 0; j < Q; ++j) {
+    const float d = part[j].x - mean;
+    squares += fmaf(n * d, d, part[j].y);
+  }
+  return make_float2(mean, squares);
+}
 
 // NaN or infinite data give NaN statistics (their mean is NaN or infinite).
 __device__ __forceinline__ float variance_of(float mean, float squares, float count) {
@@ -175,11 +278,10 @@ __device__ __forceinline__ float lane_sum(float v, int lanes) {
 // one, and part 0 is never empty. All threads of the block call this with the same `items` of
 // `parts` entries each; `done(item, mean, squares)` runs on one lane per item.
 template <typename Part, typename Done>
-__device__ __forceinline__ void join_moments(int items, int parts, int threads, Part part,
-                                             Done done) {
-  const int lanes = lanes_per(items, threads);
-  const int lane = threadIdx.x % lanes;
-  const int step = threads / lanes;
+__device__ __forceinline__ void join_moments(int items, int parts, Part part, Done done) {
+  const int lanes = lanes_per(items, kNormThreads);
+  const int lane = threadIdx.x & (lanes - 1);
+  const int step = kNormThreads / lanes;
   for (int base = 0; base < items; base += step) {
     const int item = base + threadIdx.x / lanes;
     const bool live = item < items;
@@ -187,6 +289,7 @@ __device__ __forceinline__ void join_moments(int items, int parts, int threads, 
     float2 first = make_float2(0.0f, 0.0f);
     if (live) {
       part(item, 0, first);
+#pragma unroll 4
       for (int i = lane; i < parts; i += lanes) {
         float2 v;
         const float c = part(item, i, v);
@@ -199,6 +302,7 @@ __device__ __forceinline__ void join_moments(int items, int parts, int threads, 
     const float mean = first.x + total / n;
     float squares = 0.0f;
     if (live) {
+#pragma unroll 4
       for (int i = lane; i < parts; i += lanes) {
         float2 v;
         const float c = part(item, i, v);
@@ -213,16 +317,16 @@ __device__ __forceinline__ void join_moments(int items, int parts, int threads, 
 
 // Sums pairs: `part(item, i)` is entry i of the item's `parts`.
 template <typename Part, typename Done>
-__device__ __forceinline__ void join_sums(int items, int parts, int threads, Part part,
-                                          Done done) {
-  const int lanes = lanes_per(items, threads);
-  const int lane = threadIdx.x % lanes;
-  const int step = threads / lanes;
+__device__ __forceinline__ void join_sums(int items, int parts, Part part, Done done) {
+  const int lanes = lanes_per(items, kNormThreads);
+  const int lane = threadIdx.x & (lanes - 1);
+  const int step = kNormThreads / lanes;
   for (int base = 0; base < items; base += step) {
     const int item = base + threadIdx.x / lanes;
     const bool live = item < items;
     float2 total = make_float2(0.0f, 0.0f);
     if (live) {
+#pragma unroll 8
       for (int i = lane; i < parts; i += lanes) {
         const float2 v = part(item, i);
         total.x += v.x;
@@ -235,10 +339,35 @@ __device__ __forceinline__ void join_sums(int items, int parts, int threads, Par
   }
 }
 
+// A thread's place in a tile of columns: `lanes` rows of the tile's vectors at a time.
+struct TileThread {
+  int lanes, lane, col;
+  bool active;
+
+  __device__ __forceinline__ explicit TileThread(int cols) {
+    lanes = kNormThreads / cols;
+    lane = threadIdx.x / cols;
+    col = threadIdx.x - lane * cols;
+    active = lane < lanes;
+  }
+};
+
+// The kernels of a pass depend on one another and are launched with programmatic dependence: a
+// kernel's blocks may start while the last ones of the kernel before it run, and wait here before
+// they read its results (through pointers that are not __restrict__: a load that the compiler knows
+// to be constant could be moved before the wait). Every block of every kernel waits, so that a
+// kernel's completion implies that of all before it.
+__device__ __forceinline__ void wait_for_kernel_before() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_kernel_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // ---- host --------------------------------------------------------------------------------------
 
-constexpr int kNoPlan = 0;
 constexpr int kMaxNormChannels = 1 << 16;
+constexpr long long kMaxNormBlocks = 0x7FFFFFFF;  // of one launch
 
 inline int greatest_divisor(long long a, long long b) {
   while (b != 0) {
@@ -262,6 +391,10 @@ inline bool bad_norm_param(const void* data, int32_t dtype, int64_t rows, int64_
 inline float norm_bound(int activation) {
   return activation == DR_ACTIVATION_RELU ? 0.0f : -__builtin_huge_valf();
 }
+
+// Bytes that both passes over a part of the views may read for the second one to find them in L2
+// (126 MB; 80 MB read and as much written in turn is what was seen to stay).
+constexpr long long kPartBytes = 72LL << 20;
 
 // A vector width and a number of folded pixels.
 struct NormVector {
@@ -293,18 +426,19 @@ inline NormVector choose_vector(long long pixels, int channels, int dtype, long 
   return {1, 1};
 }
 
-// Cuts views into tiles of columns and chunks of rows of about `chunk_bytes`. Lowers v.vec where a
-// group is wider than a block's threads and not whole vectors (its tiles must not reach into the
-// next group). False when there would be too many blocks.
+// Cuts views into tiles of at most `most_cols` columns (at least the fewest whole groups that are
+// whole vectors) and chunks of rows of about `chunk_bytes`, whole steps of a block's threads of
+// `unroll` rows each where there are that many. Lowers v.vec where a group is wider than a block's
+// threads and not whole vectors (its tiles must not reach into the next group). False when there
+// would be too many blocks.
 inline bool cut_norm(NormShape& s, NormVector& v, long long batch, long long pixels, int channels,
                      int groups, int dtype, long long x_stride, long long grad_stride,
-                     long long chunk_bytes) {
+                     int most_cols, long long chunk_bytes, int unroll) {
   s.batch = batch;
   s.pixels = pixels;
   s.channels = channels;
   s.groups = groups;
   s.group_channels = channels / groups;
-  // Columns of the fewest whole groups that are whole vectors.
   const int d = s.group_channels;
   long long unit = d / greatest_divisor(d, v.vec);
   if (v.fold == 1 && unit > kNormThreads && d % v.vec != 0) {
@@ -316,47 +450,70 @@ inline bool cut_norm(NormShape& s, NormVector& v, long long batch, long long pix
   s.cols = static_cast<int>(static_cast<long long>(channels) * s.fold / v.vec);
   s.x_row = x_stride * s.fold;
   s.grad_row = grad_stride * s.fold;
-  s.group_tiles = 1;
+  s.pieces = 1;
   s.group_cols = 0;
-  if (s.cols <= kNormThreads) {
+  most_cols = std::min(most_cols, kNormThreads);
+  if (s.fold > 1) {
     s.tile_cols = s.cols;
     s.tiles = 1;
   } else if (unit <= kNormThreads) {
-    s.tile_cols = static_cast<int>(kNormThreads / unit * unit);
+    s.tile_cols =
+        static_cast<int>(std::min<long long>(s.cols, std::max(1LL, most_cols / unit) * unit));
     s.tiles = (s.cols + s.tile_cols - 1) / s.tile_cols;
   } else {
     s.group_cols = static_cast<int>(unit);
-    s.group_tiles = static_cast<int>((unit + kNormThreads - 1) / kNormThreads);
+    s.pieces = static_cast<int>((unit + kNormThreads - 1) / kNormThreads);
     s.tile_cols = kNormThreads;
-    s.tiles = groups * s.group_tiles;
+    s.tiles = groups * s.pieces;
   }
   const long long lanes = kNormThreads / s.tile_cols;  // rows that a block reads at once
   const long long tile_bytes = static_cast<long long>(s.tile_cols) * v.vec * dtype_bytes(dtype);
-  const long long deep = chunk_bytes / tile_bytes / lanes;
-  s.chunk_rows = std::max(1LL, std::min<long long>(deep, kMomentRows)) * lanes;
+  long long deep = chunk_bytes / tile_bytes / lanes;
+  if (deep > unroll) deep = deep / unroll * unroll;
+  s.chunk_rows = static_cast<int>(std::max(1LL, std::min<long long>(deep, kMomentRows)) * lanes);
   const long long chunks = (s.rows + s.chunk_rows - 1) / s.chunk_rows;
-  if (chunks > 0x7FFFFFFF || batch * s.tiles > 0x7FFFFFFF / std::max(1LL, chunks)) return false;
+  if (chunks > kMaxNormBlocks || batch > kMaxNormBlocks / s.tiles ||
+      chunks > kMaxNormBlocks / std::max(1LL, batch * s.tiles))
+    return false;
   s.chunks = static_cast<int>(chunks);
   return true;
 }
 
-// Bytes of a chunk: 64 KB, less where that would leave processors idle.
-inline long long norm_chunk_bytes(long long batch, long long pixels, int channels, int dtype) {
-  const long long total = batch * pixels * channels * dtype_bytes(dtype);
-  return std::max(4096LL, std::min(65536LL, total / 592));
+// The plan of a call in passes over memory. Chunks are 64 KB, less where that would leave
+// processors idle, more where a view would have over a thousand.
+constexpr int kNormUnroll = 4;
+
+inline bool plan_passes(NormShape& s, NormVector& v, long long batch, long long pixels,
+                        int channels, int groups, int dtype, long long x_stride,
+                        long long grad_stride) {
+  const long long view = pixels * channels * dtype_bytes(dtype);
+  const long long chunk = std::max(
+      view / 1024, std::max(4096LL, std::min(65536LL, batch * view / (4 * 148))));
+  return cut_norm(s, v, batch, pixels, channels, groups, dtype, x_stride, grad_stride, kNormThreads,
+                  chunk, kNormUnroll);
 }
 
-// Workspace of the forward pass: (mean, squares) of each group, chunk and tile.
-inline size_t norm_forward_bytes(const NormShape& s) {
-  return static_cast<size_t>(s.batch) * s.groups * s.chunks * s.group_tiles * sizeof(float2);
+// Views that are taken together, first pass and second: as many as stay in L2 in between.
+inline int views_at_once(const NormShape& s, int dtype, int images) {
+  const long long view = s.pixels * s.channels * dtype_bytes(dtype) * images;
+  return static_cast<int>(std::max(1LL, std::min(s.batch, kPartBytes / std::max(1LL, view))));
 }
 
-// Workspace of the backward pass: sums of each channel and chunk, of each view and channel, and
-// the two means of each view and group.
-inline size_t norm_backward_bytes(const NormShape& s) {
-  const size_t views = static_cast<size_t>(s.batch) * s.channels * sizeof(float2);
-  return align256(views * s.chunks) + align256(views) +
-         static_cast<size_t>(s.batch) * s.groups * sizeof(float2);
+// Workspace. Forward: (mean, squares) of each group (or piece of one) for each chunk. Backward: sums
+// of each channel for each chunk and of each view, and the two means of each group.
+struct NormSpace {
+  size_t parts, sums, means, total;  // offsets, and the end
+};
+
+inline NormSpace norm_space(const NormShape& s, bool backward) {
+  const size_t groups = static_cast<size_t>(s.batch) * s.groups * sizeof(float2);
+  const size_t channels = static_cast<size_t>(s.batch) * s.channels * sizeof(float2);
+  NormSpace w;
+  w.parts = 0;
+  w.sums = align256((backward ? channels : groups * s.pieces) * s.chunks);
+  w.means = w.sums + (backward ? align256(channels) : 0);
+  w.total = w.means + (backward ? groups : 0);
+  return w;
 }
 
 // The larger workspace of all the vector widths that a call may turn out to take.
@@ -371,30 +528,56 @@ inline size_t norm_workspace_bytes(long long batch, long long pixels, int channe
       continue;
     if (v.fold == 1 && channels % v.vec != 0) continue;
     NormShape s;
-    if (cut_norm(s, v, batch, pixels, channels, groups, dtype, channels, channels,
-                 norm_chunk_bytes(batch, pixels, channels, dtype)))
-      most = std::max(most, backward ? norm_backward_bytes(s) : norm_forward_bytes(s));
+    if (plan_passes(s, v, batch, pixels, channels, groups, dtype, channels, channels))
+      most = std::max(most, norm_space(s, backward).total);
   }
   return most;
 }
 
-template <typename T>
-struct TypeTag {
-  using type = T;
+// Launches a kernel on a stream, with programmatic dependence on the one before it if `after`.
+template <typename... Params, typename... Args>
+cudaError_t launch_kernel(void (*kernel)(Params...), unsigned int blocks, unsigned int threads,
+                          cudaStream_t stream, bool after, Args... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(blocks);
+  config.blockDim = dim3(threads);
+  config.stream = stream;
+  cudaLaunchAttribute attribute = {};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = after ? 1 : 0;
+  return cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
+}
+
+template <typename T, int V, bool Silu, bool Drop>
+struct Variant {
+  using Type = T;
+  static constexpr int kVec = V;
+  static constexpr bool kSilu = Silu, kDrop = Drop;
 };
 
-// Calls fn(TypeTag<T>, integral_constant<int, V>) for a type and one of its vector widths.
+// Calls fn(Variant) for a type, one of its vector widths, an activation and with or without
+// dropout.
 template <typename Fn>
-int with_vector(int dtype, int vec, Fn fn) {
-  auto half = [&](auto tag) {
-    if (vec == 8) return fn(tag, std::integral_constant<int, 8>());
-    if (vec == 2) return fn(tag, std::integral_constant<int, 2>());
-    return fn(tag, std::integral_constant<int, 1>());
+int with_variant(int dtype, int vec, int activation, int threshold, Fn fn) {
+  const bool silu = activation == DR_ACTIVATION_SILU, drop = threshold != 0;
+  auto flags = [&](auto type, auto width) {
+    using T = typename decltype(type)::Type;
+    constexpr int V = decltype(width)::value;
+    if (silu)
+      return drop ? fn(Variant<T, V, true, true>()) : fn(Variant<T, V, true, false>());
+    return drop ? fn(Variant<T, V, false, true>()) : fn(Variant<T, V, false, false>());
   };
-  if (dtype == DR_FLOAT16) return half(TypeTag<__half>());
-  if (dtype == DR_BFLOAT16) return half(TypeTag<__nv_bfloat16>());
-  if (vec == 4) return fn(TypeTag<float>(), std::integral_constant<int, 4>());
-  return fn(TypeTag<float>(), std::integral_constant<int, 1>());
+  auto half = [&](auto type) {
+    if (vec == 8) return flags(type, std::integral_constant<int, 8>());
+    if (vec == 2) return flags(type, std::integral_constant<int, 2>());
+    return flags(type, std::integral_constant<int, 1>());
+  };
+  if (dtype == DR_FLOAT16) return half(Variant<__half, 0, false, false>());
+  if (dtype == DR_BFLOAT16) return half(Variant<__nv_bfloat16, 0, false, false>());
+  if (vec == 4) return flags(Variant<float, 0, false, false>(), std::integral_constant<int, 4>());
+  return flags(Variant<float, 0, false, false>(), std::integral_constant<int, 1>());
 }
 
 }  // namespace dr

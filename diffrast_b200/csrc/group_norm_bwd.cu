@@ -9,191 +9,262 @@ namespace {
 
 constexpr int kUnroll = 2;  // vectors of x, and as many of the gradient, a thread has under way
 
-// Constants of a thread's channels.
+// Constants of a thread's channels: z = (x + shift) scale + bias.
 template <int V>
 struct Channels {
-  float mean[V], rstd[V], weight[V], bias[V];
+  Pairs<V> shift, scale, bias;
 
   __device__ __forceinline__ void load(const NormShape& s, long long view, int first,
                                        const NormParam& w, const NormParam& b,
                                        const float* means, const float* rstds) {
+    if (V == 1) shift.p[0].y = scale.p[0].y = bias.p[0].y = 0.0f;
+    ChannelWalk c(s, first);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = (first + j) % s.channels;
-      const long long group = view * s.groups + c / s.group_channels;
-      mean[j] = __ldg(means + group);
-      rstd[j] = __ldg(rstds + group);
-      weight[j] = w.data ? load_param(w.data, w.dtype, view * w.view + c) : 1.0f;
-      bias[j] = b.data ? load_param(b.data, b.dtype, view * b.view + c) : 0.0f;
+      const long long group = view * s.groups + c.group;
+      shift.set(j, -__ldg(means + group));
+      scale.set(j, __ldg(rstds + group) * load_scale(w, view, c.channel));
+      bias.set(j, load_shift(b, view, c.channel));
+      c.next();
     }
   }
 };
 
-// Runs use(vector of x, vector of the gradient, row) over the rows first, first + step, ... < end.
-template <typename T, int V, typename Use>
+// Joins the threads' sums of a block's rows: over the rows of a warp where a tile's columns divide
+// it, then over the rows (and folded pixels) that are left. `done` gets the channel within the
+// tile.
+template <int V, typename Done>
+__device__ __forceinline__ void join_block(Pairs<V>& sum, Pairs<V>& dot, const TileThread& t,
+                                           const NormShape& s, const NormTile& tile, Done done) {
+  __shared__ float2 entry[kNormThreads * V];
+  const int width = tile.cols * V;
+  int rows = t.lanes, row = t.lane;
+  bool write = t.active;
+  if (tile.cols < 32 && 32 % tile.cols == 0) {
+    for (int d = tile.cols; d < 32; d *= 2) {
+#pragma unroll
+      for (int j = 0; j < Pairs<V>::kCount; ++j) {
+        sum.p[j].x += __shfl_xor_sync(0xFFFFFFFFu, sum.p[j].x, d);
+        dot.p[j].x += __shfl_xor_sync(0xFFFFFFFFu, dot.p[j].x, d);
+        if (V > 1) {
+          sum.p[j].y += __shfl_xor_sync(0xFFFFFFFFu, sum.p[j].y, d);
+          dot.p[j].y += __shfl_xor_sync(0xFFFFFFFFu, dot.p[j].y, d);
+        }
+      }
+    }
+    rows = kNormThreads / 32;
+    row = threadIdx.x / 32;
+    write = threadIdx.x % 32 < tile.cols;
+  }
+  if (write) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      entry[row * width + t.col * V + j] = make_float2(sum.get(j), dot.get(j));
+  }
+  __syncthreads();
+  const int items = s.fold > 1 ? s.channels : width;
+  join_sums(items, rows * s.fold, [&](int item, int i) { return entry[i * items + item]; }, done);
+}
+
+// Gives the vectors of x and of the gradient in the rows first, first + step, ... below `end` of a
+// column to `use(x, gradient)` in order, kUnroll of them at a time. `Last`: nothing will read them
+// again.
+template <typename T, int V, bool Last, typename Use>
 __device__ __forceinline__ void for_rows(const T* __restrict__ x, long long x_row,
                                          const T* __restrict__ grad, long long grad_row, int first,
                                          int step, int end, Use use) {
   using P = Packed<T, V>;
-  for (int row = first; row < end; row += kUnroll * step) {
+  auto load = [](const T* at) {
+    return Last ? __ldcs(reinterpret_cast<const P*>(at)) : *reinterpret_cast<const P*>(at);
+  };
+  x += first * x_row;
+  grad += first * grad_row;
+  x_row *= step;
+  grad_row *= step;
+  int left = end - first;
+  for (; left > (kUnroll - 1) * step; left -= kUnroll * step) {
     P p[kUnroll], g[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      if (row + u * step < end) {
-        p[u] = *reinterpret_cast<const P*>(x + (row + u * step) * x_row);
-        g[u] = *reinterpret_cast<const P*>(grad + (row + u * step) * grad_row);
-      }
+      p[u] = load(x);
+      g[u] = load(grad);
+      x += x_row;
+      grad += grad_row;
     }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (row + u * step < end) use(p[u], g[u], row + u * step);
+    for (int u = 0; u < kUnroll; ++u) use(load_pairs<T, V>(p[u]), load_pairs<T, V>(g[u]));
+  }
+  for (; left > 0; left -= step) {
+    use(load_pairs<T, V>(load(x)), load_pairs<T, V>(load(grad)));
+    x += x_row;
+    grad += grad_row;
   }
 }
 
-// Sums of q and q (x - m) of each channel over one chunk of rows in one tile of columns.
+// First pass: sums of q and q (x - m) of each channel over one chunk of rows in one tile of columns.
 // parts [batch][chunks][channels].
 template <typename T, int V, bool Silu, bool Drop>
-__global__ void __launch_bounds__(kNormThreads) norm_sums_kernel(
-    const T* __restrict__ x, const T* __restrict__ grad, NormShape s, NormParam weight,
+__global__ void __launch_bounds__(kNormThreads, 3) norm_sums_kernel(
+    const T* __restrict__ x, const T* __restrict__ grad, NormShape s, int view0, NormParam weight,
     NormParam bias, float bound, DropKey key, const float* __restrict__ mean,
     const float* __restrict__ rstd, float2* __restrict__ parts) {
-  __shared__ float2 entry[kNormThreads * V];
-  long long block = blockIdx.x;
-  const int chunk = static_cast<int>(block % s.chunks);
-  block /= s.chunks;
-  const NormTile tile = norm_tile(s, V, static_cast<int>(block % s.tiles));
-  const long long view = block / s.tiles;
-  const int lanes = kNormThreads / tile.cols;
-  const int col = threadIdx.x % tile.cols, lane = threadIdx.x / tile.cols;
-  const long long row0 = chunk * s.chunk_rows;
-  const int rows = static_cast<int>(min(s.chunk_rows, s.rows - row0));
-  const int width = tile.cols * V;
-  if (lane < lanes) {
+  let_next_kernel_start();
+  const NormBlock b = norm_block(s, V, view0, blockIdx.x);
+  const TileThread t(b.tile.cols);
+  const int col = (b.tile.col + t.col) * V;
+  Pairs<V> sum, dot;
+#pragma unroll
+  for (int j = 0; j < Pairs<V>::kCount; ++j) sum.p[j] = dot.p[j] = both(0.0f);
+  if (t.active) {
     Channels<V> c;
-    c.load(s, view, (tile.col + col) * V, weight, bias, mean, rstd);
+    c.load(s, b.view, col, weight, bias, mean, rstd);
     const unsigned long long seed = Drop ? load_seed(key) : 0;
     const long long out_row = static_cast<long long>(s.channels) * s.fold;
-    const long long offset = (view * s.rows + row0) * out_row + (tile.col + col) * V;
-    float sum[V], dot[V];
+    long long at = (b.first + t.lane) * out_row + col;
+    const long long step = t.lanes * out_row;
+    for_rows<T, V, false>(x + b.first * s.x_row + col, s.x_row, grad + b.first * s.grad_row + col,
+                          s.grad_row, t.lane, t.lanes, b.rows,
+                          [&](const Pairs<V>& v, Pairs<V> q) {
+      if (Drop) apply_dropout<V>(q, at, key, seed);
+      at += step;
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum[j] = 0.0f, dot[j] = 0.0f;
-    for_rows<T, V>(x + (view * s.rows + row0) * s.x_row + (tile.col + col) * V, s.x_row,
-                   grad + (view * s.rows + row0) * s.grad_row + (tile.col + col) * V, s.grad_row,
-                   lane, lanes, rows, [&](const Packed<T, V>& p, const Packed<T, V>& g, int row) {
-      float v[V], q[V];
-      unpack<T, V>(p, v);
-      unpack<T, V>(g, q);
-      if (Drop) apply_dropout<V>(q, offset + row * out_row, key, seed);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = v[j] - c.mean[j];
-        const float z = fmaf(d, c.rstd[j] * c.weight[j], c.bias[j]);
-        const float t = q[j] * activate_grad<Silu>(z, bound);
-        sum[j] += t;
-        dot[j] = fmaf(t, d, dot[j]);
+      for (int j = 0; j < Pairs<V>::kCount; ++j) {
+        const float2 d = add2(v.p[j], c.shift.p[j]);
+        const float2 z = fma2(d, c.scale.p[j], c.bias.p[j]);
+        const float2 u = activate_grad<Silu>(q.p[j], z, bound);
+        sum.p[j] = add2(sum.p[j], u);
+        dot.p[j] = fma2(u, d, dot.p[j]);
       }
     });
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      entry[lane * width + col * V + j] = make_float2(sum[j], dot[j]);
   }
-  __syncthreads();
-  const int items = s.fold > 1 ? s.channels : width;
-  const int first = s.fold > 1 ? 0 : tile.col * V;
-  join_sums(
-      items, lanes * s.fold, kNormThreads,
-      [&](int item, int i) { return entry[i * items + item]; },
-      [&](int item, float2 total) {
-        parts[(view * s.chunks + chunk) * s.channels + first + item] = total;
-      });
+  const int first = s.fold > 1 ? 0 : b.tile.col * V;
+  join_block<V>(sum, dot, t, s, b.tile, [&](int item, float2 total) {
+    parts[(static_cast<long long>(b.view) * s.chunks + b.chunk) * s.channels + first + item] = total;
+  });
+  wait_for_kernel_before();
 }
 
-// Per view: the channels' sums over the chunks, then the groups' two means. One block for each
-// view and each run of groups (`run_groups` of them).
-__global__ void __launch_bounds__(kNormThreads) norm_means_kernel(
-    const float2* __restrict__ parts, NormShape s, NormParam weight, int runs, int run_groups,
-    const float* __restrict__ rstd, float2* __restrict__ sums, float2* __restrict__ means) {
-  const long long view = blockIdx.x / runs;
+// Joins the parts of a view's channels, 32 of them at a time by 32 lanes each, and forms the two
+// means of their groups. A block has a run of whole groups of at most 32 channels, or one group.
+constexpr int kMeansThreads = 1024;
+
+__global__ void __launch_bounds__(kMeansThreads) norm_means_kernel(
+    const float2* parts, NormShape s, int view0, NormParam weight, int runs,
+    int run_groups, const float* __restrict__ rstd, float2* __restrict__ sums,
+    float2* __restrict__ means) {
+  __shared__ float2 entry[32][33];
+  __shared__ float2 scaled[32];
+  let_next_kernel_start();
+  wait_for_kernel_before();
+  const long long view = view0 + blockIdx.x / runs;
+  const int d = s.group_channels;
   const int group0 = static_cast<int>(blockIdx.x % runs) * run_groups;
-  const int groups = min(run_groups, s.groups - group0);
-  const int d = s.group_channels, first = group0 * d;
-  join_sums(
-      groups * d, s.chunks, kNormThreads,
-      [&](int item, int i) { return parts[(view * s.chunks + i) * s.channels + first + item]; },
-      [&](int item, float2 total) {
-        total.y *= rstd[view * s.groups + (first + item) / d];
-        sums[view * s.channels + first + item] = total;
-      });
-  __syncthreads();
-  const float count = static_cast<float>(s.pixels) * static_cast<float>(d);
-  join_sums(
-      groups, d, kNormThreads,
-      [&](int item, int i) {
-        const int c = first + item * d + i;
-        const float w =
-            weight.data ? load_param(weight.data, weight.dtype, view * weight.view + c) : 1.0f;
-        const float2 v = sums[view * s.channels + c];
-        return make_float2(v.x * w, v.y * w);
-      },
-      [&](int item, float2 total) {
-        means[view * s.groups + group0 + item] = make_float2(total.x / count, total.y / count);
-      });
+  const int channel0 = group0 * d;
+  const int channels = min(run_groups, s.groups - group0) * d;
+  const int x = threadIdx.x % 32, y = threadIdx.x / 32;
+  const float inverse = 1.0f / (static_cast<float>(s.pixels) * static_cast<float>(d));
+  float2 group = make_float2(0.0f, 0.0f);  // of a group wider than 32 channels
+  for (int base = 0; base < channels; base += 32) {
+    const int c = channel0 + base + x;
+    float2 total = make_float2(0.0f, 0.0f);
+    if (base + x < channels) {
+      const float2* from = parts + view * s.chunks * s.channels + c;
+#pragma unroll 8
+      for (int i = y; i < s.chunks; i += 32) {
+        const float2 v = from[static_cast<long long>(i) * s.channels];
+        total.x += v.x;
+        total.y += v.y;
+      }
+    }
+    entry[y][x] = total;
+    __syncthreads();
+    // Channel y of the 32 is summed by warp y.
+    total = entry[x][y];
+    total.x = lane_sum(total.x, 32);
+    total.y = lane_sum(total.y, 32);
+    if (x == 0) {
+      const int channel = channel0 + base + y;
+      float2 w = make_float2(0.0f, 0.0f);
+      if (base + y < channels) {
+        total.y *= rstd[view * s.groups + channel / d];
+        sums[view * s.channels + channel] = total;
+        const float scale = load_scale(weight, view, channel);
+        w = make_float2(total.x * scale, total.y * scale);
+      }
+      scaled[y] = w;
+    }
+    __syncthreads();
+    if (d > 32) {
+      if (y == 0) {
+        group.x += lane_sum(scaled[x].x, 32);
+        group.y += lane_sum(scaled[x].y, 32);
+      }
+    } else if (threadIdx.x < channels / d) {
+      for (int i = 0; i < d; ++i) {
+        group.x += scaled[threadIdx.x * d + i].x;
+        group.y += scaled[threadIdx.x * d + i].y;
+      }
+    }
+  }
+  if (threadIdx.x < (d > 32 ? 1 : channels / d))
+    means[view * s.groups + group0 + threadIdx.x] =
+        make_float2(group.x * inverse, group.y * inverse);
 }
 
-// grad x = r (q w - A - h B) over one chunk of rows in one tile of columns.
+// Second pass: grad x = r (q w - A - h B) over one chunk of rows in one tile of columns, from the
+// end of the views to their start (what the first pass read last is still in L2).
 template <typename T, int V, bool Silu, bool Drop>
-__global__ void __launch_bounds__(kNormThreads) norm_grad_kernel(
-    const T* __restrict__ x, const T* __restrict__ grad, NormShape s, NormParam weight,
+__global__ void __launch_bounds__(kNormThreads, 3) norm_grad_kernel(
+    const T* __restrict__ x, const T* __restrict__ grad, NormShape s, int view0, NormParam weight,
     NormParam bias, float bound, DropKey key, const float* __restrict__ mean,
-    const float* __restrict__ rstd, const float2* __restrict__ means, T* __restrict__ grad_x) {
-  long long block = blockIdx.x;
-  const int chunk = static_cast<int>(block % s.chunks);
-  block /= s.chunks;
-  const NormTile tile = norm_tile(s, V, static_cast<int>(block % s.tiles));
-  const long long view = block / s.tiles;
-  const int lanes = kNormThreads / tile.cols;
-  const int col = threadIdx.x % tile.cols, lane = threadIdx.x / tile.cols;
-  if (lane >= lanes) return;
-  const long long row0 = chunk * s.chunk_rows;
-  const int rows = static_cast<int>(min(s.chunk_rows, s.rows - row0));
+    const float* __restrict__ rstd, const float2* means, T* __restrict__ grad_x) {
+  let_next_kernel_start();
+  const NormBlock b = norm_block(s, V, view0, gridDim.x - 1 - blockIdx.x);
+  const TileThread t(b.tile.cols);
+  const int col = (b.tile.col + t.col) * V;
   Channels<V> c;
-  c.load(s, view, (tile.col + col) * V, weight, bias, mean, rstd);
-  float shift[V], slope[V];
+  if (t.active) c.load(s, b.view, col, weight, bias, mean, rstd);
+  wait_for_kernel_before();
+  if (!t.active) return;
+  Pairs<V> base, slope;  // grad x = u scale + d slope + base
+  if (V == 1) base.p[0].y = slope.p[0].y = 0.0f;
+  ChannelWalk walk(s, col);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int channel = ((tile.col + col) * V + j) % s.channels;
-    const float2 m = __ldg(means + view * s.groups + channel / s.group_channels);
-    shift[j] = -c.rstd[j] * m.x;
-    slope[j] = -c.rstd[j] * c.rstd[j] * m.y;
+    const long long group = static_cast<long long>(b.view) * s.groups + walk.group;
+    const float r = __ldg(rstd + group);
+    const float2 m = means[group];
+    base.set(j, -r * m.x);
+    slope.set(j, -r * r * m.y);
+    walk.next();
   }
   const unsigned long long seed = Drop ? load_seed(key) : 0;
   const long long out_row = static_cast<long long>(s.channels) * s.fold;
-  const long long offset = (view * s.rows + row0) * out_row + (tile.col + col) * V;
-  for_rows<T, V>(x + (view * s.rows + row0) * s.x_row + (tile.col + col) * V, s.x_row,
-                 grad + (view * s.rows + row0) * s.grad_row + (tile.col + col) * V, s.grad_row,
-                 lane, lanes, rows, [&](const Packed<T, V>& p, const Packed<T, V>& g, int row) {
-    float v[V], q[V];
-    unpack<T, V>(p, v);
-    unpack<T, V>(g, q);
-    const long long at = offset + row * out_row;
+  long long at = (b.first + t.lane) * out_row + col;
+  const long long step = t.lanes * out_row;
+  for_rows<T, V, true>(x + b.first * s.x_row + col, s.x_row, grad + b.first * s.grad_row + col,
+                       s.grad_row, t.lane, t.lanes, b.rows, [&](Pairs<V> v, Pairs<V> q) {
     if (Drop) apply_dropout<V>(q, at, key, seed);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float d = v[j] - c.mean[j];
-      const float a = c.rstd[j] * c.weight[j];
-      const float t = q[j] * activate_grad<Silu>(fmaf(d, a, c.bias[j]), bound);
-      v[j] = fmaf(t, a, fmaf(d, slope[j], shift[j]));
+    for (int j = 0; j < Pairs<V>::kCount; ++j) {
+      const float2 d = add2(v.p[j], c.shift.p[j]);
+      const float2 z = fma2(d, c.scale.p[j], c.bias.p[j]);
+      const float2 u = activate_grad<Silu>(q.p[j], z, bound);
+      v.p[j] = fma2(u, c.scale.p[j], fma2(d, slope.p[j], base.p[j]));
     }
-    *reinterpret_cast<Packed<T, V>*>(grad_x + at) = pack<T, V>(v);
+    __stcs(reinterpret_cast<Packed<T, V>*>(grad_x + at), pack_pairs<T, V>(v));
+    at += step;
   });
 }
 
 // Gradients of weight and bias: sums over the views (or each view's own), 32 channels a block.
 __global__ void __launch_bounds__(kNormThreads) norm_params_kernel(
-    const float2* __restrict__ sums, long long batch, int channels, void* grad_weight,
+    const float2* sums, long long batch, int channels, void* grad_weight,
     int weight_dtype, bool weight_views, void* grad_bias, int bias_dtype, bool bias_views) {
   constexpr int kLanes = kNormThreads / 32;
   __shared__ float2 entry[kLanes][32];
+  let_next_kernel_start();
+  wait_for_kernel_before();
   const int c = blockIdx.x * 32 + threadIdx.x % 32, lane = threadIdx.x / 32;
   float2 total = make_float2(0.0f, 0.0f);
   if (c < channels) {
@@ -218,48 +289,47 @@ __global__ void __launch_bounds__(kNormThreads) norm_params_kernel(
   if (grad_bias != nullptr && !bias_views) store_param(grad_bias, bias_dtype, c, total.x);
 }
 
-template <typename T, int V>
-int run(const void* x, const void* grad, const NormShape& s, const NormParam& weight,
-        const NormParam& bias, int activation, const DropKey& key, const float* mean,
-        const float* rstd, void* grad_x, void* grad_weight, bool weight_views, void* grad_bias,
-        bool bias_views, unsigned char* workspace, cudaStream_t stream) {
-  const size_t views = static_cast<size_t>(s.batch) * s.channels * sizeof(float2);
-  auto* parts = reinterpret_cast<float2*>(workspace);
-  auto* sums = reinterpret_cast<float2*>(workspace + align256(views * s.chunks));
-  auto* means = reinterpret_cast<float2*>(workspace + align256(views * s.chunks) + align256(views));
+struct Gradients {
+  void *x, *weight, *bias;
+  int weight_dtype, bias_dtype;
+  bool weight_views, bias_views;
+};
+
+template <typename T, int V, bool Silu, bool Drop>
+int passes(const void* x, const void* grad, const NormShape& s, int dtype, const NormParam& weight,
+           const NormParam& bias, float bound, const DropKey& key, const float* mean,
+           const float* rstd, const Gradients& out, unsigned char* workspace,
+           cudaStream_t stream) {
+  const NormSpace space = norm_space(s, true);
+  auto* parts = reinterpret_cast<float2*>(workspace + space.parts);
+  auto* sums = reinterpret_cast<float2*>(workspace + space.sums);
+  auto* means = reinterpret_cast<float2*>(workspace + space.means);
   const T* in = static_cast<const T*>(x);
   const T* dy = static_cast<const T*>(grad);
-  const unsigned int blocks = static_cast<unsigned int>(s.batch * s.tiles * s.chunks);
-  const float bound = norm_bound(activation);
-  const bool drop = key.threshold != 0, silu = activation == DR_ACTIVATION_SILU;
-  auto add = [&](auto kernel) {
-    kernel<<<blocks, kNormThreads, 0, stream>>>(in, dy, s, weight, bias, bound, key, mean, rstd,
-                                                parts);
-  };
-  if (silu)
-    drop ? add(norm_sums_kernel<T, V, true, true>) : add(norm_sums_kernel<T, V, true, false>);
-  else
-    drop ? add(norm_sums_kernel<T, V, false, true>) : add(norm_sums_kernel<T, V, false, false>);
   const int run_groups = std::max(1, std::min(s.groups, 32 / s.group_channels));
   const int runs = (s.groups + run_groups - 1) / run_groups;
-  norm_means_kernel<<<static_cast<unsigned int>(s.batch * runs), kNormThreads, 0, stream>>>(
-      parts, s, weight, runs, run_groups, rstd, sums, means);
-  if (grad_x != nullptr) {
-    auto apply = [&](auto kernel) {
-      kernel<<<blocks, kNormThreads, 0, stream>>>(in, dy, s, weight, bias, bound, key, mean, rstd,
-                                                  means, static_cast<T*>(grad_x));
-    };
-    if (silu)
-      drop ? apply(norm_grad_kernel<T, V, true, true>) : apply(norm_grad_kernel<T, V, true, false>);
-    else
-      drop ? apply(norm_grad_kernel<T, V, false, true>)
-           : apply(norm_grad_kernel<T, V, false, false>);
+  const int most = views_at_once(s, dtype, 2);
+  cudaError_t err = cudaSuccess;
+  for (int view0 = 0; view0 < s.batch; view0 += most) {
+    const int views = static_cast<int>(std::min<long long>(most, s.batch - view0));
+    const unsigned int blocks = static_cast<unsigned int>(views) * s.tiles * s.chunks;
+    err = launch_kernel(norm_sums_kernel<T, V, Silu, Drop>, blocks, kNormThreads, stream,
+                        view0 > 0, in, dy, s, view0, weight, bias, bound, key, mean, rstd, parts);
+    if (err == cudaSuccess)
+      err = launch_kernel(norm_means_kernel, static_cast<unsigned int>(views) * runs,
+                          kMeansThreads, stream, true, parts, s, view0, weight, runs, run_groups,
+                          rstd, sums, means);
+    if (err == cudaSuccess && out.x != nullptr)
+      err = launch_kernel(norm_grad_kernel<T, V, Silu, Drop>, blocks, kNormThreads, stream, true,
+                          in, dy, s, view0, weight, bias, bound, key, mean, rstd, means,
+                          static_cast<T*>(out.x));
+    if (err != cudaSuccess) return static_cast<int>(err);
   }
-  if (grad_weight != nullptr || grad_bias != nullptr)
-    norm_params_kernel<<<blocks_for(s.channels, 32), kNormThreads, 0, stream>>>(
-        sums, s.batch, s.channels, grad_weight, weight.dtype, weight_views, grad_bias, bias.dtype,
-        bias_views);
-  return launch_status();
+  if (out.weight != nullptr || out.bias != nullptr)
+    err = launch_kernel(norm_params_kernel, blocks_for(s.channels, 32), kNormThreads, stream, true,
+                        sums, s.batch, s.channels, out.weight, out.weight_dtype, out.weight_views,
+                        out.bias, out.bias_dtype, out.bias_views);
+  return err == cudaSuccess ? launch_status() : static_cast<int>(err);
 }
 
 }  // namespace
@@ -288,17 +358,21 @@ extern "C" int dr_group_norm_bwd(const void* x, int64_t x_stride, const void* gr
   NormShape s;
   NormVector v = choose_vector(pixels, channels, dtype, x_stride, grad_stride,
                                {x, grad_y, grad_x});
-  if (!cut_norm(s, v, batch, pixels, channels, groups, dtype, x_stride, grad_stride,
-                norm_chunk_bytes(batch, pixels, channels, dtype)))
+  if (batch > kMaxNormBlocks ||
+      !plan_passes(s, v, batch, pixels, channels, groups, dtype, x_stride, grad_stride))
     return DR_ERR_TOO_LARGE;
-  if (workspace == nullptr || workspace_bytes < norm_backward_bytes(s))
+  if (workspace == nullptr || workspace_bytes < norm_space(s, true).total)
     return DR_ERR_WORKSPACE_TOO_SMALL;
   const NormParam w{weight, weight_dtype, weight_batch > 1 ? channels : 0};
   const NormParam b{bias, bias_dtype, bias_batch > 1 ? channels : 0};
   const DropKey key = drop_key(seed, seed_value, layer, drop_threshold);
-  return with_vector(dtype, v.vec, [&](auto type, auto width) {
-    return run<typename decltype(type)::type, decltype(width)::value>(
-        x, grad_y, s, w, b, activation, key, mean, rstd, grad_x, grad_weight, weight_batch > 1,
-        grad_bias, bias_batch > 1, static_cast<unsigned char*>(workspace), as_stream(stream));
+  const Gradients out{grad_x,      grad_weight,      grad_bias,     weight_dtype,
+                      bias_dtype,  weight_batch > 1, bias_batch > 1};
+  const float bound = norm_bound(activation);
+  return with_variant(dtype, v.vec, activation, drop_threshold, [&](auto k) {
+    using K = decltype(k);
+    return passes<typename K::Type, K::kVec, K::kSilu, K::kDrop>(
+        x, grad_y, s, dtype, w, b, bound, key, mean, rstd, out,
+        static_cast<unsigned char*>(workspace), as_stream(stream));
   });
 }

@@ -15,7 +15,7 @@
 
 #include <cstdint>
 
-#include "common.cuh"
+#include "vector.cuh"
 
 namespace dr {
 
@@ -59,10 +59,10 @@ __device__ __forceinline__ uint4 philox(unsigned long long block, unsigned int l
   return c;
 }
 
-// v[j] = kept ? v[j] * scale : 0 for the V elements from `element` on (a multiple of V; V is 1, 2,
+// v = kept ? v * scale : 0 for the V elements from `element` on (a multiple of V; V is 1, 2,
 // 4 or 8, so they share a counter). A dropped NaN or infinity gives 0 too.
 template <int V>
-__device__ __forceinline__ void apply_dropout(float (&v)[V], long long element, const DropKey& key,
+__device__ __forceinline__ void apply_dropout(Pairs<V>& v, long long element, const DropKey& key,
                                               unsigned long long seed) {
   const uint4 r = philox(static_cast<unsigned long long>(element) >> 3, key.layer, seed);
   unsigned int w[(V + 1) / 2];
@@ -80,7 +80,7 @@ __device__ __forceinline__ void apply_dropout(float (&v)[V], long long element, 
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const unsigned int bits = j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xFFFFu;
-    v[j] = bits >= key.threshold ? v[j] * key.scale : 0.0f;
+    v.set(j, bits >= key.threshold ? v.get(j) * key.scale : 0.0f);
   }
 }
 
