@@ -5,49 +5,24 @@
 namespace dr {
 namespace {
 
-// Reads the rows first, first + step, ... below `end` of a column of vectors, kNormUnroll of them
-// at a time, and gives each to `use(vector)` in order. `Last`: nothing will read them again.
-template <typename T, int V, bool Last, typename Use>
-__device__ __forceinline__ void for_rows(const T* __restrict__ x, long long stride, int first,
-                                         int step, int end, Use use) {
-  using P = Packed<T, V>;
-  auto load = [](const T* at) {
-    return Last ? __ldcs(reinterpret_cast<const P*>(at)) : *reinterpret_cast<const P*>(at);
-  };
-  x += first * stride;
-  stride *= step;
-  int left = end - first;
-  for (; left > (kNormUnroll - 1) * step; left -= kNormUnroll * step) {
-    P p[kNormUnroll];
-#pragma unroll
-    for (int u = 0; u < kNormUnroll; ++u) {
-      p[u] = load(x);
-      x += stride;
-    }
-#pragma unroll
-    for (int u = 0; u < kNormUnroll; ++u) use(load_pairs<T, V>(p[u]));
-  }
-  if (left > 0) {
-    P p[kNormUnroll - 1];
-#pragma unroll
-    for (int u = 0; u < kNormUnroll - 1; ++u)
-      if (left > u * step) p[u] = load(x + u * stride);
-#pragma unroll
-    for (int u = 0; u < kNormUnroll - 1; ++u)
-      if (left > u * step) use(load_pairs<T, V>(p[u]));
-  }
-}
+constexpr int kStages = 8;  // rows that a thread has under way
 
 // Joins the threads' moments of a block's rows into those of the tile's groups: within a thread
 // over the neighbouring channels of a group, then over the rows, then over a group's columns (and
 // folded pixels).
+template <int V>
+constexpr size_t join_bytes() {
+  return sizeof(float2) * kNormThreads * (V + (V + 1) / 2);
+}
+
 template <int V, typename Done>
 __device__ __forceinline__ void join_block(Moments<V>& moments, const TileThread& t,
                                            const NormShape& s, const NormTile& tile, int rows,
-                                           Done done) {
-  __shared__ float2 entry[kNormThreads * V];
-  __shared__ float2 column[kNormThreads * V / 2];
+                                           void* shared, Done done) {
+  auto* entry = static_cast<float2*>(shared);   // [kNormThreads * V]
+  float2* column = entry + kNormThreads * V;    // [kNormThreads * V / 2]
   __shared__ float counts[kNormThreads];  // rows of each line of entries
+  __syncthreads();
   const int d = s.group_channels;
   // Channels folded within a thread: all that its vector has of a group, where vectors do not
   // straddle groups.
@@ -132,22 +107,25 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kNormThreads, 4) norm_stats_kernel(const T* __restrict__ x,
                                                                      NormShape s, int view0,
                                                                      float2* __restrict__ parts) {
+  extern __shared__ uint4 shared[];
   let_next_kernel_start();
   const NormBlock b = norm_block(s, V, view0, blockIdx.x);
   const TileThread t(b.tile.cols);
+  RowRing<T, V, 1, kStages> ring;
+  ring.at[0] = x + b.first * s.x_row + (b.tile.col + t.col) * V;
+  ring.stride[0] = s.x_row;
+  ring.start(shared, t, b.rows);
   Moments<V> moments;
   bool first = true;
 #pragma unroll
   for (int j = 0; j < Pairs<V>::kCount; ++j)
     moments.pivot.p[j] = moments.sum.p[j] = moments.square.p[j] = both(0.0f);
-  if (t.active)
-    for_rows<T, V, false>(x + b.first * s.x_row + (b.tile.col + t.col) * V, s.x_row, t.lane,
-                          t.lanes, b.rows, [&](const Pairs<V>& v) {
-      if (first) moments.start(v);
-      first = false;
-      moments.add(v);
-    });
-  join_block<V>(moments, t, s, b.tile, b.rows, [&](int item, float mean, float squares) {
+  ring.for_rows([&](const Pairs<V> (&v)[1]) {
+    if (first) moments.start(v[0]);
+    first = false;
+    moments.add(v[0]);
+  });
+  join_block<V>(moments, t, s, b.tile, b.rows, shared, [&](int item, float mean, float squares) {
     const long long group = static_cast<long long>(b.view) * s.groups + b.tile.group + item;
     parts[(group * s.pieces + b.piece) * s.chunks + b.chunk] = make_float2(mean, squares);
   });
@@ -237,12 +215,17 @@ template <typename T, int V, bool Silu, bool Drop>
 __global__ void __launch_bounds__(kNormThreads, 4) norm_apply_kernel(
     const T* __restrict__ x, NormShape s, int view0, NormParam weight, NormParam bias, float bound,
     DropKey key, const float* mean, const float* rstd, T* __restrict__ y) {
+  extern __shared__ uint4 shared[];
   let_next_kernel_start();
   const NormBlock b = norm_block(s, V, view0, gridDim.x - 1 - blockIdx.x);
   const TileThread t(b.tile.cols);
+  const int col = (b.tile.col + t.col) * V;
+  RowRing<T, V, 1, kStages> ring;
+  ring.at[0] = x + b.first * s.x_row + col;
+  ring.stride[0] = s.x_row;
+  ring.start(shared, t, b.rows);
   wait_for_kernel_before();
   if (!t.active) return;
-  const int col = (b.tile.col + t.col) * V;
   Pairs<V> m, a, c;  // z = (x + m) a + c
   if (V == 1) m.p[0].y = a.p[0].y = c.p[0].y = 0.0f;
   ChannelWalk walk(s, col);
@@ -258,12 +241,11 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_apply_kernel(
   const long long out_row = static_cast<long long>(s.channels) * s.fold;
   long long at = (b.first + t.lane) * out_row + col;
   const long long step = t.lanes * out_row;
-  for_rows<T, V, true>(x + b.first * s.x_row + col, s.x_row, t.lane, t.lanes, b.rows,
-                       [&](const Pairs<V>& v) {
+  ring.for_rows([&](const Pairs<V> (&v)[1]) {
     Pairs<V> z;
 #pragma unroll
     for (int j = 0; j < Pairs<V>::kCount; ++j)
-      z.p[j] = activate<Silu>(fma2(add2(v.p[j], m.p[j]), a.p[j], c.p[j]), bound);
+      z.p[j] = activate<Silu>(fma2(add2(v[0].p[j], m.p[j]), a.p[j], c.p[j]), bound);
     if (Drop) apply_dropout<V>(z, at, key, seed);
     __stcs(reinterpret_cast<Packed<T, V>*>(y + at), pack_pairs<T, V>(z));
     at += step;
@@ -277,18 +259,20 @@ int passes(const void* x, const NormShape& s, int dtype, const NormParam& weight
   const T* in = static_cast<const T*>(x);
   T* out = static_cast<T*>(y);
   const int most = views_at_once(s, dtype, 1);
+  constexpr size_t ring = RowRing<T, V, 1, kStages>::kBytes;
+  constexpr size_t shared = std::max(ring, join_bytes<V>());
   for (int view0 = 0; view0 < s.batch; view0 += most) {
     const int views = static_cast<int>(std::min<long long>(most, s.batch - view0));
     const unsigned int blocks = static_cast<unsigned int>(views) * s.tiles * s.chunks;
     const unsigned int groups = static_cast<unsigned int>(views) * s.groups;
-    cudaError_t err = launch_kernel(norm_stats_kernel<T, V>, blocks, kNormThreads, stream,
+    cudaError_t err = launch_kernel(norm_stats_kernel<T, V>, blocks, kNormThreads, shared, stream,
                                     view0 > 0, in, s, view0, parts);
     if (err == cudaSuccess)
-      err = launch_kernel(norm_join_kernel<V>, groups, kNormThreads, stream, true, parts, s, view0,
-                          eps, mean, rstd);
+      err = launch_kernel(norm_join_kernel<V>, groups, kNormThreads, 0, stream, true, parts, s,
+                          view0, eps, mean, rstd);
     if (err == cudaSuccess)
-      err = launch_kernel(norm_apply_kernel<T, V, Silu, Drop>, blocks, kNormThreads, stream, true,
-                          in, s, view0, weight, bias, bound, key, mean, rstd, out);
+      err = launch_kernel(norm_apply_kernel<T, V, Silu, Drop>, blocks, kNormThreads, ring, stream,
+                          true, in, s, view0, weight, bias, bound, key, mean, rstd, out);
     if (err != cudaSuccess) return static_cast<int>(err);
   }
   return launch_status();

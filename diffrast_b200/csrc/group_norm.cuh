@@ -352,6 +352,103 @@ struct TileThread {
   }
 };
 
+// Copies to shared memory (a 32-bit address) that run beside the thread. A copy of 2 bytes, which
+// the hardware does not have, is a load and a store.
+template <int Bytes>
+__device__ __forceinline__ void copy_async(unsigned int to, const void* from) {
+  if constexpr (Bytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else if constexpr (Bytes >= 4)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(Bytes)
+                 : "memory");
+  else
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(to),
+                 "h"(*static_cast<const unsigned short*>(from))
+                 : "memory");
+}
+__device__ __forceinline__ void copy_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int Pending>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(Pending) : "memory");
+}
+
+template <typename P>
+__device__ __forceinline__ P load_slot(unsigned int at) {
+  P p;
+  if constexpr (sizeof(P) == 16)
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(p.x), "=r"(p.y), "=r"(p.z), "=r"(p.w)
+                 : "r"(at)
+                 : "memory");
+  else if constexpr (sizeof(P) == 4)
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(p) : "r"(at) : "memory");
+  else
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(p) : "r"(at) : "memory");
+  return p;
+}
+
+// A thread's rows on their way to it: it copies its own vectors (of Images images) into its own
+// slots of shared memory, Stages rows ahead of the one it works on. No slot is shared, so the
+// copies need no barriers, and they hold no registers: with batches of loads in registers instead,
+// the sums of the backward pass read memory at 1.9 TB/s, for want of bytes under way.
+template <typename T, int V, int Images, int Stages>
+struct RowRing {
+  using P = Packed<T, V>;
+  static constexpr unsigned int kSlot = sizeof(P) * kNormThreads;
+  static constexpr size_t kBytes = static_cast<size_t>(kSlot) * Images * Stages;
+
+  const T* at[Images];
+  long long stride[Images];
+  unsigned int slots;
+  int count;
+
+  // Rows lane, lane + lanes, ... below `rows` of columns that start at at[].
+  __device__ __forceinline__ void start(void* shared, const TileThread& t, int rows) {
+    slots = static_cast<unsigned int>(__cvta_generic_to_shared(shared)) +
+            threadIdx.x * static_cast<unsigned int>(sizeof(P));
+    count = t.active && t.lane < rows ? (rows - t.lane + t.lanes - 1) / t.lanes : 0;
+#pragma unroll
+    for (int k = 0; k < Images; ++k) {
+      at[k] += t.lane * stride[k];
+      stride[k] *= t.lanes;
+    }
+#pragma unroll
+    for (int u = 0; u < Stages; ++u) {
+      if (u < count) fetch(u);
+      copy_commit();
+    }
+  }
+
+  __device__ __forceinline__ void fetch(int u) {
+#pragma unroll
+    for (int k = 0; k < Images; ++k) {
+      copy_async<sizeof(P)>(slots + (u * Images + k) * kSlot, at[k]);
+      at[k] += stride[k];
+    }
+  }
+
+  // Calls use(vectors) for the rows in order.
+  template <typename Use>
+  __device__ __forceinline__ void for_rows(Use use) {
+    for (int left = count; left > 0; left -= Stages) {
+#pragma unroll
+      for (int u = 0; u < Stages; ++u) {
+        if (u > 0 && u >= left) break;
+        copy_wait<Stages - 1>();
+        Pairs<V> v[Images];
+#pragma unroll
+        for (int k = 0; k < Images; ++k)
+          v[k] = load_pairs<T, V>(load_slot<P>(slots + (u * Images + k) * kSlot));
+        use(v);
+        if (u + Stages < left) fetch(u);
+        copy_commit();
+      }
+    }
+  }
+};
+
 // The kernels of a pass depend on one another and are launched with programmatic dependence: a
 // kernel's blocks may start while the last ones of the kernel before it run, and wait here before
 // they read its results (through pointers that are not __restrict__: a load that the compiler knows
@@ -427,13 +524,12 @@ inline NormVector choose_vector(long long pixels, int channels, int dtype, long 
 }
 
 // Cuts views into tiles of at most `most_cols` columns (at least the fewest whole groups that are
-// whole vectors) and chunks of rows of about `chunk_bytes`, whole steps of a block's threads of
-// `unroll` rows each where there are that many. Lowers v.vec where a group is wider than a block's
+// whole vectors) and chunks of rows of about `chunk_bytes`. Lowers v.vec where a group is wider than a block's
 // threads and not whole vectors (its tiles must not reach into the next group). False when there
 // would be too many blocks.
 inline bool cut_norm(NormShape& s, NormVector& v, long long batch, long long pixels, int channels,
                      int groups, int dtype, long long x_stride, long long grad_stride,
-                     int most_cols, long long chunk_bytes, int unroll) {
+                     int most_cols, long long chunk_bytes) {
   s.batch = batch;
   s.pixels = pixels;
   s.channels = channels;
@@ -468,8 +564,7 @@ inline bool cut_norm(NormShape& s, NormVector& v, long long batch, long long pix
   }
   const long long lanes = kNormThreads / s.tile_cols;  // rows that a block reads at once
   const long long tile_bytes = static_cast<long long>(s.tile_cols) * v.vec * dtype_bytes(dtype);
-  long long deep = chunk_bytes / tile_bytes / lanes;
-  if (deep > unroll) deep = deep / unroll * unroll;
+  const long long deep = chunk_bytes / tile_bytes / lanes;
   s.chunk_rows = static_cast<int>(std::max(1LL, std::min<long long>(deep, kMomentRows)) * lanes);
   const long long chunks = (s.rows + s.chunk_rows - 1) / s.chunk_rows;
   if (chunks > kMaxNormBlocks || batch > kMaxNormBlocks / s.tiles ||
@@ -481,8 +576,6 @@ inline bool cut_norm(NormShape& s, NormVector& v, long long batch, long long pix
 
 // The plan of a call in passes over memory. Chunks are 64 KB, less where that would leave
 // processors idle, more where a view would have over a thousand.
-constexpr int kNormUnroll = 4;
-
 inline bool plan_passes(NormShape& s, NormVector& v, long long batch, long long pixels,
                         int channels, int groups, int dtype, long long x_stride,
                         long long grad_stride) {
@@ -490,7 +583,7 @@ inline bool plan_passes(NormShape& s, NormVector& v, long long batch, long long 
   const long long chunk = std::max(
       view / 1024, std::max(4096LL, std::min(65536LL, batch * view / (4 * 148))));
   return cut_norm(s, v, batch, pixels, channels, groups, dtype, x_stride, grad_stride, kNormThreads,
-                  chunk, kNormUnroll);
+                  chunk);
 }
 
 // Views that are taken together, first pass and second: as many as stay in L2 in between.
@@ -537,10 +630,11 @@ inline size_t norm_workspace_bytes(long long batch, long long pixels, int channe
 // Launches a kernel on a stream, with programmatic dependence on the one before it if `after`.
 template <typename... Params, typename... Args>
 cudaError_t launch_kernel(void (*kernel)(Params...), unsigned int blocks, unsigned int threads,
-                          cudaStream_t stream, bool after, Args... args) {
+                          size_t shared, cudaStream_t stream, bool after, Args... args) {
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(blocks);
   config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = shared;
   config.stream = stream;
   cudaLaunchAttribute attribute = {};
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -7,7 +7,7 @@
 namespace dr {
 namespace {
 
-constexpr int kUnroll = 2;  // vectors of x, and as many of the gradient, a thread has under way
+constexpr int kStages = 4;  // rows of x and of the gradient that a thread has under way
 
 // Constants of a thread's channels: z = (x + shift) scale + bias.
 template <int V>
@@ -35,8 +35,10 @@ struct Channels {
 // tile.
 template <int V, typename Done>
 __device__ __forceinline__ void join_block(Pairs<V>& sum, Pairs<V>& dot, const TileThread& t,
-                                           const NormShape& s, const NormTile& tile, Done done) {
-  __shared__ float2 entry[kNormThreads * V];
+                                           const NormShape& s, const NormTile& tile, void* shared,
+                                           Done done) {
+  auto* entry = static_cast<float2*>(shared);  // [kNormThreads * V]
+  __syncthreads();
   const int width = tile.cols * V;
   int rows = t.lanes, row = t.lane;
   bool write = t.active;
@@ -66,41 +68,6 @@ __device__ __forceinline__ void join_block(Pairs<V>& sum, Pairs<V>& dot, const T
   join_sums(items, rows * s.fold, [&](int item, int i) { return entry[i * items + item]; }, done);
 }
 
-// Gives the vectors of x and of the gradient in the rows first, first + step, ... below `end` of a
-// column to `use(x, gradient)` in order, kUnroll of them at a time. `Last`: nothing will read them
-// again.
-template <typename T, int V, bool Last, typename Use>
-__device__ __forceinline__ void for_rows(const T* __restrict__ x, long long x_row,
-                                         const T* __restrict__ grad, long long grad_row, int first,
-                                         int step, int end, Use use) {
-  using P = Packed<T, V>;
-  auto load = [](const T* at) {
-    return Last ? __ldcs(reinterpret_cast<const P*>(at)) : *reinterpret_cast<const P*>(at);
-  };
-  x += first * x_row;
-  grad += first * grad_row;
-  x_row *= step;
-  grad_row *= step;
-  int left = end - first;
-  for (; left > (kUnroll - 1) * step; left -= kUnroll * step) {
-    P p[kUnroll], g[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      p[u] = load(x);
-      g[u] = load(grad);
-      x += x_row;
-      grad += grad_row;
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) use(load_pairs<T, V>(p[u]), load_pairs<T, V>(g[u]));
-  }
-  for (; left > 0; left -= step) {
-    use(load_pairs<T, V>(load(x)), load_pairs<T, V>(load(grad)));
-    x += x_row;
-    grad += grad_row;
-  }
-}
-
 // First pass: sums of q and q (x - m) of each channel over one chunk of rows in one tile of columns.
 // parts [batch][chunks][channels].
 template <typename T, int V, bool Silu, bool Drop>
@@ -108,10 +75,17 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_sums_kernel(
     const T* __restrict__ x, const T* __restrict__ grad, NormShape s, int view0, NormParam weight,
     NormParam bias, float bound, DropKey key, const float* __restrict__ mean,
     const float* __restrict__ rstd, float2* __restrict__ parts) {
+  extern __shared__ uint4 shared[];
   let_next_kernel_start();
   const NormBlock b = norm_block(s, V, view0, blockIdx.x);
   const TileThread t(b.tile.cols);
   const int col = (b.tile.col + t.col) * V;
+  RowRing<T, V, 2, kStages> ring;
+  ring.at[0] = x + b.first * s.x_row + col;
+  ring.at[1] = grad + b.first * s.grad_row + col;
+  ring.stride[0] = s.x_row;
+  ring.stride[1] = s.grad_row;
+  ring.start(shared, t, b.rows);
   Pairs<V> sum, dot;
 #pragma unroll
   for (int j = 0; j < Pairs<V>::kCount; ++j) sum.p[j] = dot.p[j] = both(0.0f);
@@ -122,23 +96,21 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_sums_kernel(
     const long long out_row = static_cast<long long>(s.channels) * s.fold;
     long long at = (b.first + t.lane) * out_row + col;
     const long long step = t.lanes * out_row;
-    for_rows<T, V, false>(x + b.first * s.x_row + col, s.x_row, grad + b.first * s.grad_row + col,
-                          s.grad_row, t.lane, t.lanes, b.rows,
-                          [&](const Pairs<V>& v, Pairs<V> q) {
-      if (Drop) apply_dropout<V>(q, at, key, seed);
+    ring.for_rows([&](Pairs<V> (&v)[2]) {
+      if (Drop) apply_dropout<V>(v[1], at, key, seed);
       at += step;
 #pragma unroll
       for (int j = 0; j < Pairs<V>::kCount; ++j) {
-        const float2 d = add2(v.p[j], c.shift.p[j]);
+        const float2 d = add2(v[0].p[j], c.shift.p[j]);
         const float2 z = fma2(d, c.scale.p[j], c.bias.p[j]);
-        const float2 u = activate_grad<Silu>(q.p[j], z, bound);
+        const float2 u = activate_grad<Silu>(v[1].p[j], z, bound);
         sum.p[j] = add2(sum.p[j], u);
         dot.p[j] = fma2(u, d, dot.p[j]);
       }
     });
   }
   const int first = s.fold > 1 ? 0 : b.tile.col * V;
-  join_block<V>(sum, dot, t, s, b.tile, [&](int item, float2 total) {
+  join_block<V>(sum, dot, t, s, b.tile, shared, [&](int item, float2 total) {
     parts[(static_cast<long long>(b.view) * s.chunks + b.chunk) * s.channels + first + item] = total;
   });
   wait_for_kernel_before();
@@ -218,10 +190,17 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_grad_kernel(
     const T* __restrict__ x, const T* __restrict__ grad, NormShape s, int view0, NormParam weight,
     NormParam bias, float bound, DropKey key, const float* __restrict__ mean,
     const float* __restrict__ rstd, const float2* means, T* __restrict__ grad_x) {
+  extern __shared__ uint4 shared[];
   let_next_kernel_start();
   const NormBlock b = norm_block(s, V, view0, gridDim.x - 1 - blockIdx.x);
   const TileThread t(b.tile.cols);
   const int col = (b.tile.col + t.col) * V;
+  RowRing<T, V, 2, kStages> ring;
+  ring.at[0] = x + b.first * s.x_row + col;
+  ring.at[1] = grad + b.first * s.grad_row + col;
+  ring.stride[0] = s.x_row;
+  ring.stride[1] = s.grad_row;
+  ring.start(shared, t, b.rows);
   Channels<V> c;
   if (t.active) c.load(s, b.view, col, weight, bias, mean, rstd);
   wait_for_kernel_before();
@@ -242,17 +221,16 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_grad_kernel(
   const long long out_row = static_cast<long long>(s.channels) * s.fold;
   long long at = (b.first + t.lane) * out_row + col;
   const long long step = t.lanes * out_row;
-  for_rows<T, V, true>(x + b.first * s.x_row + col, s.x_row, grad + b.first * s.grad_row + col,
-                       s.grad_row, t.lane, t.lanes, b.rows, [&](Pairs<V> v, Pairs<V> q) {
-    if (Drop) apply_dropout<V>(q, at, key, seed);
+  ring.for_rows([&](Pairs<V> (&v)[2]) {
+    if (Drop) apply_dropout<V>(v[1], at, key, seed);
 #pragma unroll
     for (int j = 0; j < Pairs<V>::kCount; ++j) {
-      const float2 d = add2(v.p[j], c.shift.p[j]);
+      const float2 d = add2(v[0].p[j], c.shift.p[j]);
       const float2 z = fma2(d, c.scale.p[j], c.bias.p[j]);
-      const float2 u = activate_grad<Silu>(q.p[j], z, bound);
-      v.p[j] = fma2(u, c.scale.p[j], fma2(d, slope.p[j], base.p[j]));
+      const float2 u = activate_grad<Silu>(v[1].p[j], z, bound);
+      v[0].p[j] = fma2(u, c.scale.p[j], fma2(d, slope.p[j], base.p[j]));
     }
-    __stcs(reinterpret_cast<Packed<T, V>*>(grad_x + at), pack_pairs<T, V>(v));
+    __stcs(reinterpret_cast<Packed<T, V>*>(grad_x + at), pack_pairs<T, V>(v[0]));
     at += step;
   });
 }
@@ -309,24 +287,26 @@ int passes(const void* x, const void* grad, const NormShape& s, int dtype, const
   const int run_groups = std::max(1, std::min(s.groups, 32 / s.group_channels));
   const int runs = (s.groups + run_groups - 1) / run_groups;
   const int most = views_at_once(s, dtype, 2);
+  constexpr size_t ring = RowRing<T, V, 2, kStages>::kBytes;
+  constexpr size_t shared = std::max(ring, sizeof(float2) * kNormThreads * V);
   cudaError_t err = cudaSuccess;
   for (int view0 = 0; view0 < s.batch; view0 += most) {
     const int views = static_cast<int>(std::min<long long>(most, s.batch - view0));
     const unsigned int blocks = static_cast<unsigned int>(views) * s.tiles * s.chunks;
-    err = launch_kernel(norm_sums_kernel<T, V, Silu, Drop>, blocks, kNormThreads, stream,
+    err = launch_kernel(norm_sums_kernel<T, V, Silu, Drop>, blocks, kNormThreads, shared, stream,
                         view0 > 0, in, dy, s, view0, weight, bias, bound, key, mean, rstd, parts);
     if (err == cudaSuccess)
       err = launch_kernel(norm_means_kernel, static_cast<unsigned int>(views) * runs,
-                          kMeansThreads, stream, true, parts, s, view0, weight, runs, run_groups,
+                          kMeansThreads, 0, stream, true, parts, s, view0, weight, runs, run_groups,
                           rstd, sums, means);
     if (err == cudaSuccess && out.x != nullptr)
-      err = launch_kernel(norm_grad_kernel<T, V, Silu, Drop>, blocks, kNormThreads, stream, true,
+      err = launch_kernel(norm_grad_kernel<T, V, Silu, Drop>, blocks, kNormThreads, ring, stream, true,
                           in, dy, s, view0, weight, bias, bound, key, mean, rstd, means,
                           static_cast<T*>(out.x));
     if (err != cudaSuccess) return static_cast<int>(err);
   }
   if (out.weight != nullptr || out.bias != nullptr)
-    err = launch_kernel(norm_params_kernel, blocks_for(s.channels, 32), kNormThreads, stream, true,
+    err = launch_kernel(norm_params_kernel, blocks_for(s.channels, 32), kNormThreads, 0, stream, true,
                         sums, s.batch, s.channels, out.weight, out.weight_dtype, out.weight_views,
                         out.bias, out.bias_dtype, out.bias_views);
   return err == cudaSuccess ? launch_status() : static_cast<int>(err);
