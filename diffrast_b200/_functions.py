@@ -713,18 +713,20 @@ class GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, weight: Tensor | None, bias: Tensor | None, seed: Tensor | None,
                 groups: int, eps: float, activation: int, drop: K.Drop):
-        y, stats = K.group_norm_fwd(x, groups, weight, bias, eps, activation,
+        y, state = K.group_norm_fwd(x, groups, weight, bias, eps, activation,
                                     drop._replace(seed=seed))
-        ctx.save_for_backward(*(_saveable(t) for t in (x, weight, bias, seed, stats)))
+        ctx.save_for_backward(*(_saveable(t) for t in (x, weight, bias, seed, state)))
         ctx.groups, ctx.activation, ctx.drop = groups, activation, drop
         return y
 
     @staticmethod
     @first_order("group_norm")
     def backward(ctx, grad_out):
-        x, weight, bias, seed, stats = ctx.saved_tensors
-        grads = K.group_norm_bwd(x, grad_out, ctx.groups, weight, bias, stats, ctx.activation,
-                                 ctx.drop._replace(seed=seed), ctx.needs_input_grad[:3])
+        x, weight, bias, seed, state = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        grads = K.group_norm_bwd(x, grad_out, ctx.groups, weight if need[1] else None,
+                                 bias if need[2] else None, state, ctx.activation,
+                                 ctx.drop._replace(seed=seed), need[0])
         return *grads, None, None, None, None, None
 
 

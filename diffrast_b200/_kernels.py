@@ -811,49 +811,48 @@ def _param(t: Tensor | None, channels: int) -> tuple[int | None, int, int]:
 @timed("group_norm_fwd")
 def group_norm_fwd(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None, eps: float,
                    activation: int, drop: Drop) -> tuple[Tensor, Tensor]:
-    """``(y, stats)``: the normalised image and ``[2, batch, groups]`` means and reciprocal
-    standard deviations. ``x`` is ``[batch, ..., channels]`` and not empty."""
+    """``(y, state)``: the normalised image and what the backward pass needs beside ``x``.
+    ``x`` is ``[batch, ..., channels]`` and not empty."""
     x, stride = feature_rows(x)
     batch, channels = x.shape[0], x.shape[-1]
     pixels = x.numel() // (batch * channels)
     dtype = N.FEATURE_DTYPES[x.dtype]
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, batch, groups), dtype=torch.float32, device=x.device)
+    state = torch.empty(batch * (3 * channels + groups), dtype=torch.float32, device=x.device)
     work = _scratch(_norm_workspace_bytes(batch, pixels, channels, groups, dtype, 0), x.device)
-    mean = stats.data_ptr()
     N.check(
         N.lib().dr_group_norm_fwd(x.data_ptr(), stride, dtype, batch, pixels, channels, groups,
                                   *_param(weight, channels), *_param(bias, channels), eps,
                                   activation, drop.threshold, N.ptr(drop.seed), drop.value,
-                                  drop.layer, y.data_ptr(), mean, mean + 4 * batch * groups,
-                                  work.data_ptr(), work.numel(), N.stream(x.device)),
+                                  drop.layer, y.data_ptr(), state.data_ptr(), work.data_ptr(),
+                                  work.numel(), N.stream(x.device)),
         "dr_group_norm_fwd",
     )  # fmt: skip
-    return y, stats
+    return y, state
 
 
 @timed("group_norm_bwd")
 def group_norm_bwd(x: Tensor, grad_y: Tensor, groups: int, weight: Tensor | None,
-                   bias: Tensor | None, stats: Tensor, activation: int, drop: Drop,
-                   need: tuple[bool, bool, bool]) -> tuple[Tensor | None, ...]:
-    """Gradients of x (contiguous), weight and bias, None where not needed."""
+                   bias: Tensor | None, state: Tensor, activation: int, drop: Drop,
+                   need_x: bool) -> tuple[Tensor | None, ...]:
+    """Gradients of x (contiguous), weight and bias: into new tensors like ``weight`` and ``bias``,
+    which are None where no gradient is needed."""
     x, stride = feature_rows(x)
     grad_y, grad_stride = feature_rows(grad_y)
     batch, channels = x.shape[0], x.shape[-1]
     pixels = x.numel() // (batch * channels)
     dtype = N.FEATURE_DTYPES[x.dtype]
-    grad_x = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-    grad_w = torch.empty_like(weight) if need[1] else None
-    grad_b = torch.empty_like(bias) if need[2] else None
+    grad_x = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+    grad_w = None if weight is None else torch.empty_like(weight)
+    grad_b = None if bias is None else torch.empty_like(bias)
     work = _scratch(_norm_workspace_bytes(batch, pixels, channels, groups, dtype, 1), x.device)
-    mean = stats.data_ptr()
     N.check(
         N.lib().dr_group_norm_bwd(x.data_ptr(), stride, grad_y.data_ptr(), grad_stride, dtype,
-                                  batch, pixels, channels, groups, *_param(weight, channels),
-                                  *_param(bias, channels), mean, mean + 4 * batch * groups,
-                                  activation, drop.threshold, N.ptr(drop.seed), drop.value,
-                                  drop.layer, N.ptr(grad_x), N.ptr(grad_w), N.ptr(grad_b),
-                                  work.data_ptr(), work.numel(), N.stream(x.device)),
+                                  batch, pixels, channels, groups, state.data_ptr(), activation,
+                                  drop.threshold, N.ptr(drop.seed), drop.value, drop.layer,
+                                  N.ptr(grad_x), *_param(grad_w, channels),
+                                  *_param(grad_b, channels), work.data_ptr(), work.numel(),
+                                  N.stream(x.device)),
         "dr_group_norm_bwd",
     )  # fmt: skip
     return grad_x, grad_w, grad_b

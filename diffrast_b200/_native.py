@@ -153,17 +153,18 @@ _SIGNATURES = {
     "dr_group_norm_workspace_bytes": (
         c_size_t, [c_int64, c_int64, c_int32, c_int32, c_int32, c_int32]
     ),
+    "dr_group_norm_state_floats": (c_size_t, [c_int64, c_int32, c_int32]),
     "dr_group_norm_fwd": (
         c_int,
         [_P, c_int64, c_int32, c_int64, c_int64, c_int32, c_int32, _P, c_int32, c_int64, _P,
-         c_int32, c_int64, c_float, c_int32, c_int32, _P, c_int64, c_int64, _P, _P, _P, _P,
-         c_size_t, _P],
+         c_int32, c_int64, c_float, c_int32, c_int32, _P, c_int64, c_int64, _P, _P, _P, c_size_t,
+         _P],
     ),
     "dr_group_norm_bwd": (
         c_int,
         [_P, c_int64, _P, c_int64, c_int32, c_int64, c_int64, c_int32, c_int32, _P, c_int32,
-         c_int64, _P, c_int32, c_int64, _P, _P, c_int32, c_int32, _P, c_int64, c_int64, _P, _P,
-         _P, _P, c_size_t, _P],
+         c_int32, _P, c_int64, c_int64, _P, _P, c_int32, c_int64, _P, c_int32, c_int64, _P,
+         c_size_t, _P],
     ),
     "dr_zero": (c_int, [_P, c_size_t, _P]),
     "dr_checked_build": (c_int, []),

@@ -7,245 +7,190 @@ namespace {
 
 constexpr int kStages = 8;  // rows that a thread has under way
 
-// Joins the threads' moments of a block's rows into those of the tile's groups: within a thread
-// over the neighbouring channels of a group, then over the rows, then over a group's columns (and
-// folded pixels).
-template <int V>
-constexpr size_t join_bytes() {
-  return sizeof(float2) * kNormThreads * (V + (V + 1) / 2);
-}
-
+// Joins the threads' moments of a block's rows into those of each channel: over the rows of a warp
+// where the tile's columns divide it, then over the lines of rows that are left. `done` gets the
+// channel, counted from the tile's first, and the moment.
 template <int V, typename Done>
-__device__ __forceinline__ void join_block(Moments<V>& moments, const TileThread& t,
-                                           const NormShape& s, const NormTile& tile, int rows,
+__device__ __forceinline__ void join_block(Moments<V>& m, const NormPlace& p, const NormShape& s,
                                            void* shared, Done done) {
-  auto* entry = static_cast<float2*>(shared);   // [kNormThreads * V]
-  float2* column = entry + kNormThreads * V;    // [kNormThreads * V / 2]
-  __shared__ float counts[kNormThreads];  // rows of each line of entries
-  __syncthreads();
-  const int d = s.group_channels;
-  // Channels folded within a thread: all that its vector has of a group, where vectors do not
-  // straddle groups.
-  int q = d % V == 0 ? V : V % d == 0 ? d : 1;
-  const int per = V / q, width = tile.cols * per;
-  const int mine = t.active && t.lane < rows ? (rows - t.lane + t.lanes - 1) / t.lanes : 0;
-  int lines = t.lanes, line = t.lane;
-  bool write = t.active;
-  float n = static_cast<float>(mine);
-  if (tile.cols < 32 && 32 % tile.cols == 0) {
-    // A tile's columns divide the warp: its rows are joined first.
-    moments.move_pivot(threadIdx.x % tile.cols, n);
-    for (int d = tile.cols; d < 32; d *= 2) {
-      moments.add_lane(d);
-      n += __shfl_xor_sync(0xFFFFFFFFu, n, d);
-    }
+  auto* entry = static_cast<float2*>(shared);  // [lines][tile_cols * V]
+  __shared__ float counts[kNormThreads];       // of the lines
+  float n = static_cast<float>(p.count);
+  m.finish(n);
+  int lines = s.lanes, line = threadIdx.y;
+  bool write = true;
+  if (warp_holds_rows()) {
+    for (int d = blockDim.x; d < 32; d *= 2) m.join_lane(d, n);
+    const int thread = threadIdx.y * blockDim.x + threadIdx.x;
     lines = kNormThreads / 32;
-    line = threadIdx.x / 32;
-    write = threadIdx.x % 32 < tile.cols;
+    line = thread / 32;
+    write = thread % 32 < blockDim.x;
   }
-  if (write && t.col == 0) counts[line] = n;
+  const int width = s.tile_cols * V;
+  __syncthreads();
   if (write) {
-    const float inverse = n > 0.0f ? 1.0f / n : 0.0f;
-    float2* to = entry + (line * tile.cols + t.col) * per;
-    auto fold = [&](auto count) {
-      constexpr int Q = decltype(count)::value;
+    float2* to = entry + line * width + threadIdx.x * V;
 #pragma unroll
-      for (int j = 0; j < V / Q; ++j)
-        to[j] = n > 0.0f ? fold_channels<Q>(moments, j * Q, n, inverse) : both(0.0f);
-    };
-    if (q == V) {
-      fold(std::integral_constant<int, V>());
-    } else if constexpr (V > 1) {
-      if (q == 1) fold(std::integral_constant<int, 1>());
-      if constexpr (V > 2) {
-        if (q == 2) fold(std::integral_constant<int, 2>());
-      }
-      if constexpr (V > 4) {
-        if (q == 4) fold(std::integral_constant<int, 4>());
-      }
-    }
+    for (int j = 0; j < V; ++j) to[j] = make_float2(m.sum.get(j), m.square.get(j));
+    if (threadIdx.x == 0) counts[line] = n;
   }
   __syncthreads();
-  const int members = (s.pieces > 1 ? tile.cols * V : s.fold * d) / q;  // columns of a group
-  const float weight = static_cast<float>(q);
-  if (members == 1) {
-    join_moments(
-        width, lines,
-        [&](int item, int i, float2& v) {
-          v = entry[i * width + item];
-          return weight * counts[i];
-        },
-        done);
-    return;
+  const int items = s.fold > 1 ? s.channels : width;
+  const int valid = s.fold > 1 ? items : min(width, s.cols * V - (p.col - static_cast<int>(threadIdx.x) * V));
+  for (int item = threadIdx.y * blockDim.x + threadIdx.x; item < valid;
+       item += blockDim.x * blockDim.y) {
+    const float2 first = entry[item];
+    float total_n = 0.0f, total = 0.0f;
+    for (int l = 0; l < lines; ++l) {
+      const float c = counts[l];
+      for (int f = 0; f < s.fold; ++f) {
+        total_n += c;
+        total = fmaf(c, entry[l * width + f * items + item].x - first.x, total);
+      }
+    }
+    const float offset = __fdividef(total, total_n);
+    float squares = 0.0f;
+    for (int l = 0; l < lines; ++l) {
+      const float c = counts[l];
+      for (int f = 0; f < s.fold; ++f) {
+        const float2 v = entry[l * width + f * items + item];
+        const float d = v.x - first.x - offset;
+        squares += fmaf(c * d, d, v.y);
+      }
+    }
+    done(item, make_float2(first.x + offset, squares));
   }
-  const float2* from = entry;
-  if (lines > 1) {
-    join_moments(
-        width, lines,
-        [&](int item, int i, float2& v) {
-          v = entry[i * width + item];
-          return weight * counts[i];
-        },
-        [&](int item, float mean, float squares) { column[item] = make_float2(mean, squares); });
-    __syncthreads();
-    from = column;
-  }
-  const int span = s.fold > 1 ? d / q : members;  // neighbouring columns of a group
-  join_moments(
-      tile.groups, members,
-      [&](int item, int i, float2& v) {
-        const int f = s.fold > 1 ? i / span : 0;
-        v = from[f * (s.channels / q) + item * span + i - f * span];
-        return weight * static_cast<float>(rows);
-      },
-      done);
 }
 
-// First pass: the statistics of one chunk of rows in one tile of columns.
-// parts [batch][groups][pieces][chunks].
+// First pass: the moments of each channel over one chunk of rows in one tile of columns.
+// parts [batch][chunks][channels] of (mean, squared deviations).
 template <typename T, int V>
 __global__ void __launch_bounds__(kNormThreads, 4) norm_stats_kernel(const T* __restrict__ x,
                                                                      NormShape s, int view0,
                                                                      float2* __restrict__ parts) {
   extern __shared__ uint4 shared[];
   let_next_kernel_start();
-  const NormBlock b = norm_block(s, V, view0, blockIdx.x);
-  const TileThread t(b.tile.cols);
+  const NormPlace p(s, V, view0 + blockIdx.z, blockIdx.y, blockIdx.x);
   RowRing<T, V, 1, kStages> ring;
-  ring.at[0] = x + b.first * s.x_row + (b.tile.col + t.col) * V;
-  ring.stride[0] = s.x_row;
-  ring.start(shared, t, b.rows);
-  Moments<V> moments;
+  ring.image(0, x, s.x_row, p, s.lanes);
+  ring.start(shared, p.count);
+  Moments<V> m;
+  m.clear();
   bool first = true;
-#pragma unroll
-  for (int j = 0; j < Pairs<V>::kCount; ++j)
-    moments.pivot.p[j] = moments.sum.p[j] = moments.square.p[j] = both(0.0f);
   ring.for_rows([&](const Pairs<V> (&v)[1]) {
-    if (first) moments.start(v[0]);
+    if (first) m.start(v[0]);
     first = false;
-    moments.add(v[0]);
+    m.add(v[0]);
   });
-  join_block<V>(moments, t, s, b.tile, b.rows, shared, [&](int item, float mean, float squares) {
-    const long long group = static_cast<long long>(b.view) * s.groups + b.tile.group + item;
-    parts[(group * s.pieces + b.piece) * s.chunks + b.chunk] = make_float2(mean, squares);
-  });
+  parts += (static_cast<long long>(p.view) * s.chunks + p.chunk) * s.channels;
+  if (s.fold == 1) parts += blockIdx.y * s.tile_cols * V;
+  join_block<V>(m, p, s, shared, [&](int item, float2 moment) { parts[item] = moment; });
   wait_for_kernel_before();
 }
 
-// Sums over a block, for all of its threads.
-__device__ __forceinline__ float block_sum(float v, float* shared) {
-  v = lane_sum(v, 32);
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = v;
-  __syncthreads();
-  float total = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kNormThreads / 32; ++i) total += shared[i];
-  return total;
-}
-
-// Joins the parts of one view and group: kJoin of them for each thread at a time, kept in registers
-// between the sum that gives their mean and the sum of squares about it; then with those before.
-constexpr int kJoin = 4;
-
-template <int V>
-__global__ void __launch_bounds__(kNormThreads) norm_join_kernel(const float2* parts,
-                                                                 NormShape s, int view0, float eps,
-                                                                 float* __restrict__ mean,
-                                                                 float* __restrict__ rstd) {
-  __shared__ float shared[kNormThreads / 32];
+// Joins the parts of a view's channels and the channels of its groups, and leaves the constants of
+// the second pass: table [batch][3][channels] of -mean, rstd * weight and bias.
+__global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(
+    const float2* parts, NormShape s, int view0, NormParam weight, NormParam bias, float eps,
+    float* __restrict__ rstd, float* __restrict__ table) {
+  __shared__ float2 entry[32][33];
+  __shared__ Moment channel[32];
+  __shared__ float2 result;  // of a group wider than 32 channels
   let_next_kernel_start();
   wait_for_kernel_before();
-  const long long group = static_cast<long long>(view0) * s.groups + blockIdx.x;
-  const int count = s.pieces * s.chunks;
-  parts += group * count;
-  const float2 pivot = parts[0];
-  float all = 0.0f, all_mean = 0.0f, all_squares = 0.0f;
-  for (int base = 0; base < count; base += kJoin * kNormThreads) {
-    float2 v[kJoin];
-    float n[kJoin];
-    float total_n = 0.0f, total = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kJoin; ++k) {
-      const int i = base + k * kNormThreads + threadIdx.x;
-      v[k] = pivot;
-      n[k] = 0.0f;
-      if (i < count) {
-        v[k] = parts[i];
-        const int piece = s.pieces > 1 ? i / s.chunks : 0, chunk = i - piece * s.chunks;
-        const long long rows = min(static_cast<long long>(s.chunk_rows),
-                                   s.rows - static_cast<long long>(chunk) * s.chunk_rows);
-        const int width = s.pieces > 1
-                              ? min(s.tile_cols, s.group_cols - piece * s.tile_cols) * V
-                              : s.group_channels * s.fold;
-        n[k] = static_cast<float>(rows) * static_cast<float>(width);
+  const JoinPlace p(s, view0);
+  const int x = threadIdx.x % 32, y = threadIdx.x / 32;
+  const int d = s.group_channels;
+  parts += static_cast<long long>(p.view) * s.chunks * s.channels + p.channel;
+  table += static_cast<long long>(p.view) * 3 * s.channels;
+  rstd += static_cast<long long>(p.view) * s.groups;
+  const float chunk_count = static_cast<float>(s.chunk_rows) * static_cast<float>(s.fold);
+  const float last_count =
+      static_cast<float>(s.rows - static_cast<long long>(s.chunks - 1) * s.chunk_rows) *
+      static_cast<float>(s.fold);
+  auto write = [&](int c, float mean, float r) {
+    table[c] = -mean;
+    table[s.channels + c] = r * load_scale(weight, p.view, c);
+    table[2 * s.channels + c] = load_shift(bias, p.view, c);
+  };
+  Moment wide = {0.0f, 0.0f, 0.0f};
+  for (int base = 0; base < p.channels; base += 32) {
+    // This lane's chunks of channel x.
+    Moment m = {0.0f, 0.0f, 0.0f};
+    if (base + x < p.channels) {
+#pragma unroll 8
+      for (int i = y; i < s.chunks; i += 32) {
+        const float2 v = parts[static_cast<long long>(i) * s.channels + base + x];
+        m.join({i + 1 < s.chunks ? chunk_count : last_count, v.x, v.y});
       }
     }
-#pragma unroll
-    for (int k = 0; k < kJoin; ++k) {
-      total_n += n[k];
-      total = fmaf(n[k], v[k].x - pivot.x, total);
+    entry[y][x] = make_float2(m.mean, m.squares);
+    __syncthreads();
+    // Channel y, from its 32 lanes; lane i has ceil((chunks - i) / 32) chunks.
+    const float2 v = entry[x][y];
+    const int chunks = x < s.chunks ? (s.chunks - x + 31) / 32 : 0;
+    const bool last = chunks > 0 && (s.chunks - 1) % 32 == x;
+    m = {chunk_count * static_cast<float>(chunks - (last ? 1 : 0)) + (last ? last_count : 0.0f),
+         v.x, v.y};
+    m.join_warp();
+    if (x == 0) channel[y] = base + y < p.channels ? m : Moment{0.0f, 0.0f, 0.0f};
+    __syncthreads();
+    if (y == 0) {
+      m = channel[x];
+      if (d > 32) {
+        m.join_warp();
+        if (base == 0)
+          wide = m;
+        else
+          wide.join(m);
+      } else if (x < p.channels) {
+        const int g = x / d;
+        Moment group = channel[g * d];
+        for (int i = 1; i < d; ++i) group.join(channel[g * d + i]);
+        const float r = rstd_of(group, eps);
+        if (x == g * d) rstd[p.group + g] = r;
+        write(p.channel + x, group.mean, r);
+      }
     }
-    total_n = block_sum(total_n, shared);
-    total = block_sum(total, shared);
-    const float m = total / total_n;  // about the pivot
-    float squares = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kJoin; ++k) {
-      const float d = v[k].x - pivot.x - m;
-      squares += n[k] > 0.0f ? fmaf(n[k] * d, d, v[k].y) : 0.0f;
-    }
-    squares = block_sum(squares, shared);
-    const float sum_n = all + total_n, d = m - all_mean;
-    all_squares += squares + d * d * (all * (total_n / sum_n));
-    all_mean += d * (total_n / sum_n);
-    all = sum_n;
+    __syncthreads();
   }
+  if (d <= 32) return;
   if (threadIdx.x == 0) {
-    const float m = pivot.x + all_mean;
-    const float values = static_cast<float>(s.pixels) * static_cast<float>(s.group_channels);
-    mean[group] = m;
-    rstd[group] = rsqrtf(variance_of(m, all_squares, values) + eps);
+    result = make_float2(wide.mean, rstd_of(wide, eps));
+    rstd[p.group] = result.y;
   }
+  __syncthreads();
+  for (int c = threadIdx.x; c < p.channels; c += kJoinThreads)
+    write(p.channel + c, result.x, result.y);
 }
 
 // Second pass: normalise, scale, activate and drop one chunk of rows in one tile of columns. Blocks
 // run from the end of the views to their start: what the first pass read last is still in L2.
 template <typename T, int V, bool Silu, bool Drop>
 __global__ void __launch_bounds__(kNormThreads, 4) norm_apply_kernel(
-    const T* __restrict__ x, NormShape s, int view0, NormParam weight, NormParam bias, float bound,
-    DropKey key, const float* mean, const float* rstd, T* __restrict__ y) {
+    const T* __restrict__ x, NormShape s, int view0, const float* table, float bound, DropKey key,
+    T* __restrict__ y) {
   extern __shared__ uint4 shared[];
   let_next_kernel_start();
-  const NormBlock b = norm_block(s, V, view0, gridDim.x - 1 - blockIdx.x);
-  const TileThread t(b.tile.cols);
-  const int col = (b.tile.col + t.col) * V;
+  const NormPlace p(s, V, view0 + gridDim.z - 1 - blockIdx.z, gridDim.y - 1 - blockIdx.y,
+                    gridDim.x - 1 - blockIdx.x);
   RowRing<T, V, 1, kStages> ring;
-  ring.at[0] = x + b.first * s.x_row + col;
-  ring.stride[0] = s.x_row;
-  ring.start(shared, t, b.rows);
+  ring.image(0, x, s.x_row, p, s.lanes);
+  ring.start(shared, p.count);
   wait_for_kernel_before();
-  if (!t.active) return;
-  Pairs<V> m, a, c;  // z = (x + m) a + c
-  if (V == 1) m.p[0].y = a.p[0].y = c.p[0].y = 0.0f;
-  ChannelWalk walk(s, col);
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const long long group = static_cast<long long>(b.view) * s.groups + walk.group;
-    m.set(j, -mean[group]);
-    a.set(j, rstd[group] * load_scale(weight, b.view, walk.channel));
-    c.set(j, load_shift(bias, b.view, walk.channel));
-    walk.next();
-  }
+  if (p.count == 0) return;
+  Affine<V> c;
+  c.load(table, s, p.view, p.col);
   const unsigned long long seed = Drop ? load_seed(key) : 0;
   const long long out_row = static_cast<long long>(s.channels) * s.fold;
-  long long at = (b.first + t.lane) * out_row + col;
-  const long long step = t.lanes * out_row;
+  long long at = p.first * out_row + p.col;
+  const long long step = s.lanes * out_row;
   ring.for_rows([&](const Pairs<V> (&v)[1]) {
     Pairs<V> z;
 #pragma unroll
     for (int j = 0; j < Pairs<V>::kCount; ++j)
-      z.p[j] = activate<Silu>(fma2(add2(v[0].p[j], m.p[j]), a.p[j], c.p[j]), bound);
+      z.p[j] = activate<Silu>(fma2(add2(v[0].p[j], c.shift.p[j]), c.scale.p[j], c.bias.p[j]),
+                              bound);
     if (Drop) apply_dropout<V>(z, at, key, seed);
     __stcs(reinterpret_cast<Packed<T, V>*>(y + at), pack_pairs<T, V>(z));
     at += step;
@@ -254,28 +199,29 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_apply_kernel(
 
 template <typename T, int V, bool Silu, bool Drop>
 int passes(const void* x, const NormShape& s, int dtype, const NormParam& weight,
-           const NormParam& bias, float eps, float bound, const DropKey& key, void* y, float* mean,
+           const NormParam& bias, float eps, float bound, const DropKey& key, void* y, float* table,
            float* rstd, float2* parts, cudaStream_t stream) {
   const T* in = static_cast<const T*>(x);
   T* out = static_cast<T*>(y);
-  const int most = views_at_once(s, dtype, 1);
+  const int most = views_at_once(s.batch, s.pixels, s.channels, dtype, 1);
+  const unsigned int runs = join_runs(s);
+  const dim3 threads(s.tile_cols, s.lanes);
   constexpr size_t ring = RowRing<T, V, 1, kStages>::kBytes;
-  constexpr size_t shared = std::max(ring, join_bytes<V>());
-  for (int view0 = 0; view0 < s.batch; view0 += most) {
+  constexpr size_t shared = std::max(ring, sizeof(float2) * kNormThreads * V);
+  cudaError_t err = cudaSuccess;
+  for (long long view0 = 0; view0 < s.batch && err == cudaSuccess; view0 += most) {
     const int views = static_cast<int>(std::min<long long>(most, s.batch - view0));
-    const unsigned int blocks = static_cast<unsigned int>(views) * s.tiles * s.chunks;
-    const unsigned int groups = static_cast<unsigned int>(views) * s.groups;
-    cudaError_t err = launch_kernel(norm_stats_kernel<T, V>, blocks, kNormThreads, shared, stream,
-                                    view0 > 0, in, s, view0, parts);
+    const dim3 blocks(s.chunks, s.tiles, views);
+    err = launch_kernel(norm_stats_kernel<T, V>, blocks, threads, shared, stream, view0 > 0, in, s,
+                        view0, parts);
     if (err == cudaSuccess)
-      err = launch_kernel(norm_join_kernel<V>, groups, kNormThreads, 0, stream, true, parts, s,
-                          view0, eps, mean, rstd);
+      err = launch_kernel(norm_join_kernel, dim3(runs, views), kJoinThreads, 0, stream, true,
+                          parts, s, view0, weight, bias, eps, rstd, table);
     if (err == cudaSuccess)
-      err = launch_kernel(norm_apply_kernel<T, V, Silu, Drop>, blocks, kNormThreads, ring, stream,
-                          true, in, s, view0, weight, bias, bound, key, mean, rstd, out);
-    if (err != cudaSuccess) return static_cast<int>(err);
+      err = launch_kernel(norm_apply_kernel<T, V, Silu, Drop>, blocks, threads, ring, stream, true,
+                          in, s, view0, table, bound, key, out);
   }
-  return launch_status();
+  return err == cudaSuccess ? launch_status() : static_cast<int>(err);
 }
 
 }  // namespace
@@ -283,9 +229,15 @@ int passes(const void* x, const NormShape& s, int dtype, const NormParam& weight
 
 using namespace dr;
 
+extern "C" size_t dr_group_norm_state_floats(int64_t batch, int32_t channels, int32_t groups) {
+  return batch < 0 || channels < 1 || groups < 1
+             ? 0
+             : static_cast<size_t>(batch) * (3 * static_cast<size_t>(channels) + groups);
+}
+
 extern "C" size_t dr_group_norm_workspace_bytes(int64_t batch, int64_t pixels, int32_t channels,
                                                 int32_t groups, int32_t dtype, int32_t backward) {
-  if (bad_norm_sizes(batch, pixels, channels, groups, dtype)) return 0;
+  if (bad_norm_sizes(batch, pixels, channels, groups, dtype) || too_large(batch, pixels)) return 0;
   return norm_workspace_bytes(batch, pixels, channels, groups, dtype, backward != 0);
 }
 
@@ -295,31 +247,35 @@ extern "C" int dr_group_norm_fwd(const void* x, int64_t x_stride, int32_t dtype,
                                  const void* bias, int32_t bias_dtype, int64_t bias_batch,
                                  float eps, int32_t activation, int32_t drop_threshold,
                                  const int64_t* seed, int64_t seed_value, int64_t layer, void* y,
-                                 float* mean, float* rstd, void* workspace,
-                                 size_t workspace_bytes, void* stream) {
+                                 float* state, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
   if (bad_norm_sizes(batch, pixels, channels, groups, dtype) || x_stride < channels ||
       bad_norm_param(weight, weight_dtype, weight_batch, batch) ||
       bad_norm_param(bias, bias_dtype, bias_batch, batch) || activation < DR_ACTIVATION_NONE ||
       activation > DR_ACTIVATION_SILU || bad_drop(drop_threshold, layer))
     return DR_ERR_INVALID_ARGUMENT;
   if (batch == 0 || pixels == 0) return DR_OK;
-  if (x == nullptr || y == nullptr || mean == nullptr || rstd == nullptr)
+  if (x == nullptr || y == nullptr || state == nullptr || !aligned_to(state, 16))
     return DR_ERR_INVALID_ARGUMENT;
+  if (too_large(batch, pixels)) return DR_ERR_TOO_LARGE;
   NormShape s;
-  NormVector v = choose_vector(pixels, channels, dtype, x_stride, channels, {x, y});
-  if (batch > kMaxNormBlocks ||
-      !plan_passes(s, v, batch, pixels, channels, groups, dtype, x_stride, channels))
-    return DR_ERR_TOO_LARGE;
+  const NormVector v = choose_vector(pixels, channels, dtype, x_stride, channels, {x, y});
+  plan_passes(s, v, batch, pixels, channels, groups, dtype, x_stride, channels, 1);
   if (workspace == nullptr || workspace_bytes < norm_space(s, false).total)
     return DR_ERR_WORKSPACE_TOO_SMALL;
-  const NormParam w{weight, weight_dtype, weight_batch > 1 ? channels : 0};
-  const NormParam b{bias, bias_dtype, bias_batch > 1 ? channels : 0};
+  auto param = [&](const void* data, int32_t type, int64_t rows) {
+    return data != nullptr ? NormParam{data, true, type, rows > 1 ? channels : 0}
+                           : NormParam{state, false, DR_FLOAT32, 0};
+  };
+  const NormParam w = param(weight, weight_dtype, weight_batch);
+  const NormParam b = param(bias, bias_dtype, bias_batch);
   const DropKey key = drop_key(seed, seed_value, layer, drop_threshold);
   const float bound = norm_bound(activation);
+  float* rstd = state + static_cast<size_t>(batch) * 3 * channels;
   return with_variant(dtype, v.vec, activation, drop_threshold, [&](auto k) {
     using K = decltype(k);
     return passes<typename K::Type, K::kVec, K::kSilu, K::kDrop>(
-        x, s, dtype, w, b, eps, bound, key, y, mean, rstd, static_cast<float2*>(workspace),
+        x, s, dtype, w, b, eps, bound, key, y, state, rstd, static_cast<float2*>(workspace),
         as_stream(stream));
   });
 }

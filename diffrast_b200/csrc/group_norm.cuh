@@ -12,8 +12,17 @@
 // A view is a matrix of pixels by channels whose rows are read in vectors of V values. Where the
 // channels do not fill whole 16-byte vectors but the rows follow one another without gaps, `fold`
 // pixels are taken as one row of fold * channels (7 channels of float32: 4 pixels are 7 vectors).
-// A block's threads are R rows by the vectors of a tile of columns, so that a thread keeps its
-// channels, and their constants in registers, for all its rows.
+// A block's threads are `lanes` rows by the vectors of a tile of columns (threadIdx.y and .x), so
+// that a thread keeps its channels, and their constants in registers, for all its rows. Blocks sum
+// over channels, whatever their groups, so tiles may cut groups; a small kernel between the two
+// passes joins the blocks' sums of each channel and the channels of each group, and leaves the
+// constants of each view's channels for the second pass as it reads them.
+//
+// What a block does once costs as much as many of its rows: with the statistics joined per group in
+// every block, divisions for the threads' places and the channels' constants formed by every
+// thread, 1000 instructions of a warp were spent beside 35 for each row of vectors, and a view of
+// 8 MB took 17 us with all its data in L2. Hence the block's shape, the sums by channel and the
+// tables of constants.
 #pragma once
 
 #include <algorithm>
@@ -31,95 +40,43 @@ constexpr int kNormThreads = 256;
 // How the views are cut up (made by cut_norm).
 struct NormShape {
   long long batch;
-  long long rows;       // rows of a view: pixels / fold
+  long long rows;    // rows of a view: pixels / fold
   long long pixels;
   int channels, groups, group_channels;
   int fold;
-  int cols;             // vectors in a row
-  int tile_cols;        // vectors in a tile of columns (the last tile may have fewer)
-  int tiles;            // of a row; whole groups each, unless groups are cut
-  int pieces;           // tiles that a group is cut into, or 1
-  int group_cols;       // vectors of a group that is cut
-  int chunk_rows;       // rows of one block's work
-  int chunks;           // of a view
+  int cols;          // vectors in a row
+  int tile_cols;     // vectors in a tile of columns (the last tile may have fewer)
+  int tiles;         // of a row
+  int lanes;         // rows of a block's threads
+  int chunk_rows;    // rows of one block's work
+  int lane_rows;     // of those, rows of each lane
+  int chunks;        // of a view
   // Elements between the rows of x and of the output's gradient.
   long long x_row, grad_row;
 };
 
+// Weight or bias. `data` is an address that may be read even where the parameter is absent (the
+// constant's table then): a kernel given NULL instead faulted although it read the parameter only
+// under a test, as a load that the compiler moves before the test does.
 struct NormParam {
-  const void* data;  // NULL: ones (weight) or zeros (bias)
+  const void* data;
+  bool present;      // otherwise ones (weight) or zeros (bias)
   int dtype;
   long long view;    // elements between the views' rows (0: one row for all)
 };
 
-struct NormTile {
-  int col, cols;      // first vector and vectors
-  int group, groups;  // first group and groups (the one group when it is cut)
-};
-
-// Work of one block: a chunk of rows in a tile of columns.
-struct NormBlock {
-  int view, chunk, piece;
-  NormTile tile;
-  int rows;
-  long long first;  // first row, counted over the views
-};
-
-__device__ __forceinline__ NormBlock norm_block(const NormShape& s, int vec, int view0,
-                                                unsigned int index) {
-  NormBlock b;
-  const unsigned int rest = index / s.chunks;
-  b.chunk = static_cast<int>(index - rest * s.chunks);
-  const unsigned int view = rest / s.tiles;
-  const int tile = static_cast<int>(rest - view * s.tiles);
-  b.view = view0 + static_cast<int>(view);
-  b.piece = 0;
-  if (s.pieces > 1) {
-    b.tile.group = tile / s.pieces;
-    b.piece = tile - b.tile.group * s.pieces;
-    b.tile.col = b.tile.group * s.group_cols + b.piece * s.tile_cols;
-    b.tile.cols = min(s.tile_cols, s.group_cols - b.piece * s.tile_cols);
-    b.tile.groups = 1;
-  } else {
-    b.tile.col = tile * s.tile_cols;
-    b.tile.cols = min(s.tile_cols, s.cols - b.tile.col);
-    b.tile.group = s.fold > 1 ? 0 : b.tile.col * vec / s.group_channels;
-    b.tile.groups = s.fold > 1 ? s.groups : b.tile.cols * vec / s.group_channels;
-  }
-  const long long row0 = static_cast<long long>(b.chunk) * s.chunk_rows;
-  b.rows = static_cast<int>(min(static_cast<long long>(s.chunk_rows), s.rows - row0));
-  b.first = b.view * s.rows + row0;
-  return b;
-}
-
-// The channels of a thread's vector one after the other, with their groups: one division for all.
-struct ChannelWalk {
-  int channel, group, rest, channels, size;
-
-  __device__ __forceinline__ ChannelWalk(const NormShape& s, int first)
-      : channels(s.channels), size(s.group_channels) {
-    channel = s.fold > 1 ? first % channels : first;
-    group = channel / size;
-    rest = channel - group * size;
-  }
-  __device__ __forceinline__ void next() {
-    ++channel;
-    if (++rest == size) rest = 0, ++group;
-    if (channel == channels) channel = 0, group = 0;
-  }
-};
-
-__device__ __forceinline__ float load_param(const void* data, int dtype, long long i) {
-  if (dtype == DR_FLOAT32) return __ldg(static_cast<const float*>(data) + i);
-  if (dtype == DR_FLOAT16) return __half2float(__ldg(static_cast<const __half*>(data) + i));
-  return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(data) + i));
+__device__ __forceinline__ float load_param(const NormParam& p, long long view, int channel) {
+  const long long i = view * p.view + channel;
+  if (p.dtype == DR_FLOAT32) return static_cast<const float*>(p.data)[i];
+  if (p.dtype == DR_FLOAT16) return __half2float(static_cast<const __half*>(p.data)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p.data)[i]);
 }
 
 __device__ __forceinline__ float load_scale(const NormParam& w, long long view, int channel) {
-  return w.data ? load_param(w.data, w.dtype, view * w.view + channel) : 1.0f;
+  return w.present ? load_param(w, view, channel) : 1.0f;
 }
 __device__ __forceinline__ float load_shift(const NormParam& b, long long view, int channel) {
-  return b.data ? load_param(b.data, b.dtype, view * b.view + channel) : 0.0f;
+  return b.present ? load_param(b, view, channel) : 0.0f;
 }
 
 __device__ __forceinline__ void store_param(void* data, int dtype, long long i, float v) {
@@ -131,18 +88,21 @@ __device__ __forceinline__ void store_param(void* data, int dtype, long long i, 
     static_cast<__nv_bfloat16*>(data)[i] = __float2bfloat16_rn(v);
 }
 
-// 1 / (1 + exp(-z)), from the hardware's exponential (of 2) and reciprocal, each within two units
-// in the last place of float32. For z below -88 the exponential is infinite and the result 0.
+// 1 / (1 + exp(-z)) of a pair. The special-function unit gives 16 results a clock and processor,
+// and with an exponential and a reciprocal for each value it was the busiest unit (74% of its rate
+// in the second pass), so the two values share one reciprocal: 1 / a = b / (a b). Exponents are cut
+// at 2^63, so that the product stays finite: below z = -43.7 the result is 2^-63 instead of less.
+// Exponential and reciprocal are within two units in the last place of float32. A NaN gives 2^-63
+// (the cut drops it), and its product with z is NaN again.
 __device__ __forceinline__ float2 sigmoid2(float2 z) {
   const float2 t = mul2(z, both(-1.4426950408889634f));
   float2 e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(fminf(t.x, 63.0f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(fminf(t.y, 63.0f)));
   e = add2(e, both(1.0f));
-  float2 s;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(e.x));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(e.y));
-  return s;
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e.x * e.y));
+  return mul2(both(r), make_float2(e.y, e.x));
 }
 
 // The activations: SiLU, or a clamp from below that is the identity with bound -infinity and ReLU
@@ -167,188 +127,128 @@ __device__ __forceinline__ float2 activate_grad(float2 q, float2 z, float bound)
 // Running moments of V channels. Values are summed as differences from the thread's first value
 // k: with n values, sum (x - k)^2 is at most n times their sum of squared deviations from their
 // mean (k is one of them), so rounding grows by no more than n, whatever the offset of the data.
-// Blocks give a thread at most kMomentRows rows; a warp's threads that share a column are joined
-// about the first one's pivot, which multiplies that number by the rows that a warp holds.
-constexpr int kMomentRows = 64;
+// Blocks give a thread at most kThreadRows rows.
+constexpr int kThreadRows = 128;
 
 template <int V>
 struct Moments {
+  static constexpr int kPairs = Pairs<V>::kCount;
   Pairs<V> pivot, sum, square;  // the pivot is kept negated
 
   __device__ __forceinline__ void start(const Pairs<V>& v) {
 #pragma unroll
-    for (int j = 0; j < Pairs<V>::kCount; ++j) {
-      pivot.p[j] = make_float2(-v.p[j].x, -v.p[j].y);
-      sum.p[j] = square.p[j] = both(0.0f);
-    }
+    for (int j = 0; j < kPairs; ++j) pivot.p[j] = make_float2(-v.p[j].x, -v.p[j].y);
+  }
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) pivot.p[j] = sum.p[j] = square.p[j] = both(0.0f);
   }
 
   __device__ __forceinline__ void add(const Pairs<V>& v) {
 #pragma unroll
-    for (int j = 0; j < Pairs<V>::kCount; ++j) {
+    for (int j = 0; j < kPairs; ++j) {
       const float2 d = add2(v.p[j], pivot.p[j]);
       sum.p[j] = add2(sum.p[j], d);
       square.p[j] = fma2(d, d, square.p[j]);
     }
   }
 
-  // Moves to the pivots of a lane of the warp: sum (x - l) = sum (x - k) + n (k - l) and
-  // sum (x - l)^2 = sum (x - k)^2 + (k - l) (2 sum (x - k) + n (k - l)). Without values (n = 0)
-  // the sums stay zero.
-  __device__ __forceinline__ void move_pivot(int from_lane, float n) {
+  // Turns the sums of n values into their mean (in sum) and their sum of squared deviations from
+  // it (in square). A sum of squares that overflowed stays infinite.
+  __device__ __forceinline__ void finish(float n) {
+    const float2 inverse = both(n > 0.0f ? __fdividef(1.0f, n) : 0.0f);
 #pragma unroll
-    for (int j = 0; j < Pairs<V>::kCount; ++j) {
-      float2 l;
-      l.x = __shfl_sync(0xFFFFFFFFu, pivot.p[j].x, from_lane);
-      l.y = V > 1 ? __shfl_sync(0xFFFFFFFFu, pivot.p[j].y, from_lane) : 0.0f;
-      const float2 d = n > 0.0f ? make_float2(l.x - pivot.p[j].x, l.y - pivot.p[j].y) : both(0.0f);
-      const float2 nd = mul2(both(n), d);
-      square.p[j] = fma2(d, fma2(both(2.0f), sum.p[j], nd), square.p[j]);
-      sum.p[j] = add2(sum.p[j], nd);
-      pivot.p[j] = l;
+    for (int j = 0; j < kPairs; ++j) {
+      const float2 offset = mul2(sum.p[j], inverse);
+      const float2 total = square.p[j];
+      const float2 s = fma2(make_float2(-offset.x, -offset.y), sum.p[j], total);
+      square.p[j].x = total.x < __int_as_float(0x7f800000) ? fmaxf(0.0f, s.x) : total.x;
+      square.p[j].y = total.y < __int_as_float(0x7f800000) ? fmaxf(0.0f, s.y) : total.y;
+      sum.p[j] = make_float2(offset.x - pivot.p[j].x, offset.y - pivot.p[j].y);
     }
   }
 
-  // Adds the sums of the lane at this distance, about the same pivots.
-  __device__ __forceinline__ void add_lane(int distance) {
+  // Joins the finished moments of n values with those of the lane at a distance:
+  //   mean + (mean' - mean) n' / (n + n'),  squares + squares' + (mean' - mean)^2 n n' / (n + n').
+  __device__ __forceinline__ void join_lane(int distance, float& n) {
+    const float other = __shfl_xor_sync(0xFFFFFFFFu, n, distance);
+    const float share = other > 0.0f ? __fdividef(other, n + other) : 0.0f;
 #pragma unroll
-    for (int j = 0; j < Pairs<V>::kCount; ++j) {
-      float2 a, b = both(0.0f);
-      a.x = __shfl_xor_sync(0xFFFFFFFFu, sum.p[j].x, distance);
-      b.x = __shfl_xor_sync(0xFFFFFFFFu, square.p[j].x, distance);
-      a.y = V > 1 ? __shfl_xor_sync(0xFFFFFFFFu, sum.p[j].y, distance) : 0.0f;
-      b.y = V > 1 ? __shfl_xor_sync(0xFFFFFFFFu, square.p[j].y, distance) : 0.0f;
-      sum.p[j] = add2(sum.p[j], a);
-      square.p[j] = add2(square.p[j], b);
+    for (int j = 0; j < kPairs; ++j) {
+      float2 m, q;
+      m.x = __shfl_xor_sync(0xFFFFFFFFu, sum.p[j].x, distance);
+      q.x = __shfl_xor_sync(0xFFFFFFFFu, square.p[j].x, distance);
+      m.y = V > 1 ? __shfl_xor_sync(0xFFFFFFFFu, sum.p[j].y, distance) : 0.0f;
+      q.y = V > 1 ? __shfl_xor_sync(0xFFFFFFFFu, square.p[j].y, distance) : 0.0f;
+      const float2 d = make_float2(m.x - sum.p[j].x, m.y - sum.p[j].y);
+      sum.p[j] = fma2(d, both(share), sum.p[j]);
+      square.p[j] = fma2(mul2(d, both(n * share)), d, add2(square.p[j], q));
     }
-  }
-
-  // (mean, sum of squared deviations) of channel j over n values.
-  __device__ __forceinline__ float2 get(int j, float n, float inverse) const {
-    const float offset = sum.get(j) * inverse;
-    // An overflown or NaN sum of squares stays what it is.
-    const float total = square.get(j);
-    const float squares = total < __int_as_float(0x7f800000)
-                              ? fmaxf(0.0f, fmaf(-n * offset, offset, total))
-                              : total;
-    return make_float2(offset - pivot.get(j), squares);
+    n += other;
   }
 };
 
-// Moments of Q neighbouring channels of a thread, n values each, as one part of n Q values.
-template <int Q, int V>
-__device__ __forceinline__ float2 fold_channels(const Moments<V>& m, int first, float n,
-                                                float inverse) {
-  float2 part[Q];
-  float mean = 0.0f;
-#pragma unroll
-  for (int j = 0; j < Q; ++j) part[j] = m.get(first + j, n, inverse);
-#pragma unroll
-  for (int j = 0; j < Q; ++j) mean += part[j].x - part[0].x;
-  mean = fmaf(mean, 1.0f / Q, part[0].x);
-  float squares = 0.0f;
-#pragma unroll
-  for (int j = 0; j < Q; ++j) {
-    const float d = part[j].x - mean;
-    squares += fmaf(n * d, d, part[j].y);
+// (count, mean, squared deviations) of some values, and of those joined with others.
+struct Moment {
+  float n, mean, squares;
+
+  __device__ __forceinline__ void join(const Moment& o) {
+    const float share = o.n > 0.0f ? __fdividef(o.n, n + o.n) : 0.0f;
+    const float d = o.mean - mean;
+    mean = fmaf(d, share, mean);
+    squares = fmaf(d * (n * share), d, squares + o.squares);
+    n += o.n;
   }
-  return make_float2(mean, squares);
-}
+  __device__ __forceinline__ Moment lane(int distance) const {
+    return {__shfl_xor_sync(0xFFFFFFFFu, n, distance),
+            __shfl_xor_sync(0xFFFFFFFFu, mean, distance),
+            __shfl_xor_sync(0xFFFFFFFFu, squares, distance)};
+  }
+  __device__ __forceinline__ void join_warp() {
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) join(lane(d));
+  }
+};
 
 // NaN or infinite data give NaN statistics (their mean is NaN or infinite).
-__device__ __forceinline__ float variance_of(float mean, float squares, float count) {
-  return isfinite(mean) ? squares / count : __int_as_float(0x7fc00000);
+__device__ __forceinline__ float rstd_of(const Moment& m, float eps) {
+  return isfinite(m.mean) ? rsqrtf(m.squares / m.n + eps) : __int_as_float(0x7fc00000);
 }
 
-// Lanes (a power of two, at most 32) that share one of `items` reductions of a block.
-__device__ __forceinline__ int lanes_per(int items, int threads) {
-  int lanes = 1;
-  while (lanes < 32 && items * lanes * 2 <= threads) lanes *= 2;
-  return lanes;
-}
-
-__device__ __forceinline__ float lane_sum(float v, int lanes) {
-  for (int d = lanes / 2; d > 0; d /= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
   return v;
 }
 
-// Joins (mean, squared deviations) of parts with the given counts into those of their union:
-//   mean = m_0 + sum n_i (m_i - m_0) / N,  squares = sum (s_i + n_i (m_i - mean)^2).
-// `part(item, i, value)` returns the count of part i and its value; a part of count 0 has a finite
-// one, and part 0 is never empty. All threads of the block call this with the same `items` of
-// `parts` entries each; `done(item, mean, squares)` runs on one lane per item.
-template <typename Part, typename Done>
-__device__ __forceinline__ void join_moments(int items, int parts, Part part, Done done) {
-  const int lanes = lanes_per(items, kNormThreads);
-  const int lane = threadIdx.x & (lanes - 1);
-  const int step = kNormThreads / lanes;
-  for (int base = 0; base < items; base += step) {
-    const int item = base + threadIdx.x / lanes;
-    const bool live = item < items;
-    float n = 0.0f, total = 0.0f;
-    float2 first = make_float2(0.0f, 0.0f);
-    if (live) {
-      part(item, 0, first);
-#pragma unroll 4
-      for (int i = lane; i < parts; i += lanes) {
-        float2 v;
-        const float c = part(item, i, v);
-        n += c;
-        total = fmaf(c, v.x - first.x, total);
-      }
-    }
-    n = lane_sum(n, lanes);
-    total = lane_sum(total, lanes);
-    const float mean = first.x + total / n;
-    float squares = 0.0f;
-    if (live) {
-#pragma unroll 4
-      for (int i = lane; i < parts; i += lanes) {
-        float2 v;
-        const float c = part(item, i, v);
-        const float d = v.x - mean;
-        squares += c > 0.0f ? fmaf(c * d, d, v.y) : 0.0f;
-      }
-    }
-    squares = lane_sum(squares, lanes);
-    if (live && lane == 0) done(item, mean, squares);
-  }
+// Whether the rows of a warp's threads are joined by shuffles before the block's: the tile's
+// columns divide the warp.
+__device__ __forceinline__ bool warp_holds_rows() {
+  return blockDim.x < 32 && 32 % blockDim.x == 0;
 }
 
-// Sums pairs: `part(item, i)` is entry i of the item's `parts`.
-template <typename Part, typename Done>
-__device__ __forceinline__ void join_sums(int items, int parts, Part part, Done done) {
-  const int lanes = lanes_per(items, kNormThreads);
-  const int lane = threadIdx.x & (lanes - 1);
-  const int step = kNormThreads / lanes;
-  for (int base = 0; base < items; base += step) {
-    const int item = base + threadIdx.x / lanes;
-    const bool live = item < items;
-    float2 total = make_float2(0.0f, 0.0f);
-    if (live) {
-#pragma unroll 8
-      for (int i = lane; i < parts; i += lanes) {
-        const float2 v = part(item, i);
-        total.x += v.x;
-        total.y += v.y;
-      }
-    }
-    total.x = lane_sum(total.x, lanes);
-    total.y = lane_sum(total.y, lanes);
-    if (live && lane == 0) done(item, total);
-  }
-}
+// A block's place: a chunk of rows, a tile of columns and a view; and its threads'.
+struct NormPlace {
+  int view, chunk, rows;
+  int col;             // first element of this thread's vector in a row
+  int count;           // rows of this thread
+  long long first;     // its first row, counted over the views
 
-// A thread's place in a tile of columns: `lanes` rows of the tile's vectors at a time.
-struct TileThread {
-  int lanes, lane, col;
-  bool active;
-
-  __device__ __forceinline__ explicit TileThread(int cols) {
-    lanes = kNormThreads / cols;
-    lane = threadIdx.x / cols;
-    col = threadIdx.x - lane * cols;
-    active = lane < lanes;
+  __device__ __forceinline__ NormPlace(const NormShape& s, int vec, int v, int tile, int c)
+      : view(v), chunk(c) {
+    const long long row0 = static_cast<long long>(c) * s.chunk_rows;
+    rows = static_cast<int>(min(static_cast<long long>(s.chunk_rows), s.rows - row0));
+    const int x = tile * s.tile_cols + threadIdx.x;
+    const int y = threadIdx.y;
+    col = x * vec;
+    count = 0;
+    if (x < s.cols && y < rows)
+      count = rows == s.chunk_rows
+                  ? s.lane_rows
+                  : static_cast<int>(static_cast<unsigned int>(rows - y + s.lanes - 1) /
+                                     static_cast<unsigned int>(s.lanes));
+    first = v * s.rows + row0 + y;
   }
 };
 
@@ -399,21 +299,21 @@ struct RowRing {
   static constexpr unsigned int kSlot = sizeof(P) * kNormThreads;
   static constexpr size_t kBytes = static_cast<size_t>(kSlot) * Images * Stages;
 
-  const T* at[Images];
-  long long stride[Images];
+  const T* at[Images];       // next row to fetch
+  long long stride[Images];  // elements to the thread's row after it
   unsigned int slots;
   int count;
 
-  // Rows lane, lane + lanes, ... below `rows` of columns that start at at[].
-  __device__ __forceinline__ void start(void* shared, const TileThread& t, int rows) {
+  __device__ __forceinline__ void image(int k, const T* base, long long row, const NormPlace& p,
+                                        int lanes) {
+    at[k] = base + p.first * row + p.col;
+    stride[k] = lanes * row;
+  }
+
+  __device__ __forceinline__ void start(void* shared, int rows) {
     slots = static_cast<unsigned int>(__cvta_generic_to_shared(shared)) +
-            threadIdx.x * static_cast<unsigned int>(sizeof(P));
-    count = t.active && t.lane < rows ? (rows - t.lane + t.lanes - 1) / t.lanes : 0;
-#pragma unroll
-    for (int k = 0; k < Images; ++k) {
-      at[k] += t.lane * stride[k];
-      stride[k] *= t.lanes;
-    }
+            (threadIdx.y * blockDim.x + threadIdx.x) * static_cast<unsigned int>(sizeof(P));
+    count = rows;
 #pragma unroll
     for (int u = 0; u < Stages; ++u) {
       if (u < count) fetch(u);
@@ -429,6 +329,10 @@ struct RowRing {
     }
   }
 
+  __device__ __forceinline__ Pairs<V> load(int u, int k) const {
+    return load_pairs<T, V>(load_slot<P>(slots + (u * Images + k) * kSlot));
+  }
+
   // Calls use(vectors) for the rows in order.
   template <typename Use>
   __device__ __forceinline__ void for_rows(Use use) {
@@ -439,13 +343,67 @@ struct RowRing {
         copy_wait<Stages - 1>();
         Pairs<V> v[Images];
 #pragma unroll
-        for (int k = 0; k < Images; ++k)
-          v[k] = load_pairs<T, V>(load_slot<P>(slots + (u * Images + k) * kSlot));
+        for (int k = 0; k < Images; ++k) v[k] = load(u, k);
         use(v);
         if (u + Stages < left) fetch(u);
         copy_commit();
       }
     }
+  }
+};
+
+// The constants of a thread's channels out of a table of one row of `channels` floats: those of
+// the columns from `col` on, the channels repeated for each folded pixel.
+template <int V>
+__device__ __forceinline__ Pairs<V> load_row(const float* row, const NormShape& s, int col) {
+  Pairs<V> r;
+  if (V == 1) r.p[0].y = 0.0f;
+  if (s.fold > 1 || V == 1) {
+    int c = s.fold > 1 ? col % s.channels : col;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      r.set(j, row[c]);
+      if (++c == s.channels) c = 0;
+    }
+  } else if constexpr (V == 2) {
+    r.p[0] = *reinterpret_cast<const float2*>(row + col);
+  } else if constexpr (V > 2) {
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) {
+      const float4 q = reinterpret_cast<const float4*>(row + col)[j];
+      r.p[2 * j] = make_float2(q.x, q.y);
+      r.p[2 * j + 1] = make_float2(q.z, q.w);
+    }
+  }
+  return r;
+}
+
+// z = (x + shift) scale + bias, the tables that the forward pass leaves: [batch][3][channels].
+template <int V>
+struct Affine {
+  Pairs<V> shift, scale, bias;
+
+  __device__ __forceinline__ void load(const float* table, const NormShape& s, int view, int col) {
+    table += static_cast<long long>(view) * 3 * s.channels;
+    shift = load_row<V>(table, s, col);
+    scale = load_row<V>(table + s.channels, s, col);
+    bias = load_row<V>(table + 2 * s.channels, s, col);
+  }
+};
+
+// Threads of the kernels that join the blocks' sums: 32 channels by 32 lanes. A block has a run of
+// whole groups of at most 32 channels together, or one group.
+constexpr int kJoinThreads = 1024;
+
+struct JoinPlace {
+  int view, group, channel, channels;  // first group and channel, and its channels
+
+  __device__ __forceinline__ JoinPlace(const NormShape& s, int view0) {
+    const int run = s.group_channels > 32 ? 1 : 32 / s.group_channels;
+    view = view0 + blockIdx.y;
+    group = blockIdx.x * run;
+    channel = group * s.group_channels;
+    channels = min(run, s.groups - group) * s.group_channels;
   }
 };
 
@@ -464,7 +422,6 @@ __device__ __forceinline__ void let_next_kernel_start() {
 // ---- host --------------------------------------------------------------------------------------
 
 constexpr int kMaxNormChannels = 1 << 16;
-constexpr long long kMaxNormBlocks = 0x7FFFFFFF;  // of one launch
 
 inline int greatest_divisor(long long a, long long b) {
   while (b != 0) {
@@ -488,10 +445,6 @@ inline bool bad_norm_param(const void* data, int32_t dtype, int64_t rows, int64_
 inline float norm_bound(int activation) {
   return activation == DR_ACTIVATION_RELU ? 0.0f : -__builtin_huge_valf();
 }
-
-// Bytes that both passes over a part of the views may read for the second one to find them in L2
-// (126 MB; 80 MB read and as much written in turn is what was seen to stay).
-constexpr long long kPartBytes = 72LL << 20;
 
 // A vector width and a number of folded pixels.
 struct NormVector {
@@ -523,89 +476,79 @@ inline NormVector choose_vector(long long pixels, int channels, int dtype, long 
   return {1, 1};
 }
 
-// Cuts views into tiles of at most `most_cols` columns (at least the fewest whole groups that are
-// whole vectors) and chunks of rows of about `chunk_bytes`. Lowers v.vec where a group is wider than a block's
-// threads and not whole vectors (its tiles must not reach into the next group). False when there
-// would be too many blocks.
-inline bool cut_norm(NormShape& s, NormVector& v, long long batch, long long pixels, int channels,
-                     int groups, int dtype, long long x_stride, long long grad_stride,
-                     int most_cols, long long chunk_bytes) {
+// Cuts views into tiles of at most `most_cols` columns and chunks of rows of about `chunk_bytes`.
+inline void cut_norm(NormShape& s, const NormVector& v, long long batch, long long pixels,
+                     int channels, int groups, int dtype, long long x_stride,
+                     long long grad_stride, int most_cols, long long chunk_bytes) {
   s.batch = batch;
   s.pixels = pixels;
   s.channels = channels;
   s.groups = groups;
   s.group_channels = channels / groups;
-  const int d = s.group_channels;
-  long long unit = d / greatest_divisor(d, v.vec);
-  if (v.fold == 1 && unit > kNormThreads && d % v.vec != 0) {
-    v.vec = 1;
-    unit = d;
-  }
   s.fold = v.fold;
   s.rows = pixels / s.fold;
   s.cols = static_cast<int>(static_cast<long long>(channels) * s.fold / v.vec);
   s.x_row = x_stride * s.fold;
   s.grad_row = grad_stride * s.fold;
-  s.pieces = 1;
-  s.group_cols = 0;
-  most_cols = std::min(most_cols, kNormThreads);
-  if (s.fold > 1) {
-    s.tile_cols = s.cols;
-    s.tiles = 1;
-  } else if (unit <= kNormThreads) {
-    s.tile_cols =
-        static_cast<int>(std::min<long long>(s.cols, std::max(1LL, most_cols / unit) * unit));
-    s.tiles = (s.cols + s.tile_cols - 1) / s.tile_cols;
-  } else {
-    s.group_cols = static_cast<int>(unit);
-    s.pieces = static_cast<int>((unit + kNormThreads - 1) / kNormThreads);
-    s.tile_cols = kNormThreads;
-    s.tiles = groups * s.pieces;
-  }
-  const long long lanes = kNormThreads / s.tile_cols;  // rows that a block reads at once
-  const long long tile_bytes = static_cast<long long>(s.tile_cols) * v.vec * dtype_bytes(dtype);
-  const long long deep = chunk_bytes / tile_bytes / lanes;
-  s.chunk_rows = static_cast<int>(std::max(1LL, std::min<long long>(deep, kMomentRows)) * lanes);
-  const long long chunks = (s.rows + s.chunk_rows - 1) / s.chunk_rows;
-  if (chunks > kMaxNormBlocks || batch > kMaxNormBlocks / s.tiles ||
-      chunks > kMaxNormBlocks / std::max(1LL, batch * s.tiles))
-    return false;
-  s.chunks = static_cast<int>(chunks);
-  return true;
+  s.tiles = (s.cols + most_cols - 1) / most_cols;
+  s.tile_cols = (s.cols + s.tiles - 1) / s.tiles;
+  s.lanes = kNormThreads / s.tile_cols;
+  const long long step = static_cast<long long>(s.tile_cols) * s.lanes * v.vec * dtype_bytes(dtype);
+  const long long deep = std::max(1LL, std::min<long long>(chunk_bytes / step, kThreadRows));
+  s.lane_rows = static_cast<int>(deep);
+  s.chunk_rows = s.lane_rows * s.lanes;
+  s.chunks = static_cast<int>((s.rows + s.chunk_rows - 1) / s.chunk_rows);
 }
 
-// The plan of a call in passes over memory. Chunks are 64 KB, less where that would leave
-// processors idle, more where a view would have over a thousand.
-inline bool plan_passes(NormShape& s, NormVector& v, long long batch, long long pixels,
-                        int channels, int groups, int dtype, long long x_stride,
-                        long long grad_stride) {
-  const long long view = pixels * channels * dtype_bytes(dtype);
-  const long long chunk = std::max(
-      view / 1024, std::max(4096LL, std::min(65536LL, batch * view / (4 * 148))));
-  return cut_norm(s, v, batch, pixels, channels, groups, dtype, x_stride, grad_stride, kNormThreads,
-                  chunk);
+// Views, and pixels of a view, that still leave blocks and rows countable in 32 bits.
+inline bool too_large(long long batch, long long pixels) {
+  return batch > 0x7FFFFFFFLL || pixels > 0x7FFFFFFFLL;
 }
 
+// Blocks for each view of the kernels that join the blocks' sums (see JoinPlace).
+inline unsigned int join_runs(const NormShape& s) {
+  const int run = s.group_channels > 32 ? 1 : 32 / s.group_channels;
+  return static_cast<unsigned int>((s.groups + run - 1) / run);
+}
+
+// Bytes that both passes over a part of the views may read for the second one to find them in L2.
+constexpr long long kPartBytes = 72LL << 20;
+
+#include <cstdlib>
+inline long long envv(const char* n, long long d) { const char* e = getenv(n); return e ? atoll(e) : d; }
 // Views that are taken together, first pass and second: as many as stay in L2 in between.
-inline int views_at_once(const NormShape& s, int dtype, int images) {
-  const long long view = s.pixels * s.channels * dtype_bytes(dtype) * images;
-  return static_cast<int>(std::max(1LL, std::min(s.batch, kPartBytes / std::max(1LL, view))));
+inline int views_at_once(long long batch, long long pixels, int channels, int dtype, int images) {
+  const long long view = pixels * channels * dtype_bytes(dtype) * images;
+  return static_cast<int>(
+      std::max(1LL, std::min({batch, 65535LL, (envv("DRX_PART", 72) << 20) / std::max(1LL, view)})));
 }
 
-// Workspace. Forward: (mean, squares) of each group (or piece of one) for each chunk. Backward: sums
-// of each channel for each chunk and of each view, and the two means of each group.
+// The plan of a call in passes over memory: chunks for `kNormBlocks` blocks in a launch, of 8 KB at
+// least.
+constexpr int kNormBlocks = 8 * 148;
+
+inline void plan_passes(NormShape& s, const NormVector& v, long long batch, long long pixels,
+                        int channels, int groups, int dtype, long long x_stride,
+                        long long grad_stride, int images) {
+  const long long view = pixels * channels * dtype_bytes(dtype);
+  const long long part = view * views_at_once(batch, pixels, channels, dtype, images);
+  cut_norm(s, v, batch, pixels, channels, groups, dtype, x_stride, grad_stride, kNormThreads,
+           std::max(8192LL, part / envv("DRX_BLOCKS", kNormBlocks)));
+}
+
+// Workspace: a pair of each channel for each chunk; for the backward pass also one of each view and
+// channel, and the table of the second pass.
 struct NormSpace {
-  size_t parts, sums, means, total;  // offsets, and the end
+  size_t parts, sums, table, total;  // offsets, and the end
 };
 
 inline NormSpace norm_space(const NormShape& s, bool backward) {
-  const size_t groups = static_cast<size_t>(s.batch) * s.groups * sizeof(float2);
   const size_t channels = static_cast<size_t>(s.batch) * s.channels * sizeof(float2);
   NormSpace w;
   w.parts = 0;
-  w.sums = align256((backward ? channels : groups * s.pieces) * s.chunks);
-  w.means = w.sums + (backward ? align256(channels) : 0);
-  w.total = w.means + (backward ? groups : 0);
+  w.sums = align256(channels * s.chunks);
+  w.table = w.sums + (backward ? align256(channels) : 0);
+  w.total = w.table + (backward ? align256(channels) : 0);
   return w;
 }
 
@@ -621,19 +564,20 @@ inline size_t norm_workspace_bytes(long long batch, long long pixels, int channe
       continue;
     if (v.fold == 1 && channels % v.vec != 0) continue;
     NormShape s;
-    if (plan_passes(s, v, batch, pixels, channels, groups, dtype, channels, channels))
-      most = std::max(most, norm_space(s, backward).total);
+    plan_passes(s, v, batch, pixels, channels, groups, dtype, channels, channels,
+                backward ? 2 : 1);
+    most = std::max(most, norm_space(s, backward).total);
   }
   return most;
 }
 
 // Launches a kernel on a stream, with programmatic dependence on the one before it if `after`.
 template <typename... Params, typename... Args>
-cudaError_t launch_kernel(void (*kernel)(Params...), unsigned int blocks, unsigned int threads,
+cudaError_t launch_kernel(void (*kernel)(Params...), dim3 blocks, dim3 threads,
                           size_t shared, cudaStream_t stream, bool after, Args... args) {
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(blocks);
-  config.blockDim = dim3(threads);
+  config.gridDim = blocks;
+  config.blockDim = threads;
   config.dynamicSmemBytes = shared;
   config.stream = stream;
   cudaLaunchAttribute attribute = {};

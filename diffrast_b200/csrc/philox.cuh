@@ -39,7 +39,7 @@ inline DropKey drop_key(const int64_t* seed, int64_t seed_value, int64_t layer,
 }
 
 __device__ __forceinline__ unsigned long long load_seed(const DropKey& key) {
-  return key.seed != nullptr ? static_cast<unsigned long long>(__ldg(key.seed)) : key.value;
+  return key.seed != nullptr ? static_cast<unsigned long long>(*key.seed) : key.value;
 }
 
 __device__ __forceinline__ uint4 philox(unsigned long long block, unsigned int layer,

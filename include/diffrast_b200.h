@@ -505,9 +505,11 @@ int dr_dropout(const void* x, const void* residual, int64_t count, int32_t dtype
  * run of channels / groups channels (groups divides channels, at most 65536),
  *   y = dropout(act((x - mean) * rstd * weight + bias)),  rstd = 1 / sqrt(variance + eps).
  * weight and bias have their own dtype and are [weight_batch, channels] with weight_batch 1 or
- * batch, or NULL (ones, zeros). y [batch, pixels, channels] is contiguous; mean and rstd
- * [batch, groups] are kept for the backward pass. workspace: dr_group_norm_workspace_bytes(...,
- * backward 0). */
+ * batch, or NULL (ones, zeros). y [batch, pixels, channels] is contiguous. state
+ * (dr_group_norm_state_floats() floats, 16-byte aligned) is kept for the backward pass:
+ * [batch, 3, channels] of -mean, rstd * weight and bias, then [batch, groups] of rstd.
+ * workspace: dr_group_norm_workspace_bytes(..., backward 0). */
+size_t dr_group_norm_state_floats(int64_t batch, int32_t channels, int32_t groups);
 size_t dr_group_norm_workspace_bytes(int64_t batch, int64_t pixels, int32_t channels,
                                      int32_t groups, int32_t dtype, int32_t backward);
 int dr_group_norm_fwd(const void* x, int64_t x_stride, int32_t dtype, int64_t batch,
@@ -515,22 +517,21 @@ int dr_group_norm_fwd(const void* x, int64_t x_stride, int32_t dtype, int64_t ba
                       int32_t weight_dtype, int64_t weight_batch, const void* bias,
                       int32_t bias_dtype, int64_t bias_batch, float eps, int32_t activation,
                       int32_t drop_threshold, const int64_t* seed, int64_t seed_value,
-                      int64_t layer, void* y, float* mean, float* rstd, void* workspace,
+                      int64_t layer, void* y, float* state, void* workspace,
                       size_t workspace_bytes, void* stream);
 
 /* Gradients of dr_group_norm_fwd from grad_y (pixels grad_stride elements apart): grad_x
- * (contiguous, dtype), grad_weight and grad_bias (shape and dtype of weight and bias; written,
- * summed over views where those are shared). Any may be NULL. With batch or pixels 0 nothing is
- * written. The same inputs give the same bits. workspace:
+ * (contiguous, dtype), grad_weight and grad_bias (written; [weight_batch, channels] as weight and
+ * bias are, summed over views where there is one row). Any may be NULL. With batch or pixels 0
+ * nothing is written. The same inputs give the same bits. workspace:
  * dr_group_norm_workspace_bytes(..., backward 1). */
 int dr_group_norm_bwd(const void* x, int64_t x_stride, const void* grad_y, int64_t grad_stride,
                       int32_t dtype, int64_t batch, int64_t pixels, int32_t channels,
-                      int32_t groups, const void* weight, int32_t weight_dtype,
-                      int64_t weight_batch, const void* bias, int32_t bias_dtype,
-                      int64_t bias_batch, const float* mean, const float* rstd,
-                      int32_t activation, int32_t drop_threshold, const int64_t* seed,
-                      int64_t seed_value, int64_t layer, void* grad_x, void* grad_weight,
-                      void* grad_bias, void* workspace, size_t workspace_bytes, void* stream);
+                      int32_t groups, const float* state, int32_t activation,
+                      int32_t drop_threshold, const int64_t* seed, int64_t seed_value,
+                      int64_t layer, void* grad_x, void* grad_weight, int32_t weight_dtype,
+                      int64_t weight_batch, void* grad_bias, int32_t bias_dtype,
+                      int64_t bias_batch, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -89,17 +89,17 @@ def test_rows_of_feature_tensors():
 
 
 def fwd(lib, **change):
-    a = dict(x=16, x_stride=8, dtype=0, batch=2, pixels=9, channels=8, groups=2, w=None, wd=0, wb=1,
-             b=None, bd=0, bb=1, eps=1e-5, act=0, drop=0, seed=None, value=0, layer=0, y=16, mean=16,
-             rstd=16, ws=16, ws_bytes=1 << 20, stream=None)
+    a = dict(x=16, x_stride=8, dtype=0, batch=2, pixels=9, channels=8, groups=2, w=16, wd=0, wb=1,
+             b=16, bd=0, bb=1, eps=1e-5, act=0, drop=0, seed=None, value=0, layer=0, y=16, state=16,
+             ws=16, ws_bytes=1 << 20, stream=None)
     a.update(change)
     return lib.dr_group_norm_fwd(*a.values())
 
 
 def bwd(lib, **change):
     a = dict(x=16, x_stride=8, gy=16, gy_stride=8, dtype=0, batch=2, pixels=9, channels=8, groups=2,
-             w=16, wd=0, wb=1, b=16, bd=0, bb=1, mean=16, rstd=16, act=0, drop=0, seed=None, value=0,
-             layer=0, gx=16, gw=16, gb=16, ws=16, ws_bytes=1 << 20, stream=None)
+             state=16, act=0, drop=0, seed=None, value=0, layer=0, gx=16, w=16, wd=0, wb=1, b=16,
+             bd=0, bb=1, ws=16, ws_bytes=1 << 20, stream=None)
     a.update(change)
     return lib.dr_group_norm_bwd(*a.values())
 
@@ -110,16 +110,19 @@ def test_c_abi_refuses_before_any_cuda_call():
     common = [dict(dtype=3), dict(dtype=-1), dict(batch=-1), dict(pixels=-1), dict(channels=0),
               dict(groups=0), dict(groups=3), dict(x_stride=7), dict(act=3), dict(act=-1),
               dict(drop=-1), dict(drop=65536), dict(layer=-1), dict(layer=1 << 32), dict(w=16, wb=3), dict(b=16, bd=4), dict(x=None),
-              dict(mean=None), dict(rstd=None), dict(channels=1 << 17, x_stride=1 << 17)]
+              dict(state=None), dict(state=8), dict(channels=1 << 17, x_stride=1 << 17, gy_stride=1 << 17)]
     for change in common + [dict(y=None)]:
+        change.pop("gy_stride", None)
         assert fwd(lib, **change) == bad, change
-    for change in common + [dict(gy=None), dict(gy_stride=7), dict(w=None), dict(b=None)]:
+    for change in common + [dict(gy=None), dict(gy_stride=7)]:
         assert bwd(lib, **change) == bad, change
     for call in (fwd, bwd):
         assert call(lib, ws_bytes=0) == small
         assert call(lib, ws=None) == small
         assert call(lib, batch=0) == 0 and call(lib, pixels=0) == 0
+        assert call(lib, batch=1 << 31) == 10003 and call(lib, pixels=1 << 31) == 10003
     assert lib.dr_group_norm_workspace_bytes(2, 9, 8, 3, 0, 0) == 0
+    assert lib.dr_group_norm_state_floats(2, 8, 4) == 2 * (3 * 8 + 4)
     for backward in (0, 1):
         assert lib.dr_group_norm_workspace_bytes(2, 9, 8, 2, 0, backward) > 0
 
