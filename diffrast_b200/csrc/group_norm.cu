@@ -93,63 +93,69 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_stats_kernel(const T* __
 __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(
     const float2* parts, NormShape s, int view0, NormParam weight, NormParam bias, float eps,
     float* __restrict__ rstd, float* __restrict__ table) {
-  __shared__ float2 entry[32][33];
+  __shared__ float2 entry[kJoinThreads + kJoinThreads / 8];
   __shared__ Moment channel[32];
   __shared__ float2 result;  // of a group wider than 32 channels
   let_next_kernel_start();
   wait_for_kernel_before();
   const JoinPlace p(s, view0);
-  const int x = threadIdx.x % 32, y = threadIdx.x / 32;
   const int d = s.group_channels;
   parts += static_cast<long long>(p.view) * s.chunks * s.channels + p.channel;
-  table += static_cast<long long>(p.view) * 3 * s.channels;
-  rstd += static_cast<long long>(p.view) * s.groups;
+  table += static_cast<long long>(p.view) * 3 * s.channels + p.channel;
+  rstd += static_cast<long long>(p.view) * s.groups + p.group;
   const float chunk_count = static_cast<float>(s.chunk_rows) * static_cast<float>(s.fold);
   const float last_count =
       static_cast<float>(s.rows - static_cast<long long>(s.chunks - 1) * s.chunk_rows) *
       static_cast<float>(s.fold);
   auto write = [&](int c, float mean, float r) {
     table[c] = -mean;
-    table[s.channels + c] = r * load_scale(weight, p.view, c);
-    table[2 * s.channels + c] = load_shift(bias, p.view, c);
+    table[s.channels + c] = r * load_scale(weight, p.view, p.channel + c);
+    table[2 * s.channels + c] = load_shift(bias, p.view, p.channel + c);
   };
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   Moment wide = {0.0f, 0.0f, 0.0f};
-  for (int base = 0; base < p.channels; base += 32) {
+  for (int base = 0; base < p.channels; base += p.width) {
     // This lane's chunks of channel x.
     Moment m = {0.0f, 0.0f, 0.0f};
-    if (base + x < p.channels) {
+    if (base + p.x < p.channels) {
 #pragma unroll 8
-      for (int i = y; i < s.chunks; i += 32) {
-        const float2 v = parts[static_cast<long long>(i) * s.channels + base + x];
+      for (int i = p.y; i < s.chunks; i += p.lanes) {
+        const float2 v = parts[static_cast<long long>(i) * s.channels + base + p.x];
         m.join({i + 1 < s.chunks ? chunk_count : last_count, v.x, v.y});
       }
     }
-    entry[y][x] = make_float2(m.mean, m.squares);
+    entry[p.y * (p.width + 1) + p.x] = make_float2(m.mean, m.squares);
     __syncthreads();
-    // Channel y, from its 32 lanes; lane i has ceil((chunks - i) / 32) chunks.
-    const float2 v = entry[x][y];
-    const int chunks = x < s.chunks ? (s.chunks - x + 31) / 32 : 0;
-    const bool last = chunks > 0 && (s.chunks - 1) % 32 == x;
-    m = {chunk_count * static_cast<float>(chunks - (last ? 1 : 0)) + (last ? last_count : 0.0f),
-         v.x, v.y};
-    m.join_warp();
-    if (x == 0) channel[y] = base + y < p.channels ? m : Moment{0.0f, 0.0f, 0.0f};
+    // Channel `warp`, from its lanes; lane i has ceil((chunks - i) / lanes) chunks.
+    if (warp < p.width) {
+      m = {0.0f, 0.0f, 0.0f};
+      for (int i = lane; i < p.lanes; i += 32) {
+        const float2 v = entry[i * (p.width + 1) + warp];
+        const int chunks = i < s.chunks ? (s.chunks - i + p.lanes - 1) / p.lanes : 0;
+        const bool last = chunks > 0 && (s.chunks - 1) % p.lanes == i;
+        m.join({chunk_count * static_cast<float>(chunks - (last ? 1 : 0)) +
+                    (last ? last_count : 0.0f),
+                v.x, v.y});
+      }
+      m.join_warp();
+      if (lane == 0) channel[warp] = base + warp < p.channels ? m : Moment{0.0f, 0.0f, 0.0f};
+    }
     __syncthreads();
-    if (y == 0) {
-      m = channel[x];
+    if (warp == 0) {
       if (d > 32) {
+        m = channel[lane];
         m.join_warp();
         if (base == 0)
           wide = m;
         else
           wide.join(m);
-      } else if (x < p.channels) {
-        const int g = x / d;
+      } else if (lane < p.channels) {
+        const int g = lane / d;
         Moment group = channel[g * d];
         for (int i = 1; i < d; ++i) group.join(channel[g * d + i]);
         const float r = rstd_of(group, eps);
-        if (x == g * d) rstd[p.group + g] = r;
-        write(p.channel + x, group.mean, r);
+        if (lane == g * d) rstd[g] = r;
+        write(lane, group.mean, r);
       }
     }
     __syncthreads();
@@ -157,11 +163,10 @@ __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(
   if (d <= 32) return;
   if (threadIdx.x == 0) {
     result = make_float2(wide.mean, rstd_of(wide, eps));
-    rstd[p.group] = result.y;
+    rstd[0] = result.y;
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < p.channels; c += kJoinThreads)
-    write(p.channel + c, result.x, result.y);
+  for (int c = threadIdx.x; c < p.channels; c += kJoinThreads) write(c, result.x, result.y);
 }
 
 // Second pass: normalise, scale, activate and drop one chunk of rows in one tile of columns. Blocks

@@ -391,19 +391,31 @@ struct Affine {
   }
 };
 
-// Threads of the kernels that join the blocks' sums: 32 channels by 32 lanes. A block has a run of
-// whole groups of at most 32 channels together, or one group.
+// The kernels that join the blocks' sums: a block has a run of whole groups of at most 8 channels
+// together, or one group, of which it takes 8, 16 or 32 channels at a time (`width`) by as many
+// lanes as it has threads for. With 32 channels to every block, two blocks read all the parts of 64
+// channels, in 10 us; they are the only work between the two passes.
 constexpr int kJoinThreads = 1024;
+
+__host__ __device__ inline int join_run(int group_channels) {
+  return group_channels > 8 ? 1 : 8 / group_channels;
+}
 
 struct JoinPlace {
   int view, group, channel, channels;  // first group and channel, and its channels
+  int width, lanes, x, y;              // channels at a time, and the thread's place
 
   __device__ __forceinline__ JoinPlace(const NormShape& s, int view0) {
-    const int run = s.group_channels > 32 ? 1 : 32 / s.group_channels;
+    const int run = join_run(s.group_channels);
     view = view0 + blockIdx.y;
     group = blockIdx.x * run;
     channel = group * s.group_channels;
     channels = min(run, s.groups - group) * s.group_channels;
+    const int shift = s.group_channels > 16 ? 5 : s.group_channels > 8 ? 4 : 3;
+    width = 1 << shift;
+    lanes = kJoinThreads >> shift;
+    x = threadIdx.x & (width - 1);
+    y = threadIdx.x >> shift;
   }
 };
 
@@ -507,7 +519,7 @@ inline bool too_large(long long batch, long long pixels) {
 
 // Blocks for each view of the kernels that join the blocks' sums (see JoinPlace).
 inline unsigned int join_runs(const NormShape& s) {
-  const int run = s.group_channels > 32 ? 1 : 32 / s.group_channels;
+  const int run = join_run(s.group_channels);
   return static_cast<unsigned int>((s.groups + run - 1) / run);
 }
 
@@ -523,17 +535,20 @@ inline int views_at_once(long long batch, long long pixels, int channels, int dt
       std::max(1LL, std::min({batch, 65535LL, (envv("DRX_PART", 72) << 20) / std::max(1LL, view)})));
 }
 
-// The plan of a call in passes over memory: chunks for `kNormBlocks` blocks in a launch, of 8 KB at
-// least.
-constexpr int kNormBlocks = 8 * 148;
-
+// The plan of a call in passes over memory. A block's start and the join of its sums cost as much
+// as 16 rows of its threads, so chunks have about 64 KB (16 rows of 256 vectors); blocks fill the
+// processors evenly, up to `resident` to each, or several times over.
 inline void plan_passes(NormShape& s, const NormVector& v, long long batch, long long pixels,
                         int channels, int groups, int dtype, long long x_stride,
                         long long grad_stride, int images) {
   const long long view = pixels * channels * dtype_bytes(dtype);
   const long long part = view * views_at_once(batch, pixels, channels, dtype, images);
+  const long long processors = 148, resident = images == 1 ? 4 : 3, chunk = envv("DRX_CHUNK", 65536);
+  const long long each = (part + processors * chunk / 2) / (processors * chunk);
+  const long long blocks = each <= resident ? std::max(1LL, each) * processors
+                                            : (each + resident / 2) / resident * resident * processors;
   cut_norm(s, v, batch, pixels, channels, groups, dtype, x_stride, grad_stride, kNormThreads,
-           std::max(8192LL, part / envv("DRX_BLOCKS", kNormBlocks)));
+           std::max(4096LL, (part + blocks - 1) / blocks));
 }
 
 // Workspace: a pair of each channel for each chunk; for the backward pass also one of each view and

@@ -100,12 +100,11 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_sums_kernel(
 __global__ void __launch_bounds__(kJoinThreads) norm_means_kernel(
     const float2* parts, NormShape s, int view0, const float* __restrict__ affine,
     const float* __restrict__ rstd, float2* __restrict__ sums, float* __restrict__ table) {
-  __shared__ float2 entry[32][33];
+  __shared__ float2 entry[kJoinThreads + kJoinThreads / 8];
   __shared__ float2 scaled[32];
   __shared__ float2 result;  // of a group wider than 32 channels
   let_next_kernel_start();
   const JoinPlace p(s, view0);
-  const int x = threadIdx.x % 32, y = threadIdx.x / 32;
   const int d = s.group_channels;
   // rstd * weight of the channels
   affine += (static_cast<long long>(p.view) * 3 + 1) * s.channels + p.channel;
@@ -115,40 +114,45 @@ __global__ void __launch_bounds__(kJoinThreads) norm_means_kernel(
   table += static_cast<long long>(p.view) * 2 * s.channels + p.channel;
   wait_for_kernel_before();
   const float inverse = 1.0f / (static_cast<float>(s.pixels) * static_cast<float>(d));
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   float2 wide = make_float2(0.0f, 0.0f);
-  for (int base = 0; base < p.channels; base += 32) {
+  for (int base = 0; base < p.channels; base += p.width) {
     float2 total = make_float2(0.0f, 0.0f);
-    if (base + x < p.channels) {
+    if (base + p.x < p.channels) {
 #pragma unroll 8
-      for (int i = y; i < s.chunks; i += 32)
-        total = add2(total, parts[static_cast<long long>(i) * s.channels + base + x]);
+      for (int i = p.y; i < s.chunks; i += p.lanes)
+        total = add2(total, parts[static_cast<long long>(i) * s.channels + base + p.x]);
     }
-    entry[y][x] = total;
+    entry[p.y * (p.width + 1) + p.x] = total;
     __syncthreads();
-    // Channel y, from its 32 lanes.
-    total = entry[x][y];
-    total.x = warp_sum(total.x);
-    total.y = warp_sum(total.y);
-    if (x == 0) {
-      float2 w = make_float2(0.0f, 0.0f);
-      if (base + y < p.channels) {
-        const float r = rstd[(base + y) / d], scale = affine[base + y];
-        sums[base + y] = make_float2(total.x, total.y * r);
-        w = make_float2(total.x * scale, total.y * scale * r);
+    // Channel `warp`, from its lanes.
+    if (warp < p.width) {
+      total = make_float2(0.0f, 0.0f);
+      for (int i = lane; i < p.lanes; i += 32) total = add2(total, entry[i * (p.width + 1) + warp]);
+      total.x = warp_sum(total.x);
+      total.y = warp_sum(total.y);
+      if (lane == 0) {
+        float2 w = make_float2(0.0f, 0.0f);
+        const int c = base + warp;
+        if (c < p.channels) {
+          const float r = rstd[c / d], scale = affine[c];
+          sums[c] = make_float2(total.x, total.y * r);
+          w = make_float2(total.x * scale, total.y * scale * r);
+        }
+        scaled[warp] = w;
       }
-      scaled[y] = w;
     }
     __syncthreads();
-    if (y == 0) {
+    if (warp == 0) {
       if (d > 32) {
-        wide.x += warp_sum(scaled[x].x);
-        wide.y += warp_sum(scaled[x].y);
-      } else if (x < p.channels) {
-        const int g = x / d;
+        wide.x += warp_sum(scaled[lane].x);
+        wide.y += warp_sum(scaled[lane].y);
+      } else if (lane < p.channels) {
+        const int g = lane / d;
         float2 group = scaled[g * d];
         for (int i = 1; i < d; ++i) group = add2(group, scaled[g * d + i]);
-        table[x] = -group.x * inverse;
-        table[s.channels + x] = -group.y * inverse * rstd[g];
+        table[lane] = -group.x * inverse;
+        table[s.channels + lane] = -group.y * inverse * rstd[g];
       }
     }
     __syncthreads();
