@@ -706,48 +706,47 @@ class Lambert(torch.autograd.Function):
 
 
 class GroupNorm(torch.autograd.Function):
-    """Group normalisation with an activation and dropout of a feature image. ``drop`` comes
-    without its seed tensor, which is an input of its own: saved like the others, a seed that was
-    changed in place between the passes is reported instead of giving another mask."""
+    """Group normalisation with an activation and dropout of a feature image. The seed tensor is
+    saved like the other inputs, so that one changed in place between the passes is reported
+    instead of giving another mask. ``options``: (groups, eps, activation, drop)."""
 
     @staticmethod
     def forward(ctx, x: Tensor, weight: Tensor | None, bias: Tensor | None, seed: Tensor | None,
-                groups: int, eps: float, activation: int, drop: K.Drop):
-        y, state = K.group_norm_fwd(x, groups, weight, bias, eps, activation,
-                                    drop._replace(seed=seed))
-        ctx.save_for_backward(*(_saveable(t) for t in (x, weight, bias, seed, state)))
-        ctx.groups, ctx.activation, ctx.drop = groups, activation, drop
+                options: tuple):
+        groups, eps, activation, drop = options
+        y, state = K.group_norm_fwd(x, groups, weight, bias, eps, activation, drop, seed)
+        ctx.save_for_backward(_saveable(x), _saveable(weight), _saveable(bias), _saveable(seed),
+                              state)
+        ctx.options = options
         return y
 
     @staticmethod
     @first_order("group_norm")
     def backward(ctx, grad_out):
         x, weight, bias, seed, state = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        grads = K.group_norm_bwd(x, grad_out, ctx.groups, weight if need[1] else None,
-                                 bias if need[2] else None, state, ctx.activation,
-                                 ctx.drop._replace(seed=seed), need[0])
-        return *grads, None, None, None, None, None
+        groups, _, activation, drop = ctx.options
+        need_x, need_w, need_b, _, _ = ctx.needs_input_grad
+        grads = K.group_norm_bwd(x, grad_out, groups, weight if need_w else None,
+                                 bias if need_b else None, state, activation, drop, seed, need_x)
+        return *grads, None, None
 
 
 class Dropout(torch.autograd.Function):
-    """``residual + dropout(x)``; ``drop`` and ``seed`` as for :class:`GroupNorm`."""
+    """``residual + dropout(x)``; ``seed`` as for :class:`GroupNorm`."""
 
     @staticmethod
     def forward(ctx, x: Tensor, residual: Tensor | None, seed: Tensor | None, drop: K.Drop):
         ctx.save_for_backward(_saveable(seed))
         ctx.drop = drop
-        return K.dropout(x, residual, drop._replace(seed=seed))
+        return K.dropout(x, residual, drop, seed)
 
     @staticmethod
     @first_order("dropout")
     def backward(ctx, grad_out):
         (seed,) = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        grad_x = None
-        if need[0]:
-            grad_x = K.dropout(grad_out.contiguous(), None, ctx.drop._replace(seed=seed))
-        return grad_x, grad_out if need[1] else None, None, None
+        need_x, need_residual, _, _ = ctx.needs_input_grad
+        grad_x = K.dropout(grad_out.contiguous(), None, ctx.drop, seed) if need_x else None
+        return grad_x, grad_out if need_residual else None, None, None
 
 
 class ToClip(torch.autograd.Function):

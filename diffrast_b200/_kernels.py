@@ -765,13 +765,15 @@ def antialias_mse_bwd(color, rast, pos3, tri, opposite, residual, loss_grad, sca
 
 
 class Drop(NamedTuple):
-    """Dropout of a call: ``threshold`` in 2**-16 (0: none), the seed as a device word or a
-    number, and the layer."""
+    """Dropout of a call: ``threshold`` in 2**-16 (0: none), the seed as a number (used where the
+    call gets no seed tensor), and the layer."""
 
     threshold: int
-    seed: Tensor | None
     value: int
     layer: int
+
+
+NO_DROP = Drop(0, 0, 0)
 
 
 def feature_rows(t: Tensor) -> tuple[Tensor, int]:
@@ -796,6 +798,11 @@ def feature_rows(t: Tensor) -> tuple[Tensor, int]:
     return t, channels if row is None else row
 
 
+def _contiguous_like(t: Tensor) -> Tensor:
+    """An uninitialised contiguous tensor of ``t``'s shape, type and device."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 @functools.lru_cache(maxsize=256)
 def _norm_workspace_bytes(batch, pixels, channels, groups, dtype, backward) -> int:
     return N.lib().dr_group_norm_workspace_bytes(batch, pixels, channels, groups, dtype, backward)
@@ -810,22 +817,24 @@ def _param(t: Tensor | None, channels: int) -> tuple[int | None, int, int]:
 
 @timed("group_norm_fwd")
 def group_norm_fwd(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor | None, eps: float,
-                   activation: int, drop: Drop) -> tuple[Tensor, Tensor]:
+                   activation: int, drop: Drop, seed: Tensor | None) -> tuple[Tensor, Tensor]:
     """``(y, state)``: the normalised image and what the backward pass needs beside ``x``.
     ``x`` is ``[batch, ..., channels]`` and not empty."""
     x, stride = feature_rows(x)
-    batch, channels = x.shape[0], x.shape[-1]
+    shape = x.shape
+    batch, channels = shape[0], shape[-1]
     pixels = x.numel() // (batch * channels)
     dtype = N.FEATURE_DTYPES[x.dtype]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    state = torch.empty(batch * (3 * channels + groups), dtype=torch.float32, device=x.device)
-    work = _scratch(_norm_workspace_bytes(batch, pixels, channels, groups, dtype, 0), x.device)
+    y = _contiguous_like(x)
+    state = x.new_empty(batch * (3 * channels + groups), dtype=torch.float32)
+    nbytes = _norm_workspace_bytes(batch, pixels, channels, groups, dtype, 0)
+    work = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     N.check(
         N.lib().dr_group_norm_fwd(x.data_ptr(), stride, dtype, batch, pixels, channels, groups,
                                   *_param(weight, channels), *_param(bias, channels), eps,
-                                  activation, drop.threshold, N.ptr(drop.seed), drop.value,
-                                  drop.layer, y.data_ptr(), state.data_ptr(), work.data_ptr(),
-                                  work.numel(), N.stream(x.device)),
+                                  activation, drop.threshold, N.ptr(seed), drop.value, drop.layer,
+                                  y.data_ptr(), state.data_ptr(), N.ptr(work), nbytes,
+                                  N.stream(x.device)),
         "dr_group_norm_fwd",
     )  # fmt: skip
     return y, state
@@ -834,24 +843,26 @@ def group_norm_fwd(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor |
 @timed("group_norm_bwd")
 def group_norm_bwd(x: Tensor, grad_y: Tensor, groups: int, weight: Tensor | None,
                    bias: Tensor | None, state: Tensor, activation: int, drop: Drop,
-                   need_x: bool) -> tuple[Tensor | None, ...]:
+                   seed: Tensor | None, need_x: bool) -> tuple[Tensor | None, ...]:
     """Gradients of x (contiguous), weight and bias: into new tensors like ``weight`` and ``bias``,
     which are None where no gradient is needed."""
     x, stride = feature_rows(x)
     grad_y, grad_stride = feature_rows(grad_y)
-    batch, channels = x.shape[0], x.shape[-1]
+    shape = x.shape
+    batch, channels = shape[0], shape[-1]
     pixels = x.numel() // (batch * channels)
     dtype = N.FEATURE_DTYPES[x.dtype]
-    grad_x = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+    grad_x = _contiguous_like(x) if need_x else None
     grad_w = None if weight is None else torch.empty_like(weight)
     grad_b = None if bias is None else torch.empty_like(bias)
-    work = _scratch(_norm_workspace_bytes(batch, pixels, channels, groups, dtype, 1), x.device)
+    nbytes = _norm_workspace_bytes(batch, pixels, channels, groups, dtype, 1)
+    work = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     N.check(
         N.lib().dr_group_norm_bwd(x.data_ptr(), stride, grad_y.data_ptr(), grad_stride, dtype,
                                   batch, pixels, channels, groups, state.data_ptr(), activation,
-                                  drop.threshold, N.ptr(drop.seed), drop.value, drop.layer,
+                                  drop.threshold, N.ptr(seed), drop.value, drop.layer,
                                   N.ptr(grad_x), *_param(grad_w, channels),
-                                  *_param(grad_b, channels), work.data_ptr(), work.numel(),
+                                  *_param(grad_b, channels), N.ptr(work), nbytes,
                                   N.stream(x.device)),
         "dr_group_norm_bwd",
     )  # fmt: skip
@@ -859,12 +870,12 @@ def group_norm_bwd(x: Tensor, grad_y: Tensor, groups: int, weight: Tensor | None
 
 
 @timed("dropout")
-def dropout(x: Tensor, residual: Tensor | None, drop: Drop) -> Tensor:
+def dropout(x: Tensor, residual: Tensor | None, drop: Drop, seed: Tensor | None) -> Tensor:
     """``residual + dropout(x)`` of contiguous tensors (also the gradient of x, without residual)."""
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x)
     N.check(
         N.lib().dr_dropout(x.data_ptr(), N.ptr(residual), x.numel(), N.FEATURE_DTYPES[x.dtype],
-                           drop.threshold, N.ptr(drop.seed), drop.value, drop.layer, y.data_ptr(),
+                           drop.threshold, N.ptr(seed), drop.value, drop.layer, y.data_ptr(),
                            N.stream(x.device)),
         "dr_dropout",
     )  # fmt: skip

@@ -9,6 +9,7 @@ other backend and no CPU fallback: tensors on the CPU pass validation and then r
 
 from __future__ import annotations
 
+import contextlib
 import operator
 from collections.abc import Sequence
 from typing import Literal, SupportsFloat, get_args
@@ -699,17 +700,19 @@ def group_norm(
     if activation not in N.ACTIVATIONS:
         options = ", ".join(repr(a) for a in N.ACTIVATIONS)
         raise ValueError(f"Unknown activation {activation!r}; expected one of {options}.")
-    if not isinstance(eps, SupportsFloat) or not 0.0 <= float(eps) < float("inf"):
+    if not isinstance(eps, (float, SupportsFloat)) or not 0.0 <= float(eps) < float("inf"):
         raise ValueError(f"eps must be a finite number of at least 0, got {eps!r}.")
-    drop, seed = _check_dropout(dropout, seed, layer, x)
+    drop = K.NO_DROP
+    if dropout != 0.0 or seed is not None or layer != 0:
+        drop, seed = _check_dropout(dropout, seed, layer, x)
     require_cuda(x.device)
-    args = (groups, float(eps), N.ACTIVATIONS.index(activation), drop)
+    options = (groups, float(eps), N.ACTIVATIONS.index(activation), drop)
     if x.numel() == 0:
         return _empty_like(x, weight, bias)
-    with torch.cuda.device(x.device):
+    with _on_device(x):
         if _wants_grad(x, weight, bias):
-            return F.GroupNorm.apply(x, weight, bias, seed, *args)
-        return K.group_norm_fwd(x, groups, weight, bias, *args[1:3], drop._replace(seed=seed))[0]
+            return F.GroupNorm.apply(x, weight, bias, seed, options)
+        return K.group_norm_fwd(x, groups, weight, bias, *options[1:], seed)[0]
 
 
 def dropout(
@@ -752,14 +755,27 @@ def dropout(
         return _empty_like(x, residual)
     x = x.contiguous()
     residual = None if residual is None else residual.contiguous()
-    with torch.cuda.device(x.device):
+    with _on_device(x):
         if _wants_grad(x, residual):
             return F.Dropout.apply(x, residual, seed, drop)
-        return K.dropout(x, residual, drop._replace(seed=seed))
+        return K.dropout(x, residual, drop, seed)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on_device(t: Tensor):
+    """Makes ``t``'s device the current one (nothing to do where it is)."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
 def _empty_like(x: Tensor, *inputs) -> Tensor:
@@ -799,13 +815,13 @@ def _check_norm_param(t, name: str, x: Tensor) -> Tensor | None:
             f"{name} must have shape [channels] or [batch, channels], ({channels},) or "
             f"({batch}, {channels}) here, got {tuple(t.shape)}."
         )
-    _check_devices(**{"x": x, name: t})
+    if t.device != x.device:
+        _check_devices(**{"x": x, name: t})
     return t.contiguous()
 
 
 def _check_dropout(p, seed, layer, x: Tensor, name: str = "dropout"):
-    """Validate dropout arguments; returns ``(drop, seed tensor)``, the :class:`K.Drop` without
-    its seed tensor."""
+    """Validate dropout arguments; returns the :class:`K.Drop` and the seed tensor, if it is one."""
     if isinstance(p, bool) or not isinstance(p, SupportsFloat) or not 0.0 <= float(p) < 1.0:
         raise ValueError(f"{name} must be a probability in [0, 1), got {p!r}.")
     if isinstance(layer, bool) or not isinstance(layer, int) or not 0 <= layer < 1 << 32:
@@ -818,16 +834,16 @@ def _check_dropout(p, seed, layer, x: Tensor, name: str = "dropout"):
                 f"{seed.dtype} of shape {tuple(seed.shape)}."
             )
         _check_devices(x=x, seed=seed)
-        return K.Drop(threshold, None, 0, layer), seed
+        return K.Drop(threshold, 0, layer), seed
     if seed is None:
         if threshold:
             raise ValueError("seed is required with dropout.")
-        return K.Drop(0, None, 0, layer), None
+        return K.NO_DROP, None
     if isinstance(seed, bool) or not isinstance(seed, int):
         raise TypeError(f"seed must be an int or an int64 tensor of one element, got {seed!r}.")
     if not 0 <= seed < 1 << 63:
         raise ValueError(f"seed must be in [0, 2**63), got {seed}.")
-    return K.Drop(threshold, None, seed, layer), None
+    return K.Drop(threshold, seed, layer), None
 
 
 def to_clip(positions: Tensor, matrix: Tensor) -> Tensor:
