@@ -8,37 +8,34 @@ namespace {
 constexpr int kStages = 8;  // rows that a thread has under way
 
 // Joins the threads' moments of a block's rows into those of each channel: over the rows of a warp
-// where the tile's columns divide it, then over the lines of rows that are left. `done` gets the
-// channel, counted from the tile's first, and the moment.
+// where the tile's columns divide it, then over the lines of rows that are left. `n` is the
+// thread's count, `valid` the tile's channels (with folded pixels: the view's). `done` gets the
+// channel, counted from the tile's first, and (mean, squared deviations), zeros without any rows.
 template <int V, typename Done>
-__device__ __forceinline__ void join_block(Moments<V>& m, const NormPlace& p, const NormShape& s,
-                                           void* shared, Done done) {
-  auto* entry = static_cast<float2*>(shared);  // [lines][tile_cols * V]
-  __shared__ float counts[kNormThreads];       // of the lines
-  float n = static_cast<float>(p.count);
+__device__ __forceinline__ void join_block(Moments<V>& m, float n, const TileThread& t,
+                                           const NormShape& s, int valid, float2* entry,
+                                           Done done) {
+  __shared__ float counts[kNormThreads];  // of the lines
   m.finish(n);
-  int lines = s.lanes, line = threadIdx.y;
-  bool write = true;
-  if (warp_holds_rows()) {
-    for (int d = blockDim.x; d < 32; d *= 2) m.join_lane(d, n);
-    const int thread = threadIdx.y * blockDim.x + threadIdx.x;
+  int lines = s.lanes, line = t.y;
+  bool write = t.y < s.lanes;
+  if (warp_holds_rows(s.tile_cols)) {
+    for (int d = s.tile_cols; d < 32; d *= 2) m.join_lane(d, n);
     lines = kNormThreads / 32;
-    line = thread / 32;
-    write = thread % 32 < blockDim.x;
+    line = t.thread / 32;
+    write = t.thread % 32 < s.tile_cols;
   }
   const int width = s.tile_cols * V;
   __syncthreads();
   if (write) {
-    float2* to = entry + line * width + threadIdx.x * V;
+    float2* to = entry + line * width + t.x * V;
 #pragma unroll
     for (int j = 0; j < V; ++j) to[j] = make_float2(m.sum.get(j), m.square.get(j));
-    if (threadIdx.x == 0) counts[line] = n;
+    if (t.x == 0) counts[line] = n;
   }
   __syncthreads();
   const int items = s.fold > 1 ? s.channels : width;
-  const int valid = s.fold > 1 ? items : min(width, s.cols * V - (p.col - static_cast<int>(threadIdx.x) * V));
-  for (int item = threadIdx.y * blockDim.x + threadIdx.x; item < valid;
-       item += blockDim.x * blockDim.y) {
+  for (int item = t.thread; item < valid; item += t.threads) {
     const float2 first = entry[item];
     float total_n = 0.0f, total = 0.0f;
     for (int l = 0; l < lines; ++l) {
@@ -48,7 +45,7 @@ __device__ __forceinline__ void join_block(Moments<V>& m, const NormPlace& p, co
         total = fmaf(c, entry[l * width + f * items + item].x - first.x, total);
       }
     }
-    const float offset = __fdividef(total, total_n);
+    const float offset = total_n > 0.0f ? __fdividef(total, total_n) : 0.0f;
     float squares = 0.0f;
     for (int l = 0; l < lines; ++l) {
       const float c = counts[l];
@@ -84,7 +81,13 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_stats_kernel(const T* __
   });
   parts += (static_cast<long long>(p.view) * s.chunks + p.chunk) * s.channels;
   if (s.fold == 1) parts += blockIdx.y * s.tile_cols * V;
-  join_block<V>(m, p, s, shared, [&](int item, float2 moment) { parts[item] = moment; });
+  const int tile_col = blockIdx.y * s.tile_cols;
+  const int valid = s.fold > 1 ? s.channels : min(s.tile_cols, s.cols - tile_col) * V;
+  const TileThread t = {static_cast<int>(threadIdx.x), static_cast<int>(threadIdx.y),
+                        static_cast<int>(threadIdx.y * blockDim.x + threadIdx.x),
+                        static_cast<int>(blockDim.x * blockDim.y)};
+  join_block<V>(m, static_cast<float>(p.count), t, s, valid, reinterpret_cast<float2*>(shared),
+                [&](int item, float2 moment) { parts[item] = moment; });
   wait_for_kernel_before();
 }
 
@@ -172,7 +175,7 @@ __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(
 // Second pass: normalise, scale, activate and drop one chunk of rows in one tile of columns. Blocks
 // run from the end of the views to their start: what the first pass read last is still in L2.
 template <typename T, int V, bool Silu, bool Drop>
-__global__ void __launch_bounds__(kNormThreads, 4) norm_apply_kernel(
+__global__ void __launch_bounds__(kNormThreads, Drop ? 3 : 4) norm_apply_kernel(
     const T* __restrict__ x, NormShape s, int view0, const float* table, float bound, DropKey key,
     T* __restrict__ y) {
   extern __shared__ uint4 shared[];
@@ -202,13 +205,125 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_apply_kernel(
   });
 }
 
+// The whole pass by clusters of blocks (see "clusters" in group_norm.cuh).
 template <typename T, int V, bool Silu, bool Drop>
-int passes(const void* x, const NormShape& s, int dtype, const NormParam& weight,
-           const NormParam& bias, float eps, float bound, const DropKey& key, void* y, float* table,
+__global__ void __launch_bounds__(kNormThreads, Drop ? 3 : 4) norm_cluster_kernel(
+    const T* __restrict__ x, NormShape s, ClusterPlan t, NormParam weight, NormParam bias,
+    float eps, float bound, DropKey key, T* __restrict__ y, float* __restrict__ table,
+    float* __restrict__ rstd) {
+  extern __shared__ uint4 shared[];
+  auto* bytes = reinterpret_cast<unsigned char*>(shared);
+  auto* entry = reinterpret_cast<float2*>(bytes + t.slots);
+  const int width = s.tile_cols * V;
+  auto* channel = reinterpret_cast<float2*>(bytes + t.slots + t.entries);  // [width]
+  auto* constants = reinterpret_cast<float*>(channel + width);             // [3][width]
+  const ClusterShare p(s, t, V);
+  SlabRows<T, V, 1> rows;
+  rows.slots = static_cast<unsigned int>(__cvta_generic_to_shared(shared)) +
+               threadIdx.x * static_cast<unsigned int>(sizeof(Packed<T, V>));
+  rows.count = p.mine;
+  rows.fetch({x + p.first * s.x_row + p.col}, {s.lanes * s.x_row});
+  // Weight and bias, while the rows are on their way.
+  for (int item = threadIdx.x; item < p.channels; item += kNormThreads) {
+    constants[width + item] = load_scale(weight, p.view, p.channel + item);
+    constants[2 * width + item] = load_shift(bias, p.view, p.channel + item);
+  }
+  copy_wait<0>();
+  Moments<V> m;
+  m.clear();
+  bool first = true;
+  rows.for_rows([&](const Pairs<V> (&v)[1]) {
+    if (first) m.start(v[0]);
+    first = false;
+    m.add(v[0]);
+  });
+  join_block<V>(m, static_cast<float>(p.mine), p.at, s, p.channels, entry,
+                [&](int item, float2 moment) { channel[item] = moment; });
+  const int d = s.group_channels;
+  float2* joined = channel;
+  if (t.size > 1) {
+    auto cluster = cooperative_groups::this_cluster();
+    cluster.sync();
+    joined = entry;  // its readers are behind the cluster's barrier
+    for (int item = threadIdx.x; item < p.channels; item += kNormThreads) {
+      float2 v[kMostCluster];
+#pragma unroll
+      for (int r = 0; r < kMostCluster; ++r)
+        if (r < t.size) v[r] = *cluster.map_shared_rank(channel + item, r);
+      Moment c = {0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int r = 0; r < kMostCluster; ++r)
+        if (r < t.size) c.join({p.values_of(s, t, r), v[r].x, v[r].y});
+      joined[item] = make_float2(c.mean, c.squares);
+    }
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  }
+  __syncthreads();
+  // The groups' moments, and from them the channels' constants.
+  const int groups = p.channels / d;
+  const int lanes = lanes_for(groups), lane = threadIdx.x & (lanes - 1);
+  const int step = kNormThreads / lanes;
+  const float all = static_cast<float>(s.pixels);
+  for (int base = 0; base < groups; base += step) {
+    const int g = base + threadIdx.x / lanes;
+    Moment c = {0.0f, 0.0f, 0.0f};
+    if (g < groups) {
+      for (int i = lane; i < d; i += lanes) {
+        const float2 v = joined[g * d + i];
+        c.join({all, v.x, v.y});
+      }
+    }
+    for (int e = 1; e < lanes; e *= 2) c.join(c.lane(e));
+    const int leader = (threadIdx.x & 31) & ~(lanes - 1);
+    const float mean = __shfl_sync(0xFFFFFFFFu, c.mean, leader);
+    const float r = __shfl_sync(0xFFFFFFFFu, rstd_of(c, eps), leader);
+    if (g < groups) {
+      for (int i = lane; i < d; i += lanes) {
+        const int item = g * d + i;
+        const float scale = r * constants[width + item], offset = constants[2 * width + item];
+        constants[item] = -mean;
+        constants[width + item] = scale;
+        if (p.rank == 0) {
+          float* row = table + static_cast<long long>(p.view) * 3 * s.channels + p.channel + item;
+          row[0] = -mean;
+          row[s.channels] = scale;
+          row[2 * s.channels] = offset;
+        }
+      }
+      if (p.rank == 0 && lane == 0)
+        rstd[static_cast<long long>(p.view) * s.groups + p.channel / d + g] = r;
+    }
+  }
+  __syncthreads();
+  if (p.mine > 0) {
+    const Pairs<V> shift = load_constants<V>(constants, s, p);
+    const Pairs<V> scale = load_constants<V>(constants + width, s, p);
+    const Pairs<V> offset = load_constants<V>(constants + 2 * width, s, p);
+    const unsigned long long seed = Drop ? load_seed(key) : 0;
+    const long long out_row = static_cast<long long>(s.channels) * s.fold;
+    long long at = p.first * out_row + p.col;
+    const long long stride = s.lanes * out_row;
+    rows.for_rows([&](const Pairs<V> (&v)[1]) {
+      Pairs<V> z;
+#pragma unroll
+      for (int j = 0; j < Pairs<V>::kCount; ++j)
+        z.p[j] = activate<Silu>(fma2(add2(v[0].p[j], shift.p[j]), scale.p[j], offset.p[j]), bound);
+      if (Drop) apply_dropout<V>(z, at, key, seed);
+      __stcs(reinterpret_cast<Packed<T, V>*>(y + at), pack_pairs<T, V>(z));
+      at += stride;
+    });
+  }
+  // No block ends while another may still read its sums.
+  if (t.size > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+template <typename T, int V, bool Silu, bool Drop>
+int passes(const void* x, const NormShape& s, const NormParam& weight, const NormParam& bias,
+           float eps, float bound, const DropKey& key, void* y, float* table,
            float* rstd, float2* parts, cudaStream_t stream) {
   const T* in = static_cast<const T*>(x);
   T* out = static_cast<T*>(y);
-  const int most = views_at_once(s.batch, s.pixels, s.channels, dtype, 1);
+  const int most = views_at_once(s.batch);
   const unsigned int runs = join_runs(s);
   const dim3 threads(s.tile_cols, s.lanes);
   constexpr size_t ring = RowRing<T, V, 1, kStages>::kBytes;
@@ -264,10 +379,16 @@ extern "C" int dr_group_norm_fwd(const void* x, int64_t x_stride, int32_t dtype,
     return DR_ERR_INVALID_ARGUMENT;
   if (too_large(batch, pixels)) return DR_ERR_TOO_LARGE;
   NormShape s;
+  ClusterPlan t;
   const NormVector v = choose_vector(pixels, channels, dtype, x_stride, channels, {x, y});
-  plan_passes(s, v, batch, pixels, channels, groups, dtype, x_stride, channels, 1);
-  if (workspace == nullptr || workspace_bytes < norm_space(s, false).total)
-    return DR_ERR_WORKSPACE_TOO_SMALL;
+  const bool clusters = plan_clusters(s, t, v, batch, pixels, channels, groups, dtype, x_stride,
+                                      channels, 1, kResident[0], processors());
+  if (!clusters) {
+    plan_passes(s, v, batch, pixels, channels, groups, dtype, x_stride, channels, kResident[0],
+                processors());
+    if (workspace == nullptr || workspace_bytes < norm_space(s, false).total)
+      return DR_ERR_WORKSPACE_TOO_SMALL;
+  }
   auto param = [&](const void* data, int32_t type, int64_t rows) {
     return data != nullptr ? NormParam{data, true, type, rows > 1 ? channels : 0}
                            : NormParam{state, false, DR_FLOAT32, 0};
@@ -279,8 +400,13 @@ extern "C" int dr_group_norm_fwd(const void* x, int64_t x_stride, int32_t dtype,
   float* rstd = state + static_cast<size_t>(batch) * 3 * channels;
   return with_variant(dtype, v.vec, activation, drop_threshold, [&](auto k) {
     using K = decltype(k);
-    return passes<typename K::Type, K::kVec, K::kSilu, K::kDrop>(
-        x, s, dtype, w, b, eps, bound, key, y, state, rstd, static_cast<float2*>(workspace),
+    using T = typename K::Type;
+    if (clusters)
+      return launch_clusters<norm_cluster_kernel<T, K::kVec, K::kSilu, K::kDrop>>(
+          t, as_stream(stream), static_cast<const T*>(x), s, t, w, b, eps, bound, key,
+          static_cast<T*>(y), state, rstd);
+    return passes<T, K::kVec, K::kSilu, K::kDrop>(
+        x, s, w, b, eps, bound, key, y, state, rstd, static_cast<float2*>(workspace),
         as_stream(stream));
   });
 }

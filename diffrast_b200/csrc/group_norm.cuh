@@ -26,9 +26,13 @@
 #pragma once
 
 #include <algorithm>
+#include <atomic>
+#include <cmath>
 #include <cstdint>
 #include <initializer_list>
 #include <type_traits>
+
+#include <cooperative_groups.h>
 
 #include "philox.cuh"
 #include "vector.cuh"
@@ -224,8 +228,8 @@ __device__ __forceinline__ float warp_sum(float v) {
 
 // Whether the rows of a warp's threads are joined by shuffles before the block's: the tile's
 // columns divide the warp.
-__device__ __forceinline__ bool warp_holds_rows() {
-  return blockDim.x < 32 && 32 % blockDim.x == 0;
+__host__ __device__ inline bool warp_holds_rows(int tile_cols) {
+  return tile_cols < 32 && 32 % tile_cols == 0;
 }
 
 // A block's place: a chunk of rows, a tile of columns and a view; and its threads'.
@@ -419,6 +423,134 @@ struct JoinPlace {
   }
 };
 
+// ---- clusters ----------------------------------------------------------------------------------
+//
+// A slab is a tile of whole groups of one view. Where a cluster of blocks can hold one in shared
+// memory, each block copies its share of the rows, sums over it, reads the other blocks' sums of
+// each channel from their shared memory, and finishes its rows from its own: one launch, and the
+// image is read once and written once. (Larger teams, over all processors and through memory, had
+// some 18 us from one slab's copies to its results, and too little shared memory to cover that with
+// other slabs: 171 us for the 78 us of the two passes on four images of 512 x 512 x 64.)
+
+constexpr int kMostCluster = 16;
+
+struct ClusterPlan {
+  int size;              // blocks of a cluster
+  long long slabs;       // of all views
+  int block_rows;        // rows of a block's share
+  unsigned int slots;    // bytes of the rows
+  unsigned int entries;  // bytes of the joins' entries, after them
+  unsigned int shared;   // bytes in all
+};
+
+// A thread's place in a tile.
+struct TileThread {
+  int x, y;    // vector and row
+  int thread;  // of the block's
+  int threads;
+};
+
+// A block's share of a slab.
+struct ClusterShare {
+  int view, tile, rank, rows;
+  int col;           // first element of the thread's vector in a row
+  int mine;          // the thread's rows
+  int channel;       // first channel of the tile
+  int channels;      // of the tile
+  long long first;   // the thread's first row, counted over the views
+  TileThread at;
+
+  __device__ __forceinline__ ClusterShare(const NormShape& s, const ClusterPlan& t, int vec) {
+    at.thread = threadIdx.x;
+    at.threads = kNormThreads;
+    at.y = threadIdx.x / s.tile_cols;
+    at.x = threadIdx.x - at.y * s.tile_cols;
+    const unsigned int slab = blockIdx.x / t.size;
+    rank = static_cast<int>(blockIdx.x - slab * t.size);
+    view = static_cast<int>(slab / s.tiles);
+    tile = static_cast<int>(slab - view * static_cast<unsigned int>(s.tiles));
+    const long long row0 = static_cast<long long>(rank) * t.block_rows;
+    rows = static_cast<int>(max(0LL, min(static_cast<long long>(t.block_rows), s.rows - row0)));
+    const int x = tile * s.tile_cols + at.x;
+    col = x * vec;
+    mine = x < s.cols && at.y < s.lanes && at.y < rows ? (rows - at.y + s.lanes - 1) / s.lanes : 0;
+    channel = s.fold > 1 ? 0 : tile * s.tile_cols * vec;
+    channels = s.fold > 1 ? s.channels : min(s.tile_cols, s.cols - tile * s.tile_cols) * vec;
+    first = view * s.rows + row0 + at.y;
+  }
+
+  // Values of a channel in a rank's share.
+  __device__ __forceinline__ float values_of(const NormShape& s, const ClusterPlan& t, int r) const {
+    const long long left = s.rows - static_cast<long long>(r) * t.block_rows;
+    return static_cast<float>(max(0LL, min(static_cast<long long>(t.block_rows), left))) *
+           static_cast<float>(s.fold);
+  }
+};
+
+// The constants of a thread's channels out of a row of a tile's in shared memory.
+template <int V>
+__device__ __forceinline__ Pairs<V> load_constants(const float* row, const NormShape& s,
+                                                   const ClusterShare& p) {
+  Pairs<V> r;
+  if (V == 1) r.p[0].y = 0.0f;
+  int c = p.col - p.channel;
+  if (s.fold > 1) c %= s.channels;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    r.set(j, row[c]);
+    if (++c == s.channels && s.fold > 1) c = 0;
+  }
+  return r;
+}
+
+// Lanes (a power of two, at most 32) that a block's threads can give to each of `items`.
+__device__ __forceinline__ int lanes_for(int items) {
+  if (items >= kNormThreads) return 1;
+  return min(32, 1 << (31 - __clz(kNormThreads / items)));
+}
+
+// One thread's rows of a slab in shared memory.
+template <typename T, int V, int Images>
+struct SlabRows {
+  using P = Packed<T, V>;
+  static constexpr unsigned int kSlot = sizeof(P) * kNormThreads;
+
+  unsigned int slots;
+  int count;
+
+  // Starts the copies of rows first, first + lanes, ... of the images, `count` of them.
+  __device__ __forceinline__ void fetch(const T* const (&from)[Images],
+                                        const long long (&stride)[Images]) {
+    const T* at[Images];
+#pragma unroll
+    for (int k = 0; k < Images; ++k) at[k] = from[k];
+    unsigned int to = slots;
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) {
+#pragma unroll
+      for (int k = 0; k < Images; ++k) {
+        copy_async<sizeof(P)>(to + k * kSlot, at[k]);
+        at[k] += stride[k];
+      }
+      to += Images * kSlot;
+    }
+    copy_commit();
+  }
+
+  template <typename Use>
+  __device__ __forceinline__ void for_rows(Use use) const {
+    unsigned int at = slots;
+#pragma unroll 2
+    for (int i = 0; i < count; ++i) {
+      Pairs<V> v[Images];
+#pragma unroll
+      for (int k = 0; k < Images; ++k) v[k] = load_pairs<T, V>(load_slot<P>(at + k * kSlot));
+      use(v);
+      at += Images * kSlot;
+    }
+  }
+};
+
 // The kernels of a pass depend on one another and are launched with programmatic dependence: a
 // kernel's blocks may start while the last ones of the kernel before it run, and wait here before
 // they read its results (through pointers that are not __restrict__: a load that the compiler knows
@@ -523,32 +655,144 @@ inline unsigned int join_runs(const NormShape& s) {
   return static_cast<unsigned int>((s.groups + run - 1) / run);
 }
 
-// Bytes that both passes over a part of the views may read for the second one to find them in L2.
-constexpr long long kPartBytes = 72LL << 20;
+constexpr int kMostShared = 220 * 1024;  // dynamic shared memory of a block
 
-#include <cstdlib>
-inline long long envv(const char* n, long long d) { const char* e = getenv(n); return e ? atoll(e) : d; }
-// Views that are taken together, first pass and second: as many as stay in L2 in between.
-inline int views_at_once(long long batch, long long pixels, int channels, int dtype, int images) {
-  const long long view = pixels * channels * dtype_bytes(dtype) * images;
-  return static_cast<int>(
-      std::max(1LL, std::min({batch, 65535LL, (envv("DRX_PART", 72) << 20) / std::max(1LL, view)})));
+// Blocks of a processor that the kernels' registers allow, forward and backward.
+constexpr int kResident[2] = {4, 3};
+
+// Largest image that is taken in clusters. With the two passes, an image of 32 KB takes 8.0 us
+// forward and 6.9 us backward, in clusters 6.4 and 4.4 us, and two launches less; at 2 MB both
+// take 11 and 10 us, and at 8 MB the passes are a third faster.
+constexpr long long kClusterBytes = 1LL << 20;
+
+// The plan of a call in clusters, or false where none fits: tiles of whole groups, and blocks to a
+// cluster, by the estimated time in microseconds. A block's own is what is fixed (2, or 3 with a
+// cluster), its bytes at a processor's share of the memory, and its rows' instructions; the blocks
+// of a processor overlap, `resident` by registers and fewer by shared memory.
+inline bool plan_clusters(NormShape& s, ClusterPlan& t, const NormVector& v, long long batch,
+                          long long pixels, int channels, int groups, int dtype,
+                          long long x_stride, long long grad_stride, int images, int resident,
+                          int processors) {
+  const int d = channels / groups, size = dtype_bytes(dtype);
+  const int most_cols = kNormThreads / 2;
+  const int row_cols = static_cast<int>(static_cast<long long>(channels) * v.fold / v.vec);
+  const int unit = v.fold > 1 ? row_cols : d / greatest_divisor(d, v.vec);
+  const long long rows = pixels / v.fold;
+  double best = 1e30;
+  if (unit > most_cols || batch * pixels * channels * size > kClusterBytes) return false;
+  for (int cols = unit; cols <= std::min(row_cols, most_cols); cols *= 2) {
+    const long long tiles = (row_cols + cols - 1) / cols;
+    const long long slabs = batch * tiles;
+    const int lanes = kNormThreads / cols, width = cols * v.vec;
+    const int lines = warp_holds_rows(cols) ? kNormThreads / 32 : lanes;
+    const long long entries = static_cast<long long>(align256(sizeof(float2) * lines * width));
+    const long long extra = entries + static_cast<long long>(align256(20 * width));
+    const long long slot = static_cast<long long>(kNormThreads) * v.vec * size * images;
+    for (int team = 1; team <= kMostCluster; team *= 2) {
+      const long long block_rows = (rows + team - 1) / team;
+      const long long lane_rows = (block_rows + lanes - 1) / lanes;
+      const long long shared = lane_rows * slot + extra;
+      if (shared > kMostShared || slabs * team > 0x7FFFFFFF) continue;
+      const double here = static_cast<double>(
+          std::min<long long>(resident, 228 * 1024 / (shared + 2048)));
+      const double narrow = tiles == 1 || width * size >= 64 ? 1.0 : width * size >= 32 ? 1.3 : 2.0;
+      const double move =
+          static_cast<double>(block_rows) * width * size * (images + 1) * narrow / 43.5e3;
+      const double work = static_cast<double>(lane_rows) * (images == 1 ? 0.16 : 0.31) + 1.0;
+      const double fixed = team == 1 ? 2.0 : team <= 8 ? 3.0 : 3.5;
+      const double each = static_cast<double>(slabs * team) / processors;
+      const double waves = std::ceil(each / here);
+      const double together = std::min(here, std::ceil(each));
+      const double time =
+          waves * std::max({move * together, work * together, move + work + fixed});
+      if (time >= best) continue;
+      best = time;
+      t = ClusterPlan{team,
+                      slabs,
+                      static_cast<int>(block_rows),
+                      static_cast<unsigned int>(lane_rows * slot),
+                      static_cast<unsigned int>(entries),
+                      static_cast<unsigned int>(shared)};
+      cut_norm(s, v, batch, pixels, channels, groups, dtype, x_stride, grad_stride, cols, 0);
+      s.tiles = static_cast<int>(tiles);
+      s.tile_cols = cols;
+      s.lanes = lanes;
+    }
+  }
+  return best < 1e30;
+}
+
+// Workspace of a backward pass in clusters: the views' sums.
+inline size_t cluster_space(const NormShape& s) {
+  return sizeof(float2) * static_cast<size_t>(s.batch) * s.channels;
+}
+
+// Processors of the current device, looked up once for each.
+inline int processors() {
+  static std::atomic<int> known[64];
+  int device = 0, count = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return 148;
+  if (device < 64 && (count = known[device].load(std::memory_order_relaxed)) > 0) return count;
+  if (cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    return 148;
+  if (device < 64) known[device].store(count, std::memory_order_relaxed);
+  return count;
+}
+
+// Launches a kernel of clusters.
+template <auto Kernel, typename... Args>
+int launch_clusters(const ClusterPlan& t, cudaStream_t stream, Args... args) {
+  static std::atomic<unsigned long long> allowed;  // devices where its limits were raised
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return static_cast<int>(err);
+  const unsigned long long bit = device < 64 ? 1ull << device : 0;
+  if ((allowed.load(std::memory_order_relaxed) & bit) == 0) {
+    err = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
+    if (err == cudaSuccess)
+      err = cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (err != cudaSuccess) return static_cast<int>(err);
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned int>(t.slabs * t.size));
+  config.blockDim = dim3(kNormThreads);
+  config.dynamicSmemBytes = t.shared;
+  config.stream = stream;
+  cudaLaunchAttribute attribute = {};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = t.size;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = t.size > 1 ? 1 : 0;
+  err = cudaLaunchKernelEx(&config, Kernel, args...);
+  return err == cudaSuccess ? launch_status() : static_cast<int>(err);
+}
+
+// Views of one launch.
+inline int views_at_once(long long batch) {
+  return static_cast<int>(std::min(batch, 65535LL));
 }
 
 // The plan of a call in passes over memory. A block's start and the join of its sums cost as much
-// as 16 rows of its threads, so chunks have about 64 KB (16 rows of 256 vectors); blocks fill the
-// processors evenly, up to `resident` to each, or several times over.
+// as 16 rows of its threads, so a block has 16 rows of them (64 KB of 16-byte vectors), up to 32
+// where the blocks fill the processors many times over; blocks fill the processors evenly, up to
+// `resident` to each, or several times over. Four images of 512 x 512 x 64 bfloat16 take 91, 82 and
+// 78 us forward with 8, 16 and 32 rows, two of 128 x 128 x 256 take 83, 76 and 82 us.
 inline void plan_passes(NormShape& s, const NormVector& v, long long batch, long long pixels,
                         int channels, int groups, int dtype, long long x_stride,
-                        long long grad_stride, int images) {
-  const long long view = pixels * channels * dtype_bytes(dtype);
-  const long long part = view * views_at_once(batch, pixels, channels, dtype, images);
-  const long long processors = 148, resident = images == 1 ? 4 : 3, chunk = envv("DRX_CHUNK", 65536);
-  const long long each = (part + processors * chunk / 2) / (processors * chunk);
-  const long long blocks = each <= resident ? std::max(1LL, each) * processors
-                                            : (each + resident / 2) / resident * resident * processors;
+                        long long grad_stride, int resident, int processors) {
+  const int size = dtype_bytes(dtype);
+  const long long bytes = pixels * channels * size * views_at_once(batch);
+  const long long row = static_cast<long long>(kNormThreads) * v.vec * size;
+  const long long waves = bytes / (16 * row * resident * processors);
+  const long long chunk = (waves >= 3 ? 32 : 16) * row;
+  const long long each = (bytes + processors * chunk / 2) / (processors * chunk);
+  const long long blocks =
+      processors * (each <= resident ? std::max(1LL, each)
+                                     : (each + resident / 2) / resident * resident);
   cut_norm(s, v, batch, pixels, channels, groups, dtype, x_stride, grad_stride, kNormThreads,
-           std::max(4096LL, (part + blocks - 1) / blocks));
+           std::max(row, (bytes + blocks - 1) / blocks));
 }
 
 // Workspace: a pair of each channel for each chunk; for the backward pass also one of each view and
@@ -570,7 +814,7 @@ inline NormSpace norm_space(const NormShape& s, bool backward) {
 // The larger workspace of all the vector widths that a call may turn out to take.
 inline size_t norm_workspace_bytes(long long batch, long long pixels, int channels, int groups,
                                    int dtype, bool backward) {
-  const int widest = 16 / dtype_bytes(dtype);
+  const int widest = 16 / dtype_bytes(dtype), images = backward ? 2 : 1;
   const int fold = widest / greatest_divisor(channels, widest);
   size_t most = 0;
   for (NormVector v : {NormVector{widest, fold}, NormVector{2, 1}, NormVector{1, 1}}) {
@@ -579,9 +823,15 @@ inline size_t norm_workspace_bytes(long long batch, long long pixels, int channe
       continue;
     if (v.fold == 1 && channels % v.vec != 0) continue;
     NormShape s;
-    plan_passes(s, v, batch, pixels, channels, groups, dtype, channels, channels,
-                backward ? 2 : 1);
-    most = std::max(most, norm_space(s, backward).total);
+    ClusterPlan t;
+    if (plan_clusters(s, t, v, batch, pixels, channels, groups, dtype, channels, channels, images,
+                      kResident[backward], processors())) {
+      if (backward) most = std::max(most, cluster_space(s));
+    } else {
+      plan_passes(s, v, batch, pixels, channels, groups, dtype, channels, channels,
+                  kResident[backward], processors());
+      most = std::max(most, norm_space(s, backward).total);
+    }
   }
   return most;
 }

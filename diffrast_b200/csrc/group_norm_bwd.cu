@@ -10,15 +10,16 @@ namespace {
 constexpr int kStages = 4;  // rows of x and of the gradient that a thread has under way
 
 // Joins the threads' sums of a block's rows into those of each channel: over the rows of a warp
-// where the tile's columns divide it, then over the lines of rows that are left.
+// where the tile's columns divide it, then over the lines of rows that are left. `valid` is the
+// tile's channels (with folded pixels: the view's).
 template <int V, typename Done>
-__device__ __forceinline__ void join_block(Pairs<V>& sum, Pairs<V>& dot, const NormPlace& p,
-                                           const NormShape& s, void* shared, Done done) {
-  auto* entry = static_cast<float2*>(shared);  // [lines][tile_cols * V]
-  int lines = s.lanes, line = threadIdx.y;
-  bool write = true;
-  if (warp_holds_rows()) {
-    for (int d = blockDim.x; d < 32; d *= 2) {
+__device__ __forceinline__ void join_block(Pairs<V>& sum, Pairs<V>& dot, const TileThread& t,
+                                           const NormShape& s, int valid, float2* entry,
+                                           Done done) {
+  int lines = s.lanes, line = t.y;
+  bool write = t.y < s.lanes;
+  if (warp_holds_rows(s.tile_cols)) {
+    for (int d = s.tile_cols; d < 32; d *= 2) {
 #pragma unroll
       for (int j = 0; j < Pairs<V>::kCount; ++j) {
         float2 a, b;
@@ -30,23 +31,20 @@ __device__ __forceinline__ void join_block(Pairs<V>& sum, Pairs<V>& dot, const N
         dot.p[j] = add2(dot.p[j], b);
       }
     }
-    const int thread = threadIdx.y * blockDim.x + threadIdx.x;
     lines = kNormThreads / 32;
-    line = thread / 32;
-    write = thread % 32 < blockDim.x;
+    line = t.thread / 32;
+    write = t.thread % 32 < s.tile_cols;
   }
   const int width = s.tile_cols * V;
   __syncthreads();
   if (write) {
-    float2* to = entry + line * width + threadIdx.x * V;
+    float2* to = entry + line * width + t.x * V;
 #pragma unroll
     for (int j = 0; j < V; ++j) to[j] = make_float2(sum.get(j), dot.get(j));
   }
   __syncthreads();
   const int items = s.fold > 1 ? s.channels : width;
-  const int valid = s.fold > 1 ? items : min(width, s.cols * V - (p.col - static_cast<int>(threadIdx.x) * V));
-  for (int item = threadIdx.y * blockDim.x + threadIdx.x; item < valid;
-       item += blockDim.x * blockDim.y) {
+  for (int item = t.thread; item < valid; item += t.threads) {
     float2 total = make_float2(0.0f, 0.0f);
     for (int l = 0; l < lines * s.fold; ++l) total = add2(total, entry[l * items + item]);
     done(item, total);
@@ -56,7 +54,7 @@ __device__ __forceinline__ void join_block(Pairs<V>& sum, Pairs<V>& dot, const N
 // First pass: sums of q and q (x - m) of each channel over one chunk of rows in one tile of columns.
 // parts [batch][chunks][channels].
 template <typename T, int V, bool Silu, bool Drop>
-__global__ void __launch_bounds__(kNormThreads, 3) norm_sums_kernel(
+__global__ void __launch_bounds__(kNormThreads, Drop ? 2 : 3) norm_sums_kernel(
     const T* __restrict__ x, const T* __restrict__ grad, NormShape s, int view0,
     const float* __restrict__ table, float bound, DropKey key, float2* __restrict__ parts) {
   extern __shared__ uint4 shared[];
@@ -91,7 +89,13 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_sums_kernel(
   }
   parts += (static_cast<long long>(p.view) * s.chunks + p.chunk) * s.channels;
   if (s.fold == 1) parts += blockIdx.y * s.tile_cols * V;
-  join_block<V>(sum, dot, p, s, shared, [&](int item, float2 total) { parts[item] = total; });
+  const int tile_col = blockIdx.y * s.tile_cols;
+  const int valid = s.fold > 1 ? s.channels : min(s.tile_cols, s.cols - tile_col) * V;
+  const TileThread t = {static_cast<int>(threadIdx.x), static_cast<int>(threadIdx.y),
+                        static_cast<int>(threadIdx.y * blockDim.x + threadIdx.x),
+                        static_cast<int>(blockDim.x * blockDim.y)};
+  join_block<V>(sum, dot, t, s, valid, reinterpret_cast<float2*>(shared),
+                [&](int item, float2 total) { parts[item] = total; });
   wait_for_kernel_before();
 }
 
@@ -169,7 +173,7 @@ __global__ void __launch_bounds__(kJoinThreads) norm_means_kernel(
 // Second pass: grad x = r (q w - A - h B) over one chunk of rows in one tile of columns, from the
 // end of the views to their start (what the first pass read last is still in L2).
 template <typename T, int V, bool Silu, bool Drop>
-__global__ void __launch_bounds__(kNormThreads, 3) norm_grad_kernel(
+__global__ void __launch_bounds__(kNormThreads, Drop ? 2 : 3) norm_grad_kernel(
     const T* __restrict__ x, const T* __restrict__ grad, NormShape s, int view0,
     const float* __restrict__ affine, const float* table, float bound, DropKey key,
     T* __restrict__ grad_x) {
@@ -244,8 +248,158 @@ struct Gradients {
   bool weight_views, bias_views;
 };
 
+// The whole pass by clusters of blocks (see "clusters" in group_norm.cuh). The gradients of weight
+// and bias are written here where they are sums of one view (`direct`); otherwise the views' sums
+// are left for norm_params_kernel.
 template <typename T, int V, bool Silu, bool Drop>
-int passes(const void* x, const void* grad, const NormShape& s, int dtype, const float* affine,
+__global__ void __launch_bounds__(kNormThreads, Drop ? 2 : 3) norm_cluster_bwd_kernel(
+    const T* __restrict__ x, const T* __restrict__ grad, NormShape s, ClusterPlan t,
+    const float* __restrict__ affine, const float* __restrict__ rstd, float bound, DropKey key,
+    Gradients out, bool direct, float2* __restrict__ sums) {
+  extern __shared__ uint4 shared[];
+  auto* bytes = reinterpret_cast<unsigned char*>(shared);
+  auto* entry = reinterpret_cast<float2*>(bytes + t.slots);
+  const int width = s.tile_cols * V;
+  auto* channel = reinterpret_cast<float2*>(bytes + t.slots + t.entries);  // [width]
+  auto* constants = reinterpret_cast<float*>(channel + width);             // [2][width]
+  T* grad_x = static_cast<T*>(out.x);
+  const ClusterShare p(s, t, V);
+  SlabRows<T, V, 2> rows;
+  rows.slots = static_cast<unsigned int>(__cvta_generic_to_shared(shared)) +
+               threadIdx.x * static_cast<unsigned int>(sizeof(Packed<T, V>));
+  rows.count = p.mine;
+  rows.fetch({x + p.first * s.x_row + p.col, grad + p.first * s.grad_row + p.col},
+             {s.lanes * s.x_row, s.lanes * s.grad_row});
+  const unsigned long long seed = Drop ? load_seed(key) : 0;
+  const long long out_row = static_cast<long long>(s.channels) * s.fold;
+  const long long start = p.first * out_row + p.col, stride = s.lanes * out_row;
+  Affine<V> c;
+  Pairs<V> sum, dot;
+#pragma unroll
+  for (int j = 0; j < Pairs<V>::kCount; ++j) sum.p[j] = dot.p[j] = both(0.0f);
+  if (p.mine > 0) c.load(affine, s, p.view, p.col);
+  copy_wait<0>();
+  long long at = start;
+  rows.for_rows([&](Pairs<V> (&v)[2]) {
+    if (Drop) apply_dropout<V>(v[1], at, key, seed);
+    at += stride;
+#pragma unroll
+    for (int j = 0; j < Pairs<V>::kCount; ++j) {
+      const float2 e = add2(v[0].p[j], c.shift.p[j]);
+      const float2 z = fma2(e, c.scale.p[j], c.bias.p[j]);
+      const float2 u = activate_grad<Silu>(v[1].p[j], z, bound);
+      sum.p[j] = add2(sum.p[j], u);
+      dot.p[j] = fma2(u, e, dot.p[j]);
+    }
+  });
+  join_block<V>(sum, dot, p.at, s, p.channels, entry,
+                [&](int item, float2 total) { channel[item] = total; });
+  const int d = s.group_channels;
+  float2* joined = channel;
+  if (t.size > 1) {
+    auto cluster = cooperative_groups::this_cluster();
+    cluster.sync();
+    joined = entry;  // its readers are behind the cluster's barrier
+    for (int item = threadIdx.x; item < p.channels; item += kNormThreads) {
+      float2 v[kMostCluster];
+#pragma unroll
+      for (int r = 0; r < kMostCluster; ++r)
+        if (r < t.size) v[r] = *cluster.map_shared_rank(channel + item, r);
+      float2 total = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int r = 0; r < kMostCluster; ++r)
+        if (r < t.size) total = add2(total, v[r]);
+      joined[item] = total;
+    }
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  }
+  __syncthreads();
+  // The groups' means, and from them the channels' constants of grad x.
+  const int groups = p.channels / d;
+  const int lanes = lanes_for(groups), lane = threadIdx.x & (lanes - 1);
+  const int step = kNormThreads / lanes;
+  const float inverse = 1.0f / (static_cast<float>(s.pixels) * static_cast<float>(d));
+  const float* scales = affine + (static_cast<long long>(p.view) * 3 + 1) * s.channels + p.channel;
+  const float* rs = rstd + static_cast<long long>(p.view) * s.groups + p.channel / d;
+  for (int base = 0; base < groups; base += step) {
+    const int g = base + threadIdx.x / lanes;
+    float2 total = make_float2(0.0f, 0.0f);
+    float r = 0.0f;
+    if (g < groups) {
+      r = __ldg(rs + g);
+      for (int i = lane; i < d; i += lanes) {
+        const float2 v = joined[g * d + i];
+        const float scale = __ldg(scales + g * d + i);
+        total = add2(total, make_float2(v.x * scale, v.y * r * scale));
+      }
+    }
+    for (int e = 1; e < lanes; e *= 2) {
+      total.x += __shfl_xor_sync(0xFFFFFFFFu, total.x, e);
+      total.y += __shfl_xor_sync(0xFFFFFFFFu, total.y, e);
+    }
+    if (g < groups) {
+      for (int i = lane; i < d; i += lanes) {
+        const int item = g * d + i;
+        constants[item] = -total.x * inverse;
+        constants[width + item] = -total.y * inverse * r;
+        if (p.rank == 0) {
+          const float2 v = joined[item];
+          const long long own = static_cast<long long>(p.view) * s.channels + p.channel + item;
+          if (!direct) {
+            sums[own] = make_float2(v.x, v.y * r);
+          } else {
+            if (out.weight != nullptr) store_param(out.weight, out.weight_dtype, own, v.y * r);
+            if (out.bias != nullptr) store_param(out.bias, out.bias_dtype, own, v.x);
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (p.mine > 0 && grad_x != nullptr) {
+    const Pairs<V> base = load_constants<V>(constants, s, p);
+    const Pairs<V> slope = load_constants<V>(constants + width, s, p);
+    at = start;
+    rows.for_rows([&](Pairs<V> (&v)[2]) {
+      if (Drop) apply_dropout<V>(v[1], at, key, seed);
+#pragma unroll
+      for (int j = 0; j < Pairs<V>::kCount; ++j) {
+        const float2 e = add2(v[0].p[j], c.shift.p[j]);
+        const float2 z = fma2(e, c.scale.p[j], c.bias.p[j]);
+        const float2 u = activate_grad<Silu>(v[1].p[j], z, bound);
+        v[0].p[j] = fma2(u, c.scale.p[j], fma2(e, slope.p[j], base.p[j]));
+      }
+      __stcs(reinterpret_cast<Packed<T, V>*>(grad_x + at), pack_pairs<T, V>(v[0]));
+      at += stride;
+    });
+  }
+  // No block ends while another may still read its sums.
+  if (t.size > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+int params(const NormShape& s, const float2* sums, const Gradients& out, cudaStream_t stream,
+           bool after) {
+  if (out.weight == nullptr && out.bias == nullptr) return DR_OK;
+  return static_cast<int>(launch_kernel(
+      norm_params_kernel, blocks_for(s.channels, 32), kNormThreads, 0, stream, after, sums,
+      s.batch, s.channels, out.weight, out.weight_dtype, out.weight_views, out.bias,
+      out.bias_dtype, out.bias_views));
+}
+
+template <typename T, int V, bool Silu, bool Drop>
+int clusters(const void* x, const void* grad, const NormShape& s, const ClusterPlan& t,
+             const float* affine, const float* rstd, float bound, const DropKey& key,
+             const Gradients& out, float2* sums, cudaStream_t stream) {
+  const bool direct = s.batch == 1 || ((out.weight == nullptr || out.weight_views) &&
+                                       (out.bias == nullptr || out.bias_views));
+  const int status = launch_clusters<norm_cluster_bwd_kernel<T, V, Silu, Drop>>(
+      t, stream, static_cast<const T*>(x), static_cast<const T*>(grad), s, t, affine, rstd, bound,
+      key, out, direct, sums);
+  return status != DR_OK || direct ? status : params(s, sums, out, stream, false);
+}
+
+template <typename T, int V, bool Silu, bool Drop>
+int passes(const void* x, const void* grad, const NormShape& s, const float* affine,
            const float* rstd, float bound, const DropKey& key, const Gradients& out,
            unsigned char* workspace, cudaStream_t stream) {
   const NormSpace space = norm_space(s, true);
@@ -254,7 +408,7 @@ int passes(const void* x, const void* grad, const NormShape& s, int dtype, const
   auto* table = reinterpret_cast<float*>(workspace + space.table);
   const T* in = static_cast<const T*>(x);
   const T* dy = static_cast<const T*>(grad);
-  const int most = views_at_once(s.batch, s.pixels, s.channels, dtype, 2);
+  const int most = views_at_once(s.batch);
   const unsigned int runs = join_runs(s);
   const dim3 threads(s.tile_cols, s.lanes);
   constexpr size_t ring = RowRing<T, V, 2, kStages>::kBytes;
@@ -272,11 +426,7 @@ int passes(const void* x, const void* grad, const NormShape& s, int dtype, const
       err = launch_kernel(norm_grad_kernel<T, V, Silu, Drop>, blocks, threads, ring, stream, true,
                           in, dy, s, view0, affine, table, bound, key, static_cast<T*>(out.x));
   }
-  if (err == cudaSuccess && (out.weight != nullptr || out.bias != nullptr))
-    err = launch_kernel(norm_params_kernel, blocks_for(s.channels, 32), kNormThreads, 0, stream,
-                        true, sums, s.batch, s.channels, out.weight, out.weight_dtype,
-                        out.weight_views, out.bias, out.bias_dtype, out.bias_views);
-  return err == cudaSuccess ? launch_status() : static_cast<int>(err);
+  return err == cudaSuccess ? params(s, sums, out, stream, true) : static_cast<int>(err);
 }
 
 }  // namespace
@@ -303,11 +453,16 @@ extern "C" int dr_group_norm_bwd(const void* x, int64_t x_stride, const void* gr
     return DR_ERR_INVALID_ARGUMENT;
   if (too_large(batch, pixels)) return DR_ERR_TOO_LARGE;
   NormShape s;
+  ClusterPlan t;
   const NormVector v = choose_vector(pixels, channels, dtype, x_stride, grad_stride,
                                      {x, grad_y, grad_x});
-  plan_passes(s, v, batch, pixels, channels, groups, dtype, x_stride, grad_stride, 2);
-  if (workspace == nullptr || workspace_bytes < norm_space(s, true).total)
-    return DR_ERR_WORKSPACE_TOO_SMALL;
+  const bool small = plan_clusters(s, t, v, batch, pixels, channels, groups, dtype, x_stride,
+                                   grad_stride, 2, kResident[1], processors());
+  if (!small)
+    plan_passes(s, v, batch, pixels, channels, groups, dtype, x_stride, grad_stride, kResident[1],
+                processors());
+  const size_t need = small ? cluster_space(s) : norm_space(s, true).total;
+  if (workspace == nullptr || workspace_bytes < need) return DR_ERR_WORKSPACE_TOO_SMALL;
   const DropKey key = drop_key(seed, seed_value, layer, drop_threshold);
   const Gradients out{grad_x,      grad_weight,      grad_bias,     weight_dtype,
                       bias_dtype,  weight_batch > 1, bias_batch > 1};
@@ -315,8 +470,12 @@ extern "C" int dr_group_norm_bwd(const void* x, int64_t x_stride, const void* gr
   const float* rstd = state + static_cast<size_t>(batch) * 3 * channels;
   return with_variant(dtype, v.vec, activation, drop_threshold, [&](auto k) {
     using K = decltype(k);
+    if (small)
+      return clusters<typename K::Type, K::kVec, K::kSilu, K::kDrop>(
+          x, grad_y, s, t, state, rstd, bound, key, out, static_cast<float2*>(workspace),
+          as_stream(stream));
     return passes<typename K::Type, K::kVec, K::kSilu, K::kDrop>(
-        x, grad_y, s, dtype, state, rstd, bound, key, out,
+        x, grad_y, s, state, rstd, bound, key, out,
         static_cast<unsigned char*>(workspace), as_stream(stream));
   });
 }

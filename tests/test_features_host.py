@@ -117,14 +117,16 @@ def test_c_abi_refuses_before_any_cuda_call():
     for change in common + [dict(gy=None), dict(gy_stride=7)]:
         assert bwd(lib, **change) == bad, change
     for call in (fwd, bwd):
-        assert call(lib, ws_bytes=0) == small
-        assert call(lib, ws=None) == small
+        # An image too large for shared memory needs scratch in both directions.
+        assert call(lib, pixels=1 << 24, ws_bytes=0) == small
+        assert call(lib, pixels=1 << 24, ws=None) == small
         assert call(lib, batch=0) == 0 and call(lib, pixels=0) == 0
         assert call(lib, batch=1 << 31) == 10003 and call(lib, pixels=1 << 31) == 10003
     assert lib.dr_group_norm_workspace_bytes(2, 9, 8, 3, 0, 0) == 0
     assert lib.dr_group_norm_state_floats(2, 8, 4) == 2 * (3 * 8 + 4)
     for backward in (0, 1):
-        assert lib.dr_group_norm_workspace_bytes(2, 9, 8, 2, 0, backward) > 0
+        assert lib.dr_group_norm_workspace_bytes(2, 1 << 24, 8, 2, 0, backward) > 0
+    assert lib.dr_group_norm_workspace_bytes(2, 9, 8, 2, 0, 0) == 0
 
     def drop(x=16, res=None, count=8, dtype=0, thr=1, y=16):
         return lib.dr_dropout(x, res, count, dtype, thr, None, 0, 0, y, None)
