@@ -382,10 +382,9 @@ extern "C" int dr_group_norm_fwd(const void* x, int64_t x_stride, int32_t dtype,
   ClusterPlan t;
   const NormVector v = choose_vector(pixels, channels, dtype, x_stride, channels, {x, y});
   const bool clusters = plan_clusters(s, t, v, batch, pixels, channels, groups, dtype, x_stride,
-                                      channels, 1, kResident[0], processors());
+                                      channels, 1, processors());
   if (!clusters) {
-    plan_passes(s, v, batch, pixels, channels, groups, dtype, x_stride, channels, kResident[0],
-                processors());
+    plan_passes(s, v, batch, pixels, channels, groups, dtype, x_stride, channels, 1, processors());
     if (workspace == nullptr || workspace_bytes < norm_space(s, false).total)
       return DR_ERR_WORKSPACE_TOO_SMALL;
   }

@@ -668,11 +668,10 @@ constexpr long long kClusterBytes = 1LL << 20;
 // The plan of a call in clusters, or false where none fits: tiles of whole groups, and blocks to a
 // cluster, by the estimated time in microseconds. A block's own is what is fixed (2, or 3 with a
 // cluster), its bytes at a processor's share of the memory, and its rows' instructions; the blocks
-// of a processor overlap, `resident` by registers and fewer by shared memory.
+// of a processor overlap, as many as its registers and shared memory hold.
 inline bool plan_clusters(NormShape& s, ClusterPlan& t, const NormVector& v, long long batch,
                           long long pixels, int channels, int groups, int dtype,
-                          long long x_stride, long long grad_stride, int images, int resident,
-                          int processors) {
+                          long long x_stride, long long grad_stride, int images, int processors) {
   const int d = channels / groups, size = dtype_bytes(dtype);
   const int most_cols = kNormThreads / 2;
   const int row_cols = static_cast<int>(static_cast<long long>(channels) * v.fold / v.vec);
@@ -694,7 +693,7 @@ inline bool plan_clusters(NormShape& s, ClusterPlan& t, const NormVector& v, lon
       const long long shared = lane_rows * slot + extra;
       if (shared > kMostShared || slabs * team > 0x7FFFFFFF) continue;
       const double here = static_cast<double>(
-          std::min<long long>(resident, 228 * 1024 / (shared + 2048)));
+          std::min<long long>(kResident[images - 1], 228 * 1024 / (shared + 2048)));
       const double narrow = tiles == 1 || width * size >= 64 ? 1.0 : width * size >= 32 ? 1.3 : 2.0;
       const double move =
           static_cast<double>(block_rows) * width * size * (images + 1) * narrow / 43.5e3;
@@ -775,18 +774,19 @@ inline int views_at_once(long long batch) {
 }
 
 // The plan of a call in passes over memory. A block's start and the join of its sums cost as much
-// as 16 rows of its threads, so a block has 16 rows of them (64 KB of 16-byte vectors), up to 32
-// where the blocks fill the processors many times over; blocks fill the processors evenly, up to
-// `resident` to each, or several times over. Four images of 512 x 512 x 64 bfloat16 take 91, 82 and
-// 78 us forward with 8, 16 and 32 rows, two of 128 x 128 x 256 take 83, 76 and 82 us.
+// as 16 rows of its threads, so a block has 16 rows of them (64 KB of 16-byte vectors), in the
+// forward pass 32 where the blocks fill the processors many times over; blocks fill the processors
+// evenly, up to `resident` to each, or several times over. Four images of 512 x 512 x 64 bfloat16
+// take 91, 82 and 78 us forward with 8, 16 and 32 rows, and 116, 114 and 122 us backward; eight of
+// 128 x 128 x 256 take 83, 76 and 82 us forward.
 inline void plan_passes(NormShape& s, const NormVector& v, long long batch, long long pixels,
                         int channels, int groups, int dtype, long long x_stride,
-                        long long grad_stride, int resident, int processors) {
-  const int size = dtype_bytes(dtype);
+                        long long grad_stride, int images, int processors) {
+  const int size = dtype_bytes(dtype), resident = kResident[images - 1];
   const long long bytes = pixels * channels * size * views_at_once(batch);
   const long long row = static_cast<long long>(kNormThreads) * v.vec * size;
   const long long waves = bytes / (16 * row * resident * processors);
-  const long long chunk = (waves >= 3 ? 32 : 16) * row;
+  const long long chunk = (waves >= 3 && images == 1 ? 32 : 16) * row;
   const long long each = (bytes + processors * chunk / 2) / (processors * chunk);
   const long long blocks =
       processors * (each <= resident ? std::max(1LL, each)
@@ -825,11 +825,11 @@ inline size_t norm_workspace_bytes(long long batch, long long pixels, int channe
     NormShape s;
     ClusterPlan t;
     if (plan_clusters(s, t, v, batch, pixels, channels, groups, dtype, channels, channels, images,
-                      kResident[backward], processors())) {
+                      processors())) {
       if (backward) most = std::max(most, cluster_space(s));
     } else {
-      plan_passes(s, v, batch, pixels, channels, groups, dtype, channels, channels,
-                  kResident[backward], processors());
+      plan_passes(s, v, batch, pixels, channels, groups, dtype, channels, channels, images,
+                  processors());
       most = std::max(most, norm_space(s, backward).total);
     }
   }

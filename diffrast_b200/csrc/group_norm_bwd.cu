@@ -457,9 +457,9 @@ extern "C" int dr_group_norm_bwd(const void* x, int64_t x_stride, const void* gr
   const NormVector v = choose_vector(pixels, channels, dtype, x_stride, grad_stride,
                                      {x, grad_y, grad_x});
   const bool small = plan_clusters(s, t, v, batch, pixels, channels, groups, dtype, x_stride,
-                                   grad_stride, 2, kResident[1], processors());
+                                   grad_stride, 2, processors());
   if (!small)
-    plan_passes(s, v, batch, pixels, channels, groups, dtype, x_stride, grad_stride, kResident[1],
+    plan_passes(s, v, batch, pixels, channels, groups, dtype, x_stride, grad_stride, 2,
                 processors());
   const size_t need = small ? cluster_space(s) : norm_space(s, true).total;
   if (workspace == nullptr || workspace_bytes < need) return DR_ERR_WORKSPACE_TOO_SMALL;

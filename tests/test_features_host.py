@@ -134,5 +134,5 @@ def test_c_abi_refuses_before_any_cuda_call():
     for change in (dict(count=-1), dict(dtype=3), dict(thr=-1), dict(thr=65536), dict(x=None),
                    dict(y=None)):
         assert drop(**change) == bad, change
-    assert drop(count=1 << 43) == 10003
+    assert drop(count=1 << 44) == 10003
     assert drop(count=0) == 0
