@@ -34,11 +34,14 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(
 #pragma unroll
   for (int n = 0; n < kCounters; ++n) {
     const long long first = base + n * kThreads * 8;
-    if (!Wide || first + 8 > count) continue;
+    if constexpr (Wide) {
+      if (first + 8 <= count) {
 #pragma unroll
-    for (int k = 0; k < kWords; ++k) {
-      a[n][k] = __ldcs(reinterpret_cast<const uint4*>(x + first) + k);
-      if (Residual) b[n][k] = __ldcs(reinterpret_cast<const uint4*>(residual + first) + k);
+        for (int k = 0; k < kWords; ++k) {
+          a[n][k] = __ldcs(reinterpret_cast<const uint4*>(x + first) + k);
+          if (Residual) b[n][k] = __ldcs(reinterpret_cast<const uint4*>(residual + first) + k);
+        }
+      }
     }
   }
 #pragma unroll

@@ -98,22 +98,27 @@ __device__ __forceinline__ void store_param(void* data, int dtype, long long i, 
 // at 2^63, so that the product stays finite: below z = -43.7 the result is 2^-63 instead of less.
 // Exponential and reciprocal are within two units in the last place of float32. A NaN gives 2^-63
 // (the cut drops it), and its product with z is NaN again.
-__device__ __forceinline__ float2 sigmoid2(float2 z) {
+__device__ __forceinline__ float2 exponentials(float2 z) {
   const float2 t = mul2(z, both(-1.4426950408889634f));
   float2 e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(fminf(t.x, 63.0f)));
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(fminf(t.y, 63.0f)));
-  e = add2(e, both(1.0f));
+  return add2(e, both(1.0f));
+}
+
+// q / (1 + exp(-z)).
+__device__ __forceinline__ float2 times_sigmoid(float2 q, float2 z) {
+  const float2 e = exponentials(z);
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e.x * e.y));
-  return mul2(both(r), make_float2(e.y, e.x));
+  return mul2(make_float2(q.x * e.y, q.y * e.x), both(r));
 }
 
 // The activations: SiLU, or a clamp from below that is the identity with bound -infinity and ReLU
 // with bound 0. The comparisons are written so that NaN passes, as it does through both.
 template <bool Silu>
 __device__ __forceinline__ float2 activate(float2 z, float bound) {
-  if (Silu) return mul2(z, sigmoid2(z));
+  if (Silu) return times_sigmoid(z, z);
   return make_float2(z.x <= bound ? bound : z.x, z.y <= bound ? bound : z.y);
 }
 
@@ -121,7 +126,7 @@ __device__ __forceinline__ float2 activate(float2 z, float bound) {
 template <bool Silu>
 __device__ __forceinline__ float2 activate_grad(float2 q, float2 z, float bound) {
   if (Silu) {
-    const float2 s = sigmoid2(z);
+    const float2 s = times_sigmoid(both(1.0f), z);
     const float2 t = fma2(make_float2(-s.x, -s.y), z, z);
     return mul2(q, fma2(s, t, s));
   }
@@ -337,18 +342,33 @@ struct RowRing {
     return load_pairs<T, V>(load_slot<P>(slots + (u * Images + k) * kSlot));
   }
 
-  // Calls use(vectors) for the rows in order.
+  template <typename Use>
+  __device__ __forceinline__ void row(int u, Use use) const {
+    copy_wait<Stages - 1>();
+    Pairs<V> v[Images];
+#pragma unroll
+    for (int k = 0; k < Images; ++k) v[k] = load(u, k);
+    use(v);
+  }
+
+  // Calls use(vectors) for the rows in order. While two rounds of the ring are left, nothing is
+  // tested.
   template <typename Use>
   __device__ __forceinline__ void for_rows(Use use) {
-    for (int left = count; left > 0; left -= Stages) {
+    int left = count;
+    for (; left >= 2 * Stages; left -= Stages) {
 #pragma unroll
       for (int u = 0; u < Stages; ++u) {
-        if (u > 0 && u >= left) break;
-        copy_wait<Stages - 1>();
-        Pairs<V> v[Images];
+        row(u, use);
+        fetch(u);
+        copy_commit();
+      }
+    }
+    for (; left > 0; left -= Stages) {
 #pragma unroll
-        for (int k = 0; k < Images; ++k) v[k] = load(u, k);
-        use(v);
+      for (int u = 0; u < Stages; ++u) {
+        if (u >= left) break;
+        row(u, use);
         if (u + Stages < left) fetch(u);
         copy_commit();
       }
