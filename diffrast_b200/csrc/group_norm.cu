@@ -100,8 +100,14 @@ __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(
   __shared__ Moment channel[32];
   __shared__ float2 result;  // of a group wider than 32 channels
   let_next_kernel_start();
-  wait_for_kernel_before();
   const JoinPlace p(s, view0);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  float scale = 1.0f, offset = 0.0f;  // weight and bias of channel `lane`, before the wait
+  if (warp == 0 && lane < p.channels) {
+    scale = load_scale(weight, p.view, p.channel + lane);
+    offset = load_shift(bias, p.view, p.channel + lane);
+  }
+  wait_for_kernel_before();
   const int d = s.group_channels;
   parts += static_cast<long long>(p.view) * s.chunks * s.channels + p.channel;
   table += static_cast<long long>(p.view) * 3 * s.channels + p.channel;
@@ -110,12 +116,11 @@ __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(
   const float last_count =
       static_cast<float>(s.rows - static_cast<long long>(s.chunks - 1) * s.chunk_rows) *
       static_cast<float>(s.fold);
-  auto write = [&](int c, float mean, float r) {
+  auto write = [&](int c, float mean, float rs, float b) {
     table[c] = -mean;
-    table[s.channels + c] = r * load_scale(weight, p.view, p.channel + c);
-    table[2 * s.channels + c] = load_shift(bias, p.view, p.channel + c);
+    table[s.channels + c] = rs;
+    table[2 * s.channels + c] = b;
   };
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   Moment wide = {0.0f, 0.0f, 0.0f};
   for (int base = 0; base < p.channels; base += p.width) {
     // This lane's chunks of channel x.
@@ -158,7 +163,7 @@ __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(
         for (int i = 1; i < d; ++i) group.join(channel[g * d + i]);
         const float r = rstd_of(group, eps);
         if (lane == g * d) rstd[g] = r;
-        write(lane, group.mean, r);
+        write(lane, group.mean, r * scale, offset);
       }
     }
     __syncthreads();
@@ -169,7 +174,9 @@ __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(
     rstd[0] = result.y;
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < p.channels; c += kJoinThreads) write(c, result.x, result.y);
+  for (int c = threadIdx.x; c < p.channels; c += kJoinThreads)
+    write(c, result.x, result.y * load_scale(weight, p.view, p.channel + c),
+          load_shift(bias, p.view, p.channel + c));
 }
 
 // Second pass: normalise, scale, activate and drop one chunk of rows in one tile of columns. Blocks
