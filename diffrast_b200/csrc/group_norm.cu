@@ -9,11 +9,11 @@ constexpr int kStages = 8;  // rows that a thread has under way
 
 // Joins the threads' moments of a block's rows into those of each channel: over the rows of a warp
 // where the tile's columns divide it, then over the lines of rows that are left. `n` is the
-// thread's count, `valid` the tile's channels (with folded pixels: the view's). `done` gets the
-// channel, counted from the tile's first, and (mean, squared deviations), zeros without any rows.
+// thread's count, `valid` the tile's channels (with folded pixels: the view's), `turn` the elements
+// before the view's rows. `done` gets the channel, counted from the tile's first, and its moment.
 template <int V, typename Done>
 __device__ __forceinline__ void join_block(Moments<V>& m, float n, const TileThread& t,
-                                           const NormShape& s, int valid, float2* entry,
+                                           const NormShape& s, int valid, int turn, float2* entry,
                                            Done done) {
   __shared__ float counts[kNormThreads];  // of the lines
   m.finish(n);
@@ -34,28 +34,32 @@ __device__ __forceinline__ void join_block(Moments<V>& m, float n, const TileThr
     if (t.x == 0) counts[line] = n;
   }
   __syncthreads();
-  const int items = s.fold > 1 ? s.channels : width;
-  for (int item = t.thread; item < valid; item += t.threads) {
-    const float2 first = entry[item];
-    float total_n = 0.0f, total = 0.0f;
-    for (int l = 0; l < lines; ++l) {
-      const float c = counts[l];
-      for (int f = 0; f < s.fold; ++f) {
-        total_n += c;
-        total = fmaf(c, entry[l * width + f * items + item].x - first.x, total);
-      }
+  // Channel by channel. With more than 16 parts to a channel and threads to spare, several threads
+  // take some of its parts each, and one of them joins what they have.
+  const int items = s.fold > 1 ? s.channels : width, parts = lines * s.fold;
+  const int sharers = parts > 16 ? max(1, min(parts / 4, t.threads / valid)) : 1;
+  auto join_parts = [&](int item, int first_part) {
+    // Channel `item` is `lead` columns on in turned rows.
+    const int at = item < turn ? item - turn + s.channels : item - turn;
+    Moment c = {0.0f, 0.0f, 0.0f};
+    for (int i = first_part; i < parts; i += sharers) {
+      const float2 v = entry[i * items + at];
+      c.join({counts[s.fold > 1 ? i / s.fold : i], v.x, v.y});
     }
-    const float offset = total_n > 0.0f ? __fdividef(total, total_n) : 0.0f;
-    float squares = 0.0f;
-    for (int l = 0; l < lines; ++l) {
-      const float c = counts[l];
-      for (int f = 0; f < s.fold; ++f) {
-        const float2 v = entry[l * width + f * items + item];
-        const float d = v.x - first.x - offset;
-        squares += fmaf(c * d, d, v.y);
-      }
-    }
-    done(item, make_float2(first.x + offset, squares));
+    return c;
+  };
+  if (sharers == 1) {
+    for (int item = t.thread; item < valid; item += t.threads) done(item, join_parts(item, 0));
+    return;
+  }
+  __shared__ Moment shares[kNormThreads];
+  const int item = t.thread / sharers;
+  if (item < valid) shares[t.thread] = join_parts(item, t.thread - item * sharers);
+  __syncthreads();
+  if (t.thread < valid) {
+    Moment c = shares[t.thread * sharers];
+    for (int i = 1; i < sharers; ++i) c.join(shares[t.thread * sharers + i]);
+    done(t.thread, c);
   }
 }
 
@@ -69,7 +73,7 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_stats_kernel(const T* __
   let_next_kernel_start();
   const NormPlace p(s, V, view0 + blockIdx.z, blockIdx.y, blockIdx.x);
   RowRing<T, V, 1, kStages> ring;
-  ring.image(0, x, s.x_row, p, s.lanes);
+  ring.image(0, x, s.x_view, s.x_row, p, s.lanes);
   ring.start(shared, p.count);
   Moments<V> m;
   m.clear();
@@ -86,21 +90,39 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_stats_kernel(const T* __
   const TileThread t = {static_cast<int>(threadIdx.x), static_cast<int>(threadIdx.y),
                         static_cast<int>(threadIdx.y * blockDim.x + threadIdx.x),
                         static_cast<int>(blockDim.x * blockDim.y)};
-  join_block<V>(m, static_cast<float>(p.count), t, s, valid, reinterpret_cast<float2*>(shared),
-                [&](int item, float2 moment) { parts[item] = moment; });
+  const bool more = p.takes_leftovers(s, blockIdx.y);
+  join_block<V>(m, static_cast<float>(p.count), t, s, valid, p.lead % s.channels,
+                reinterpret_cast<float2*>(shared), [&](int item, Moment c) {
+    if (more)
+      s.for_leftovers(p.lead, item, [&](long long e) {
+        c.join({1.0f, to_float(x[p.view * s.out_view + e]), 0.0f});
+      });
+    parts[item] = make_float2(c.mean, c.squares);
+  });
   wait_for_kernel_before();
 }
 
-// Joins the parts of a view's channels and the channels of its groups, and leaves the constants of
-// the second pass: table [batch][3][channels] of -mean, rstd * weight and bias.
+// The constants of the second pass that a group's moment leaves: table [batch][3][channels] of
+// -mean, rstd * weight and bias.
+__device__ __forceinline__ void write_constants(float* table, const NormShape& s, int view,
+                                                int channel, float mean, float scale,
+                                                float offset) {
+  table += static_cast<long long>(view) * 3 * s.channels + channel;
+  table[0] = -mean;
+  table[s.channels] = scale;
+  table[2 * s.channels] = offset;
+}
+
+// Joins the parts of a view's channels, and the channels of its groups where a block has them all;
+// otherwise leaves (mean, squares) of the channels for norm_group_kernel.
 __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(
     const float2* parts, NormShape s, int view0, NormParam weight, NormParam bias, float eps,
-    float* __restrict__ rstd, float* __restrict__ table) {
+    float* __restrict__ rstd, float* __restrict__ table, float2* __restrict__ channels) {
   __shared__ float2 entry[kJoinThreads + kJoinThreads / 8];
-  __shared__ Moment channel[32];
-  __shared__ float2 result;  // of a group wider than 32 channels
+  __shared__ Moment channel[kJoinChannels];
   let_next_kernel_start();
   const JoinPlace p(s, view0);
+  const int d = s.group_channels;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   float scale = 1.0f, offset = 0.0f;  // weight and bias of channel `lane`, before the wait
   if (warp == 0 && lane < p.channels) {
@@ -108,75 +130,81 @@ __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(
     offset = load_shift(bias, p.view, p.channel + lane);
   }
   wait_for_kernel_before();
-  const int d = s.group_channels;
   parts += static_cast<long long>(p.view) * s.chunks * s.channels + p.channel;
-  table += static_cast<long long>(p.view) * 3 * s.channels + p.channel;
-  rstd += static_cast<long long>(p.view) * s.groups + p.group;
-  const float chunk_count = static_cast<float>(s.chunk_rows) * static_cast<float>(s.fold);
+  const float fold = static_cast<float>(s.fold);
+  const float chunk_count = static_cast<float>(s.chunk_rows) * fold;
   const float last_count =
-      static_cast<float>(s.rows - static_cast<long long>(s.chunks - 1) * s.chunk_rows) *
-      static_cast<float>(s.fold);
-  auto write = [&](int c, float mean, float rs, float b) {
-    table[c] = -mean;
-    table[s.channels + c] = rs;
-    table[2 * s.channels + c] = b;
+      static_cast<float>(s.rows - static_cast<long long>(s.chunks - 1) * s.chunk_rows) * fold;
+  auto count_of = [&](int chunk) {
+    return (chunk + 1 < s.chunks ? chunk_count : last_count) +
+           (chunk == 0 ? static_cast<float>(s.leftover) : 0.0f);
   };
-  Moment wide = {0.0f, 0.0f, 0.0f};
-  for (int base = 0; base < p.channels; base += p.width) {
-    // This lane's chunks of channel x.
-    Moment m = {0.0f, 0.0f, 0.0f};
-    if (base + p.x < p.channels) {
+  // This lane's chunks of channel x.
+  Moment m = {0.0f, 0.0f, 0.0f};
+  if (p.x < p.channels) {
 #pragma unroll 8
-      for (int i = p.y; i < s.chunks; i += p.lanes) {
-        const float2 v = parts[static_cast<long long>(i) * s.channels + base + p.x];
-        m.join({i + 1 < s.chunks ? chunk_count : last_count, v.x, v.y});
-      }
+    for (int i = p.y; i < s.chunks; i += p.lanes) {
+      const float2 v = parts[static_cast<long long>(i) * s.channels + p.x];
+      m.join({count_of(i), v.x, v.y});
     }
-    entry[p.y * (p.width + 1) + p.x] = make_float2(m.mean, m.squares);
-    __syncthreads();
-    // Channel `warp`, from its lanes; lane i has ceil((chunks - i) / lanes) chunks.
-    if (warp < p.width) {
-      m = {0.0f, 0.0f, 0.0f};
-      for (int i = lane; i < p.lanes; i += 32) {
-        const float2 v = entry[i * (p.width + 1) + warp];
-        const int chunks = i < s.chunks ? (s.chunks - i + p.lanes - 1) / p.lanes : 0;
-        const bool last = chunks > 0 && (s.chunks - 1) % p.lanes == i;
-        m.join({chunk_count * static_cast<float>(chunks - (last ? 1 : 0)) +
-                    (last ? last_count : 0.0f),
-                v.x, v.y});
-      }
-      m.join_warp();
-      if (lane == 0) channel[warp] = base + warp < p.channels ? m : Moment{0.0f, 0.0f, 0.0f};
-    }
-    __syncthreads();
-    if (warp == 0) {
-      if (d > 32) {
-        m = channel[lane];
-        m.join_warp();
-        if (base == 0)
-          wide = m;
-        else
-          wide.join(m);
-      } else if (lane < p.channels) {
-        const int g = lane / d;
-        Moment group = channel[g * d];
-        for (int i = 1; i < d; ++i) group.join(channel[g * d + i]);
-        const float r = rstd_of(group, eps);
-        if (lane == g * d) rstd[g] = r;
-        write(lane, group.mean, r * scale, offset);
-      }
-    }
-    __syncthreads();
   }
-  if (d <= 32) return;
-  if (threadIdx.x == 0) {
-    result = make_float2(wide.mean, rstd_of(wide, eps));
-    rstd[0] = result.y;
+  entry[p.y * (p.width + 1) + p.x] = make_float2(m.mean, m.squares);
+  __syncthreads();
+  // Channel `warp`, from its lanes; lane i has ceil((chunks - i) / lanes) chunks.
+  if (warp < p.width) {
+    m = {0.0f, 0.0f, 0.0f};
+    for (int i = lane; i < p.lanes; i += 32) {
+      const float2 v = entry[i * (p.width + 1) + warp];
+      const int own = i < s.chunks ? (s.chunks - i + p.lanes - 1) / p.lanes : 0;
+      const bool last = own > 0 && (s.chunks - 1) % p.lanes == i;
+      float n = chunk_count * static_cast<float>(own - (last ? 1 : 0)) + (last ? last_count : 0.0f);
+      if (i == 0) n += static_cast<float>(s.leftover);
+      m.join({n, v.x, v.y});
+    }
+    m.join_warp();
+    if (lane == 0 && warp < p.channels) channel[warp] = m;
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < p.channels; c += kJoinThreads)
-    write(c, result.x, result.y * load_scale(weight, p.view, p.channel + c),
-          load_shift(bias, p.view, p.channel + c));
+  if (warp != 0 || lane >= p.channels) return;
+  if (d > kJoinChannels) {
+    const Moment c = channel[lane];
+    channels[static_cast<long long>(p.view) * s.channels + p.channel + lane] =
+        make_float2(c.mean, c.squares);
+    return;
+  }
+  const int g = lane / d;
+  Moment group = channel[g * d];
+  for (int i = 1; i < d; ++i) group.join(channel[g * d + i]);
+  const float r = rstd_of(group, eps);
+  if (lane == g * d) rstd[static_cast<long long>(p.view) * s.groups + p.channel / d + g] = r;
+  write_constants(table, s, p.view, p.channel + lane, group.mean, r * scale, offset);
+}
+
+// Joins the channels of one group of a view (groups wider than a block of norm_join_kernel).
+__global__ void __launch_bounds__(kNormThreads) norm_group_kernel(
+    const float2* channels, NormShape s, int view0, NormParam weight, NormParam bias, float eps,
+    float* __restrict__ rstd, float* __restrict__ table) {
+  __shared__ Moment warps[kNormThreads / 32];
+  let_next_kernel_start();
+  wait_for_kernel_before();
+  const int view = view0 + blockIdx.y, first = blockIdx.x * s.group_channels;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const float pixels = static_cast<float>(s.pixels);
+  Moment m = {0.0f, 0.0f, 0.0f};
+  for (int i = threadIdx.x; i < s.group_channels; i += kNormThreads) {
+    const float2 v = channels[static_cast<long long>(view) * s.channels + first + i];
+    m.join({pixels, v.x, v.y});
+  }
+  m.join_warp();
+  if (lane == 0) warps[warp] = m;
+  __syncthreads();
+  m = warps[0];
+  for (int i = 1; i < kNormThreads / 32; ++i) m.join(warps[i]);
+  const float r = rstd_of(m, eps);
+  if (threadIdx.x == 0) rstd[static_cast<long long>(view) * s.groups + blockIdx.x] = r;
+  for (int i = threadIdx.x; i < s.group_channels; i += kNormThreads)
+    write_constants(table, s, view, first + i, m.mean, r * load_scale(weight, view, first + i),
+                    load_shift(bias, view, first + i));
 }
 
 // Second pass: normalise, scale, activate and drop one chunk of rows in one tile of columns. Blocks
@@ -190,16 +218,28 @@ __global__ void __launch_bounds__(kNormThreads, Drop ? 3 : 4) norm_apply_kernel(
   const NormPlace p(s, V, view0 + gridDim.z - 1 - blockIdx.z, gridDim.y - 1 - blockIdx.y,
                     gridDim.x - 1 - blockIdx.x);
   RowRing<T, V, 1, kStages> ring;
-  ring.image(0, x, s.x_row, p, s.lanes);
+  ring.image(0, x, s.x_view, s.x_row, p, s.lanes);
   ring.start(shared, p.count);
   wait_for_kernel_before();
+  const unsigned long long seed = Drop ? load_seed(key) : 0;
+  if (p.takes_leftovers(s, gridDim.y - 1 - blockIdx.y)) {
+    const float* row = table + static_cast<long long>(p.view) * 3 * s.channels;
+    for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < s.channels;
+         c += blockDim.x * blockDim.y)
+      s.for_leftovers(p.lead, c, [&](long long e) {
+        const long long at = p.view * s.out_view + e;
+        const float z = fmaf(to_float(x[at]) + row[c], row[s.channels + c], row[2 * s.channels + c]);
+        Pairs<1> v;
+        v.p[0] = activate<Silu>(make_float2(z, 0.0f), bound);
+        if (Drop) apply_dropout<1>(v, at, key, seed);
+        y[at] = from_float<T>(v.p[0].x);
+      });
+  }
   if (p.count == 0) return;
   Affine<V> c;
-  c.load(table, s, p.view, p.col);
-  const unsigned long long seed = Drop ? load_seed(key) : 0;
-  const long long out_row = static_cast<long long>(s.channels) * s.fold;
-  long long at = p.first * out_row + p.col;
-  const long long step = s.lanes * out_row;
+  c.load(table, s, p.view, p.col + p.lead);
+  long long at = p.at(s.out_view, s.out_row);
+  const long long step = s.lanes * s.out_row;
   ring.for_rows([&](const Pairs<V> (&v)[1]) {
     Pairs<V> z;
 #pragma unroll
@@ -229,7 +269,7 @@ __global__ void __launch_bounds__(kNormThreads, Drop ? 3 : 4) norm_cluster_kerne
   rows.slots = static_cast<unsigned int>(__cvta_generic_to_shared(shared)) +
                threadIdx.x * static_cast<unsigned int>(sizeof(Packed<T, V>));
   rows.count = p.mine;
-  rows.fetch({x + p.first * s.x_row + p.col}, {s.lanes * s.x_row});
+  rows.fetch({x + p.in(s.x_view, s.x_row)}, {s.lanes * s.x_row});
   // Weight and bias, while the rows are on their way.
   for (int item = threadIdx.x; item < p.channels; item += kNormThreads) {
     constants[width + item] = load_scale(weight, p.view, p.channel + item);
@@ -244,8 +284,8 @@ __global__ void __launch_bounds__(kNormThreads, Drop ? 3 : 4) norm_cluster_kerne
     first = false;
     m.add(v[0]);
   });
-  join_block<V>(m, static_cast<float>(p.mine), p.at, s, p.channels, entry,
-                [&](int item, float2 moment) { channel[item] = moment; });
+  join_block<V>(m, static_cast<float>(p.mine), p.at, s, p.channels, 0, entry,
+                [&](int item, const Moment& c) { channel[item] = make_float2(c.mean, c.squares); });
   const int d = s.group_channels;
   float2* joined = channel;
   if (t.size > 1) {
@@ -307,9 +347,8 @@ __global__ void __launch_bounds__(kNormThreads, Drop ? 3 : 4) norm_cluster_kerne
     const Pairs<V> scale = load_constants<V>(constants + width, s, p);
     const Pairs<V> offset = load_constants<V>(constants + 2 * width, s, p);
     const unsigned long long seed = Drop ? load_seed(key) : 0;
-    const long long out_row = static_cast<long long>(s.channels) * s.fold;
-    long long at = p.first * out_row + p.col;
-    const long long stride = s.lanes * out_row;
+    long long at = p.in(s.out_view, s.out_row);
+    const long long stride = s.lanes * s.out_row;
     rows.for_rows([&](const Pairs<V> (&v)[1]) {
       Pairs<V> z;
 #pragma unroll
@@ -327,7 +366,10 @@ __global__ void __launch_bounds__(kNormThreads, Drop ? 3 : 4) norm_cluster_kerne
 template <typename T, int V, bool Silu, bool Drop>
 int passes(const void* x, const NormShape& s, const NormParam& weight, const NormParam& bias,
            float eps, float bound, const DropKey& key, void* y, float* table,
-           float* rstd, float2* parts, cudaStream_t stream) {
+           float* rstd, unsigned char* workspace, cudaStream_t stream) {
+  const NormSpace space = norm_space(s, false);
+  auto* parts = reinterpret_cast<float2*>(workspace + space.parts);
+  auto* channels = reinterpret_cast<float2*>(workspace + space.sums);
   const T* in = static_cast<const T*>(x);
   T* out = static_cast<T*>(y);
   const int most = views_at_once(s.batch);
@@ -343,7 +385,10 @@ int passes(const void* x, const NormShape& s, const NormParam& weight, const Nor
                         view0, parts);
     if (err == cudaSuccess)
       err = launch_kernel(norm_join_kernel, dim3(runs, views), kJoinThreads, 0, stream, true,
-                          parts, s, view0, weight, bias, eps, rstd, table);
+                          parts, s, view0, weight, bias, eps, rstd, table, channels);
+    if (err == cudaSuccess && s.group_channels > kJoinChannels)
+      err = launch_kernel(norm_group_kernel, dim3(s.groups, views), kNormThreads, 0, stream, true,
+                          channels, s, view0, weight, bias, eps, rstd, table);
     if (err == cudaSuccess)
       err = launch_kernel(norm_apply_kernel<T, V, Silu, Drop>, blocks, threads, ring, stream, true,
                           in, s, view0, table, bound, key, out);
@@ -387,10 +432,11 @@ extern "C" int dr_group_norm_fwd(const void* x, int64_t x_stride, int32_t dtype,
   if (too_large(batch, pixels)) return DR_ERR_TOO_LARGE;
   NormShape s;
   ClusterPlan t;
-  const NormVector v = choose_vector(pixels, channels, dtype, x_stride, channels, {x, y});
+  NormVector v = choose_vector(pixels, channels, dtype, x_stride, channels, {x, y}, false);
   const bool clusters = plan_clusters(s, t, v, batch, pixels, channels, groups, dtype, x_stride,
                                       channels, 1, processors());
   if (!clusters) {
+    v = choose_vector(pixels, channels, dtype, x_stride, channels, {x, y}, true);
     plan_passes(s, v, batch, pixels, channels, groups, dtype, x_stride, channels, 1, processors());
     if (workspace == nullptr || workspace_bytes < norm_space(s, false).total)
       return DR_ERR_WORKSPACE_TOO_SMALL;
@@ -412,7 +458,7 @@ extern "C" int dr_group_norm_fwd(const void* x, int64_t x_stride, int32_t dtype,
           t, as_stream(stream), static_cast<const T*>(x), s, t, w, b, eps, bound, key,
           static_cast<T*>(y), state, rstd);
     return passes<T, K::kVec, K::kSilu, K::kDrop>(
-        x, s, w, b, eps, bound, key, y, state, rstd, static_cast<float2*>(workspace),
+        x, s, w, b, eps, bound, key, y, state, rstd, static_cast<unsigned char*>(workspace),
         as_stream(stream));
   });
 }

@@ -12,6 +12,9 @@
 // A view is a matrix of pixels by channels whose rows are read in vectors of V values. Where the
 // channels do not fill whole 16-byte vectors but the rows follow one another without gaps, `fold`
 // pixels are taken as one row of fold * channels (7 channels of float32: 4 pixels are 7 vectors).
+// Where the pixels are no multiple of that, or views do not start on 16 bytes, the rows start at
+// the view's first whole vector (`lead` elements in), which turns their channels by as many, and
+// the elements before and after the rows are left over for one block of the view, one by one.
 // A block's threads are `lanes` rows by the vectors of a tile of columns (threadIdx.y and .x), so
 // that a thread keeps its channels, and their constants in registers, for all its rows. Blocks sum
 // over channels, whatever their groups, so tiles may cut groups; a small kernel between the two
@@ -48,6 +51,8 @@ struct NormShape {
   long long pixels;
   int channels, groups, group_channels;
   int fold;
+  int turned;        // rows start at the view's first whole vector: V, or 0
+  int leftover;      // values of each channel outside the rows
   int cols;          // vectors in a row
   int tile_cols;     // vectors in a tile of columns (the last tile may have fewer)
   int tiles;         // of a row
@@ -55,8 +60,24 @@ struct NormShape {
   int chunk_rows;    // rows of one block's work
   int lane_rows;     // of those, rows of each lane
   int chunks;        // of a view
-  // Elements between the rows of x and of the output's gradient.
-  long long x_row, grad_row;
+  // Elements between the rows, and between the views, of x and of the output's gradient (those of
+  // the contiguous results are out_row and out_view).
+  long long x_row, grad_row, out_row;
+  long long x_view, grad_view, out_view;
+
+  // Elements of a view before its rows.
+  __device__ __forceinline__ int lead(int view) const {
+    return turned == 0 ? 0 : static_cast<int>(-(view * out_view) & (turned - 1));
+  }
+  // The elements left over in a channel of a view with `lead` elements before its rows.
+  template <typename Use>
+  __device__ __forceinline__ void for_leftovers(int lead, int channel, Use use) const {
+    for (int e = channel; e < lead; e += channels) use(static_cast<long long>(e));
+    const long long end = lead + rows * out_row;
+    const int turn = static_cast<int>(end % channels);
+    long long e = end + (channel < turn ? channel - turn + channels : channel - turn);
+    for (; e < out_view; e += channels) use(e);
+  }
 };
 
 // Weight or bias. `data` is an address that may be read even where the parameter is absent (the
@@ -241,8 +262,9 @@ __host__ __device__ inline bool warp_holds_rows(int tile_cols) {
 struct NormPlace {
   int view, chunk, rows;
   int col;             // first element of this thread's vector in a row
+  int lead;            // elements before the view's rows
   int count;           // rows of this thread
-  long long first;     // its first row, counted over the views
+  long long row;       // its first row
 
   __device__ __forceinline__ NormPlace(const NormShape& s, int vec, int v, int tile, int c)
       : view(v), chunk(c) {
@@ -251,13 +273,23 @@ struct NormPlace {
     const int x = tile * s.tile_cols + threadIdx.x;
     const int y = threadIdx.y;
     col = x * vec;
+    lead = s.lead(v);
     count = 0;
     if (x < s.cols && y < rows)
       count = rows == s.chunk_rows
                   ? s.lane_rows
                   : static_cast<int>(static_cast<unsigned int>(rows - y + s.lanes - 1) /
                                      static_cast<unsigned int>(s.lanes));
-    first = v * s.rows + row0 + y;
+    row = row0 + y;
+  }
+
+  // Where this thread's first vector is in an image.
+  __device__ __forceinline__ long long at(long long view_size, long long row_size) const {
+    return view * view_size + lead + row * row_size + col;
+  }
+  // The view's first row of chunks and tiles, which takes what is left over.
+  __device__ __forceinline__ bool takes_leftovers(const NormShape& s, int tile) const {
+    return s.leftover > 0 && chunk == 0 && tile == 0;
   }
 };
 
@@ -291,6 +323,8 @@ __device__ __forceinline__ P load_slot(unsigned int at) {
                  : "=r"(p.x), "=r"(p.y), "=r"(p.z), "=r"(p.w)
                  : "r"(at)
                  : "memory");
+  else if constexpr (sizeof(P) == 8)
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(p.x), "=r"(p.y) : "r"(at) : "memory");
   else if constexpr (sizeof(P) == 4)
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(p) : "r"(at) : "memory");
   else
@@ -313,9 +347,9 @@ struct RowRing {
   unsigned int slots;
   int count;
 
-  __device__ __forceinline__ void image(int k, const T* base, long long row, const NormPlace& p,
-                                        int lanes) {
-    at[k] = base + p.first * row + p.col;
+  __device__ __forceinline__ void image(int k, const T* base, long long view, long long row,
+                                        const NormPlace& p, int lanes) {
+    at[k] = base + p.at(view, row);
     stride[k] = lanes * row;
   }
 
@@ -377,7 +411,8 @@ struct RowRing {
 };
 
 // The constants of a thread's channels out of a table of one row of `channels` floats: those of
-// the columns from `col` on, the channels repeated for each folded pixel.
+// the columns from `col` on (`lead` further where rows are turned), the channels repeated for each
+// folded pixel.
 template <int V>
 __device__ __forceinline__ Pairs<V> load_row(const float* row, const NormShape& s, int col) {
   Pairs<V> r;
@@ -416,26 +451,28 @@ struct Affine {
 };
 
 // The kernels that join the blocks' sums: a block has a run of whole groups of at most 8 channels
-// together, or one group, of which it takes 8, 16 or 32 channels at a time (`width`) by as many
-// lanes as it has threads for. With 32 channels to every block, two blocks read all the parts of 64
-// channels, in 10 us; they are the only work between the two passes.
+// together, or one group of at most 32, by as many lanes as it has threads for (with 32 channels to
+// every block, two blocks read all the parts of 64 channels, in 10 us; they are the only work
+// between the two passes). Of wider groups it has 32 channels, and a second kernel joins the
+// channels of each group (one block for a group of 256 channels took 45 us).
 constexpr int kJoinThreads = 1024;
+constexpr int kJoinChannels = 32;
 
-__host__ __device__ inline int join_run(int group_channels) {
-  return group_channels > 8 ? 1 : 8 / group_channels;
+__host__ __device__ inline int join_channels(int group_channels) {
+  if (group_channels > kJoinChannels) return kJoinChannels;
+  return group_channels > 8 ? group_channels : 8 / group_channels * group_channels;
 }
 
 struct JoinPlace {
-  int view, group, channel, channels;  // first group and channel, and its channels
-  int width, lanes, x, y;              // channels at a time, and the thread's place
+  int view, channel, channels;     // first channel, and channels
+  int width, lanes, x, y;          // of a row of threads, and the thread's place
 
   __device__ __forceinline__ JoinPlace(const NormShape& s, int view0) {
-    const int run = join_run(s.group_channels);
+    const int run = join_channels(s.group_channels);
     view = view0 + blockIdx.y;
-    group = blockIdx.x * run;
-    channel = group * s.group_channels;
-    channels = min(run, s.groups - group) * s.group_channels;
-    const int shift = s.group_channels > 16 ? 5 : s.group_channels > 8 ? 4 : 3;
+    channel = blockIdx.x * run;
+    channels = min(run, s.channels - channel);
+    const int shift = run > 16 ? 5 : run > 8 ? 4 : 3;
     width = 1 << shift;
     lanes = kJoinThreads >> shift;
     x = threadIdx.x & (width - 1);
@@ -477,7 +514,7 @@ struct ClusterShare {
   int mine;          // the thread's rows
   int channel;       // first channel of the tile
   int channels;      // of the tile
-  long long first;   // the thread's first row, counted over the views
+  long long row;     // the thread's first row
   TileThread at;
 
   __device__ __forceinline__ ClusterShare(const NormShape& s, const ClusterPlan& t, int vec) {
@@ -496,7 +533,12 @@ struct ClusterShare {
     mine = x < s.cols && at.y < s.lanes && at.y < rows ? (rows - at.y + s.lanes - 1) / s.lanes : 0;
     channel = s.fold > 1 ? 0 : tile * s.tile_cols * vec;
     channels = s.fold > 1 ? s.channels : min(s.tile_cols, s.cols - tile * s.tile_cols) * vec;
-    first = view * s.rows + row0 + at.y;
+    row = row0 + at.y;
+  }
+
+  // Where this thread's first vector is in an image.
+  __device__ __forceinline__ long long in(long long view_size, long long row_size) const {
+    return view * view_size + row * row_size + col;
   }
 
   // Values of a channel in a rank's share.
@@ -610,17 +652,29 @@ inline float norm_bound(int activation) {
   return activation == DR_ACTIVATION_RELU ? 0.0f : -__builtin_huge_valf();
 }
 
-// A vector width and a number of folded pixels.
+// A vector width and a number of folded pixels, which rows may start with at any element.
 struct NormVector {
   int vec, fold;
+  bool turned;
 };
+
+inline int widest_vector(int dtype) { return 16 / dtype_bytes(dtype); }
+inline int folded_pixels(int channels, int dtype) {
+  return widest_vector(dtype) / greatest_divisor(channels, widest_vector(dtype));
+}
+// Whether rows of folded pixels have few enough columns, and views a row of them at least.
+inline bool can_fold(long long pixels, int channels, int dtype) {
+  const long long row = static_cast<long long>(channels) * folded_pixels(channels, dtype);
+  return row / widest_vector(dtype) <= kNormThreads &&
+         pixels * channels >= row + widest_vector(dtype) - 1;
+}
 
 // The widest vectors that the addresses, the strides and the channels allow. Strides are elements
 // between the pixels of x and of the output's gradient (`channels` where there is none).
 inline NormVector choose_vector(long long pixels, int channels, int dtype, long long x_stride,
                                 long long grad_stride,
-                                std::initializer_list<const void*> pointers) {
-  const int size = dtype_bytes(dtype), widest = 16 / size;
+                                std::initializer_list<const void*> pointers, bool turn) {
+  const int size = dtype_bytes(dtype), widest = widest_vector(dtype);
   auto fits = [&](int v) {
     for (const void* p : pointers)
       if (!aligned_to(p, static_cast<size_t>(v) * size)) return false;
@@ -630,14 +684,16 @@ inline NormVector choose_vector(long long pixels, int channels, int dtype, long 
     return channels % v == 0 && x_stride % v == 0 && grad_stride % v == 0;
   };
   if (fits(widest)) {
-    if (divides(widest)) return {widest, 1};
-    const int fold = widest / greatest_divisor(channels, widest);
-    if (x_stride == channels && grad_stride == channels && pixels % fold == 0 &&
-        static_cast<long long>(channels) * fold / widest <= kNormThreads)
-      return {widest, fold};
+    if (divides(widest)) return {widest, 1, false};
+    const int fold = folded_pixels(channels, dtype);
+    if (x_stride == channels && grad_stride == channels && can_fold(pixels, channels, dtype)) {
+      if (pixels % fold == 0) return {widest, fold, false};
+      if (turn) return {widest, fold, true};
+    }
   }
-  if (widest == 8 && fits(2) && divides(2)) return {2, 1};
-  return {1, 1};
+  for (int v : {4, 2})
+    if (v < widest && fits(v) && divides(v)) return {v, 1, false};
+  return {1, 1, false};
 }
 
 // Cuts views into tiles of at most `most_cols` columns and chunks of rows of about `chunk_bytes`.
@@ -650,10 +706,17 @@ inline void cut_norm(NormShape& s, const NormVector& v, long long batch, long lo
   s.groups = groups;
   s.group_channels = channels / groups;
   s.fold = v.fold;
-  s.rows = pixels / s.fold;
+  s.turned = v.turned ? v.vec : 0;
+  s.rows = v.turned ? (pixels * channels - (v.vec - 1)) / (static_cast<long long>(channels) * v.fold)
+                    : pixels / v.fold;
+  s.leftover = static_cast<int>(pixels - s.rows * v.fold);
   s.cols = static_cast<int>(static_cast<long long>(channels) * s.fold / v.vec);
   s.x_row = x_stride * s.fold;
   s.grad_row = grad_stride * s.fold;
+  s.out_row = static_cast<long long>(channels) * s.fold;
+  s.x_view = x_stride * pixels;
+  s.grad_view = grad_stride * pixels;
+  s.out_view = channels * pixels;
   s.tiles = (s.cols + most_cols - 1) / most_cols;
   s.tile_cols = (s.cols + s.tiles - 1) / s.tiles;
   s.lanes = kNormThreads / s.tile_cols;
@@ -671,8 +734,8 @@ inline bool too_large(long long batch, long long pixels) {
 
 // Blocks for each view of the kernels that join the blocks' sums (see JoinPlace).
 inline unsigned int join_runs(const NormShape& s) {
-  const int run = join_run(s.group_channels);
-  return static_cast<unsigned int>((s.groups + run - 1) / run);
+  const int run = join_channels(s.group_channels);
+  return static_cast<unsigned int>((s.channels + run - 1) / run);
 }
 
 constexpr int kMostShared = 220 * 1024;  // dynamic shared memory of a block
@@ -815,8 +878,8 @@ inline void plan_passes(NormShape& s, const NormVector& v, long long batch, long
            std::max(row, (bytes + blocks - 1) / blocks));
 }
 
-// Workspace: a pair of each channel for each chunk; for the backward pass also one of each view and
-// channel, and the table of the second pass.
+// Workspace: a pair of each channel for each chunk, and one of each view and channel; for the
+// backward pass also the table of the second pass.
 struct NormSpace {
   size_t parts, sums, table, total;  // offsets, and the end
 };
@@ -826,7 +889,7 @@ inline NormSpace norm_space(const NormShape& s, bool backward) {
   NormSpace w;
   w.parts = 0;
   w.sums = align256(channels * s.chunks);
-  w.table = w.sums + (backward ? align256(channels) : 0);
+  w.table = w.sums + align256(channels);
   w.total = w.table + (backward ? align256(channels) : 0);
   return w;
 }
@@ -834,24 +897,29 @@ inline NormSpace norm_space(const NormShape& s, bool backward) {
 // The larger workspace of all the vector widths that a call may turn out to take.
 inline size_t norm_workspace_bytes(long long batch, long long pixels, int channels, int groups,
                                    int dtype, bool backward) {
-  const int widest = 16 / dtype_bytes(dtype), images = backward ? 2 : 1;
-  const int fold = widest / greatest_divisor(channels, widest);
+  const int widest = widest_vector(dtype), images = backward ? 2 : 1;
+  const int fold = folded_pixels(channels, dtype);
   size_t most = 0;
-  for (NormVector v : {NormVector{widest, fold}, NormVector{2, 1}, NormVector{1, 1}}) {
-    if (v.fold > 1 && (pixels % v.fold != 0 ||
-                       static_cast<long long>(channels) * v.fold / widest > kNormThreads))
-      continue;
-    if (v.fold == 1 && channels % v.vec != 0) continue;
+  auto passes = [&](const NormVector& v) {
+    NormShape s;
+    plan_passes(s, v, batch, pixels, channels, groups, dtype, channels, channels, images,
+                processors());
+    most = std::max(most, norm_space(s, backward).total);
+  };
+  for (NormVector v : {NormVector{widest, fold, false}, NormVector{4, 1, false},
+                       NormVector{2, 1, false}, NormVector{1, 1, false}}) {
+    if (v.fold > 1 && (pixels % fold != 0 || !can_fold(pixels, channels, dtype))) continue;
+    if (v.fold == 1 && (channels % v.vec != 0 || v.vec > widest)) continue;
     NormShape s;
     ClusterPlan t;
     if (plan_clusters(s, t, v, batch, pixels, channels, groups, dtype, channels, channels, images,
                       processors())) {
       if (backward) most = std::max(most, cluster_space(s));
-    } else {
-      plan_passes(s, v, batch, pixels, channels, groups, dtype, channels, channels, images,
-                  processors());
-      most = std::max(most, norm_space(s, backward).total);
+      continue;
     }
+    passes(v);
+    if (fold > 1 && pixels % fold != 0 && can_fold(pixels, channels, dtype))
+      passes({widest, fold, true});
   }
   return most;
 }
@@ -894,12 +962,14 @@ int with_variant(int dtype, int vec, int activation, int threshold, Fn fn) {
   };
   auto half = [&](auto type) {
     if (vec == 8) return flags(type, std::integral_constant<int, 8>());
+    if (vec == 4) return flags(type, std::integral_constant<int, 4>());
     if (vec == 2) return flags(type, std::integral_constant<int, 2>());
     return flags(type, std::integral_constant<int, 1>());
   };
   if (dtype == DR_FLOAT16) return half(Variant<__half, 0, false, false>());
   if (dtype == DR_BFLOAT16) return half(Variant<__nv_bfloat16, 0, false, false>());
   if (vec == 4) return flags(Variant<float, 0, false, false>(), std::integral_constant<int, 4>());
+  if (vec == 2) return flags(Variant<float, 0, false, false>(), std::integral_constant<int, 2>());
   return flags(Variant<float, 0, false, false>(), std::integral_constant<int, 1>());
 }
 

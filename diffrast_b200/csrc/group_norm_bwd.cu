@@ -11,10 +11,10 @@ constexpr int kStages = 4;  // rows of x and of the gradient that a thread has u
 
 // Joins the threads' sums of a block's rows into those of each channel: over the rows of a warp
 // where the tile's columns divide it, then over the lines of rows that are left. `valid` is the
-// tile's channels (with folded pixels: the view's).
+// tile's channels (with folded pixels: the view's), `turn` the elements before the view's rows.
 template <int V, typename Done>
 __device__ __forceinline__ void join_block(Pairs<V>& sum, Pairs<V>& dot, const TileThread& t,
-                                           const NormShape& s, int valid, float2* entry,
+                                           const NormShape& s, int valid, int turn, float2* entry,
                                            Done done) {
   int lines = s.lanes, line = t.y;
   bool write = t.y < s.lanes;
@@ -43,12 +43,48 @@ __device__ __forceinline__ void join_block(Pairs<V>& sum, Pairs<V>& dot, const T
     for (int j = 0; j < V; ++j) to[j] = make_float2(sum.get(j), dot.get(j));
   }
   __syncthreads();
-  const int items = s.fold > 1 ? s.channels : width;
-  for (int item = t.thread; item < valid; item += t.threads) {
+  // Channel by channel. With more than 16 parts to a channel and threads to spare, several threads
+  // take some of its parts each, and one of them adds what they have.
+  const int items = s.fold > 1 ? s.channels : width, parts = lines * s.fold;
+  const int sharers = parts > 16 ? max(1, min(parts / 4, t.threads / valid)) : 1;
+  auto add_parts = [&](int item, int first_part) {
+    // Channel `item` is `lead` columns on in turned rows.
+    const int at = item < turn ? item - turn + s.channels : item - turn;
     float2 total = make_float2(0.0f, 0.0f);
-    for (int l = 0; l < lines * s.fold; ++l) total = add2(total, entry[l * items + item]);
-    done(item, total);
+    for (int i = first_part; i < parts; i += sharers) total = add2(total, entry[i * items + at]);
+    return total;
+  };
+  if (sharers == 1) {
+    for (int item = t.thread; item < valid; item += t.threads) done(item, add_parts(item, 0));
+    return;
   }
+  __shared__ float2 shares[kNormThreads];
+  const int item = t.thread / sharers;
+  if (item < valid) shares[t.thread] = add_parts(item, t.thread - item * sharers);
+  __syncthreads();
+  if (t.thread < valid) {
+    float2 total = shares[t.thread * sharers];
+    for (int i = 1; i < sharers; ++i) total = add2(total, shares[t.thread * sharers + i]);
+    done(t.thread, total);
+  }
+}
+
+// One element outside the rows: x - m and q.
+struct Leftover {
+  float d, u;
+};
+
+template <typename T, bool Silu, bool Drop>
+__device__ __forceinline__ Leftover leftover_at(const T* x, const T* grad, long long at,
+                                                const float* row, int channels, int channel,
+                                                float bound, const DropKey& key,
+                                                unsigned long long seed) {
+  const float d = to_float(x[at]) + row[channel];
+  const float z = fmaf(d, row[channels + channel], row[2 * channels + channel]);
+  Pairs<1> q;
+  q.p[0] = make_float2(to_float(grad[at]), 0.0f);
+  if (Drop) apply_dropout<1>(q, at, key, seed);
+  return {d, activate_grad<Silu>(q.p[0], make_float2(z, 0.0f), bound).x};
 }
 
 // First pass: sums of q and q (x - m) of each channel over one chunk of rows in one tile of columns.
@@ -61,19 +97,18 @@ __global__ void __launch_bounds__(kNormThreads, Drop ? 2 : 3) norm_sums_kernel(
   let_next_kernel_start();
   const NormPlace p(s, V, view0 + blockIdx.z, blockIdx.y, blockIdx.x);
   RowRing<T, V, 2, kStages> ring;
-  ring.image(0, x, s.x_row, p, s.lanes);
-  ring.image(1, grad, s.grad_row, p, s.lanes);
+  ring.image(0, x, s.x_view, s.x_row, p, s.lanes);
+  ring.image(1, grad, s.grad_view, s.grad_row, p, s.lanes);
   ring.start(shared, p.count);
+  const unsigned long long seed = Drop ? load_seed(key) : 0;
   Pairs<V> sum, dot;
 #pragma unroll
   for (int j = 0; j < Pairs<V>::kCount; ++j) sum.p[j] = dot.p[j] = both(0.0f);
   if (p.count > 0) {
     Affine<V> c;
-    c.load(table, s, p.view, p.col);
-    const unsigned long long seed = Drop ? load_seed(key) : 0;
-    const long long out_row = static_cast<long long>(s.channels) * s.fold;
-    long long at = p.first * out_row + p.col;
-    const long long step = s.lanes * out_row;
+    c.load(table, s, p.view, p.col + p.lead);
+    long long at = p.at(s.out_view, s.out_row);
+    const long long step = s.lanes * s.out_row;
     ring.for_rows([&](Pairs<V> (&v)[2]) {
       if (Drop) apply_dropout<V>(v[1], at, key, seed);
       at += step;
@@ -94,80 +129,101 @@ __global__ void __launch_bounds__(kNormThreads, Drop ? 2 : 3) norm_sums_kernel(
   const TileThread t = {static_cast<int>(threadIdx.x), static_cast<int>(threadIdx.y),
                         static_cast<int>(threadIdx.y * blockDim.x + threadIdx.x),
                         static_cast<int>(blockDim.x * blockDim.y)};
-  join_block<V>(sum, dot, t, s, valid, reinterpret_cast<float2*>(shared),
-                [&](int item, float2 total) { parts[item] = total; });
+  const bool more = p.takes_leftovers(s, blockIdx.y);
+  const float* row = table + static_cast<long long>(p.view) * 3 * s.channels;
+  join_block<V>(sum, dot, t, s, valid, p.lead % s.channels, reinterpret_cast<float2*>(shared),
+                [&](int item, float2 total) {
+    if (more)
+      s.for_leftovers(p.lead, item, [&](long long e) {
+        const long long at = p.view * s.out_view + e;
+        const Leftover l = leftover_at<T, Silu, Drop>(x, grad, at, row, s.channels, item, bound, key, seed);
+        total = make_float2(total.x + l.u, fmaf(l.u, l.d, total.y));
+      });
+    parts[item] = total;
+  });
   wait_for_kernel_before();
 }
 
-// Joins the parts of a view's channels into sums [batch][channels] of q and q h, and forms the
-// constants of the second pass: table [batch][2][channels] of -r A and -r^2 B.
+// The constants of the second pass that a group's sums of q w r and q h w r leave: table
+// [batch][2][channels] of -r A and -r^2 B.
+__device__ __forceinline__ void write_constants(float* table, const NormShape& s, int view,
+                                                int channel, float2 group, float r) {
+  const float inverse =
+      1.0f / (static_cast<float>(s.pixels) * static_cast<float>(s.group_channels));
+  table += static_cast<long long>(view) * 2 * s.channels + channel;
+  table[0] = -group.x * inverse;
+  table[s.channels] = -group.y * inverse * r;
+}
+
+// Joins the parts of a view's channels into sums [batch][channels] of q and q h, and the channels of
+// its groups where a block has them all; the others are left to norm_group_means_kernel.
 __global__ void __launch_bounds__(kJoinThreads) norm_means_kernel(
     const float2* parts, NormShape s, int view0, const float* __restrict__ affine,
     const float* __restrict__ rstd, float2* __restrict__ sums, float* __restrict__ table) {
   __shared__ float2 entry[kJoinThreads + kJoinThreads / 8];
-  __shared__ float2 scaled[32];
-  __shared__ float2 result;  // of a group wider than 32 channels
+  __shared__ float2 scaled[kJoinChannels];
   let_next_kernel_start();
   const JoinPlace p(s, view0);
   const int d = s.group_channels;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   // rstd * weight of the channels
   affine += (static_cast<long long>(p.view) * 3 + 1) * s.channels + p.channel;
-  rstd += static_cast<long long>(p.view) * s.groups + p.group;
+  rstd += static_cast<long long>(p.view) * s.groups;
   parts += static_cast<long long>(p.view) * s.chunks * s.channels + p.channel;
   sums += static_cast<long long>(p.view) * s.channels + p.channel;
-  table += static_cast<long long>(p.view) * 2 * s.channels + p.channel;
   wait_for_kernel_before();
-  const float inverse = 1.0f / (static_cast<float>(s.pixels) * static_cast<float>(d));
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  float2 wide = make_float2(0.0f, 0.0f);
-  for (int base = 0; base < p.channels; base += p.width) {
-    float2 total = make_float2(0.0f, 0.0f);
-    if (base + p.x < p.channels) {
+  float2 total = make_float2(0.0f, 0.0f);
+  if (p.x < p.channels) {
 #pragma unroll 8
-      for (int i = p.y; i < s.chunks; i += p.lanes)
-        total = add2(total, parts[static_cast<long long>(i) * s.channels + base + p.x]);
-    }
-    entry[p.y * (p.width + 1) + p.x] = total;
-    __syncthreads();
-    // Channel `warp`, from its lanes.
-    if (warp < p.width) {
-      total = make_float2(0.0f, 0.0f);
-      for (int i = lane; i < p.lanes; i += 32) total = add2(total, entry[i * (p.width + 1) + warp]);
-      total.x = warp_sum(total.x);
-      total.y = warp_sum(total.y);
-      if (lane == 0) {
-        float2 w = make_float2(0.0f, 0.0f);
-        const int c = base + warp;
-        if (c < p.channels) {
-          const float r = rstd[c / d], scale = affine[c];
-          sums[c] = make_float2(total.x, total.y * r);
-          w = make_float2(total.x * scale, total.y * scale * r);
-        }
-        scaled[warp] = w;
-      }
-    }
-    __syncthreads();
-    if (warp == 0) {
-      if (d > 32) {
-        wide.x += warp_sum(scaled[lane].x);
-        wide.y += warp_sum(scaled[lane].y);
-      } else if (lane < p.channels) {
-        const int g = lane / d;
-        float2 group = scaled[g * d];
-        for (int i = 1; i < d; ++i) group = add2(group, scaled[g * d + i]);
-        table[lane] = -group.x * inverse;
-        table[s.channels + lane] = -group.y * inverse * rstd[g];
-      }
-    }
-    __syncthreads();
+    for (int i = p.y; i < s.chunks; i += p.lanes)
+      total = add2(total, parts[static_cast<long long>(i) * s.channels + p.x]);
   }
-  if (d <= 32) return;
-  if (threadIdx.x == 0) result = make_float2(-wide.x * inverse, -wide.y * inverse * rstd[0]);
+  entry[p.y * (p.width + 1) + p.x] = total;
   __syncthreads();
-  for (int c = threadIdx.x; c < p.channels; c += kJoinThreads) {
-    table[c] = result.x;
-    table[s.channels + c] = result.y;
+  // Channel `warp`, from its lanes.
+  if (warp < p.channels) {
+    total = make_float2(0.0f, 0.0f);
+    for (int i = lane; i < p.lanes; i += 32) total = add2(total, entry[i * (p.width + 1) + warp]);
+    total.x = warp_sum(total.x);
+    total.y = warp_sum(total.y);
+    if (lane == 0) {
+      const float r = rstd[(p.channel + warp) / d], scale = affine[warp];
+      sums[warp] = make_float2(total.x, total.y * r);
+      scaled[warp] = make_float2(total.x * scale, total.y * r * scale);
+    }
   }
+  __syncthreads();
+  if (warp != 0 || lane >= p.channels || d > kJoinChannels) return;
+  const int g = lane / d;
+  float2 group = scaled[g * d];
+  for (int i = 1; i < d; ++i) group = add2(group, scaled[g * d + i]);
+  write_constants(table, s, p.view, p.channel + lane, group, rstd[p.channel / d + g]);
+}
+
+// Joins the channels of one group of a view (groups wider than a block of norm_means_kernel).
+__global__ void __launch_bounds__(kNormThreads) norm_group_means_kernel(
+    const float2* sums, NormShape s, int view0, const float* __restrict__ affine,
+    const float* __restrict__ rstd, float* __restrict__ table) {
+  __shared__ float2 warps[kNormThreads / 32];
+  let_next_kernel_start();
+  wait_for_kernel_before();
+  const int view = view0 + blockIdx.y, first = blockIdx.x * s.group_channels;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const float* scales = affine + (static_cast<long long>(view) * 3 + 1) * s.channels + first;
+  float2 total = make_float2(0.0f, 0.0f);
+  for (int i = threadIdx.x; i < s.group_channels; i += kNormThreads) {
+    const float2 v = sums[static_cast<long long>(view) * s.channels + first + i];
+    total = make_float2(fmaf(v.x, scales[i], total.x), fmaf(v.y, scales[i], total.y));
+  }
+  total.x = warp_sum(total.x);
+  total.y = warp_sum(total.y);
+  if (lane == 0) warps[warp] = total;
+  __syncthreads();
+  total = warps[0];
+  for (int i = 1; i < kNormThreads / 32; ++i) total = add2(total, warps[i]);
+  const float r = rstd[static_cast<long long>(view) * s.groups + blockIdx.x];
+  for (int i = threadIdx.x; i < s.group_channels; i += kNormThreads)
+    write_constants(table, s, view, first + i, total, r);
 }
 
 // Second pass: grad x = r (q w - A - h B) over one chunk of rows in one tile of columns, from the
@@ -182,20 +238,30 @@ __global__ void __launch_bounds__(kNormThreads, Drop ? 2 : 3) norm_grad_kernel(
   const NormPlace p(s, V, view0 + gridDim.z - 1 - blockIdx.z, gridDim.y - 1 - blockIdx.y,
                     gridDim.x - 1 - blockIdx.x);
   RowRing<T, V, 2, kStages> ring;
-  ring.image(0, x, s.x_row, p, s.lanes);
-  ring.image(1, grad, s.grad_row, p, s.lanes);
+  ring.image(0, x, s.x_view, s.x_row, p, s.lanes);
+  ring.image(1, grad, s.grad_view, s.grad_row, p, s.lanes);
   ring.start(shared, p.count);
   Affine<V> c;
-  if (p.count > 0) c.load(affine, s, p.view, p.col);
-  wait_for_kernel_before();
-  if (p.count == 0) return;
-  table += static_cast<long long>(p.view) * 2 * s.channels;
-  const Pairs<V> base = load_row<V>(table, s, p.col);
-  const Pairs<V> slope = load_row<V>(table + s.channels, s, p.col);
+  if (p.count > 0) c.load(affine, s, p.view, p.col + p.lead);
   const unsigned long long seed = Drop ? load_seed(key) : 0;
-  const long long out_row = static_cast<long long>(s.channels) * s.fold;
-  long long at = p.first * out_row + p.col;
-  const long long step = s.lanes * out_row;
+  wait_for_kernel_before();
+  table += static_cast<long long>(p.view) * 2 * s.channels;
+  if (p.takes_leftovers(s, gridDim.y - 1 - blockIdx.y)) {
+    const float* row = affine + static_cast<long long>(p.view) * 3 * s.channels;
+    for (int ch = threadIdx.y * blockDim.x + threadIdx.x; ch < s.channels;
+         ch += blockDim.x * blockDim.y)
+      s.for_leftovers(p.lead, ch, [&](long long e) {
+        const long long own = p.view * s.out_view + e;
+        const Leftover l = leftover_at<T, Silu, Drop>(x, grad, own, row, s.channels, ch, bound, key, seed);
+        grad_x[own] = from_float<T>(
+            fmaf(l.u, row[s.channels + ch], fmaf(l.d, table[s.channels + ch], table[ch])));
+      });
+  }
+  if (p.count == 0) return;
+  const Pairs<V> base = load_row<V>(table, s, p.col + p.lead);
+  const Pairs<V> slope = load_row<V>(table + s.channels, s, p.col + p.lead);
+  long long at = p.at(s.out_view, s.out_row);
+  const long long step = s.lanes * s.out_row;
   ring.for_rows([&](Pairs<V> (&v)[2]) {
     if (Drop) apply_dropout<V>(v[1], at, key, seed);
 #pragma unroll
@@ -268,11 +334,10 @@ __global__ void __launch_bounds__(kNormThreads, Drop ? 2 : 3) norm_cluster_bwd_k
   rows.slots = static_cast<unsigned int>(__cvta_generic_to_shared(shared)) +
                threadIdx.x * static_cast<unsigned int>(sizeof(Packed<T, V>));
   rows.count = p.mine;
-  rows.fetch({x + p.first * s.x_row + p.col, grad + p.first * s.grad_row + p.col},
+  rows.fetch({x + p.in(s.x_view, s.x_row), grad + p.in(s.grad_view, s.grad_row)},
              {s.lanes * s.x_row, s.lanes * s.grad_row});
   const unsigned long long seed = Drop ? load_seed(key) : 0;
-  const long long out_row = static_cast<long long>(s.channels) * s.fold;
-  const long long start = p.first * out_row + p.col, stride = s.lanes * out_row;
+  const long long start = p.in(s.out_view, s.out_row), stride = s.lanes * s.out_row;
   Affine<V> c;
   Pairs<V> sum, dot;
 #pragma unroll
@@ -292,7 +357,7 @@ __global__ void __launch_bounds__(kNormThreads, Drop ? 2 : 3) norm_cluster_bwd_k
       dot.p[j] = fma2(u, e, dot.p[j]);
     }
   });
-  join_block<V>(sum, dot, p.at, s, p.channels, entry,
+  join_block<V>(sum, dot, p.at, s, p.channels, 0, entry,
                 [&](int item, float2 total) { channel[item] = total; });
   const int d = s.group_channels;
   float2* joined = channel;
@@ -422,6 +487,9 @@ int passes(const void* x, const void* grad, const NormShape& s, const float* aff
     if (err == cudaSuccess)
       err = launch_kernel(norm_means_kernel, dim3(runs, views), kJoinThreads, 0, stream, true,
                           parts, s, view0, affine, rstd, sums, table);
+    if (err == cudaSuccess && out.x != nullptr && s.group_channels > kJoinChannels)
+      err = launch_kernel(norm_group_means_kernel, dim3(s.groups, views), kNormThreads, 0, stream,
+                          true, sums, s, view0, affine, rstd, table);
     if (err == cudaSuccess && out.x != nullptr)
       err = launch_kernel(norm_grad_kernel<T, V, Silu, Drop>, blocks, threads, ring, stream, true,
                           in, dy, s, view0, affine, table, bound, key, static_cast<T*>(out.x));
@@ -454,13 +522,15 @@ extern "C" int dr_group_norm_bwd(const void* x, int64_t x_stride, const void* gr
   if (too_large(batch, pixels)) return DR_ERR_TOO_LARGE;
   NormShape s;
   ClusterPlan t;
-  const NormVector v = choose_vector(pixels, channels, dtype, x_stride, grad_stride,
-                                     {x, grad_y, grad_x});
+  NormVector v = choose_vector(pixels, channels, dtype, x_stride, grad_stride,
+                               {x, grad_y, grad_x}, false);
   const bool small = plan_clusters(s, t, v, batch, pixels, channels, groups, dtype, x_stride,
                                    grad_stride, 2, processors());
-  if (!small)
+  if (!small) {
+    v = choose_vector(pixels, channels, dtype, x_stride, grad_stride, {x, grad_y, grad_x}, true);
     plan_passes(s, v, batch, pixels, channels, groups, dtype, x_stride, grad_stride, 2,
                 processors());
+  }
   const size_t need = small ? cluster_space(s) : norm_space(s, true).total;
   if (workspace == nullptr || workspace_bytes < need) return DR_ERR_WORKSPACE_TOO_SMALL;
   const DropKey key = drop_key(seed, seed_value, layer, drop_threshold);

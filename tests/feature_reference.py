@@ -22,15 +22,20 @@ def threshold(p: float) -> int:
 
 
 def keep_mask(count: int, p: float, seed: int, layer: int = 0, first: int = 0) -> torch.Tensor:
-    """Which of the elements ``first .. first + count - 1`` are kept."""
+    """Which of the elements ``first .. first + count - 1`` are kept: the generator again, for all
+    counters at once."""
     seed &= (1 << 64) - 1
-    key = (seed & 0xFFFFFFFF, seed >> 32)
-    bits = []
-    for block in range(first // 8, (first + count + 7) // 8):
-        for word in philox4x32_10((block & 0xFFFFFFFF, block >> 32, layer, 0), key):
-            bits += [word & 0xFFFF, word >> 16]
-    skip = first % 8
-    return torch.tensor(bits[skip:skip + count]) >= threshold(p)
+    block = torch.arange(first // 8, (first + count + 7) // 8)
+    word = 0xFFFFFFFF
+    c = [block & word, block >> 32, torch.full_like(block, layer), torch.zeros_like(block)]
+    k = [seed & word, seed >> 32]
+    for _ in range(10):
+        # Products wrap in signed 64 bits, which keeps all their bits.
+        p0, p1 = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
+        c = [((p1 >> 32) & word) ^ c[1] ^ k[0], p1 & word, ((p0 >> 32) & word) ^ c[3] ^ k[1], p0 & word]
+        k = [(k[0] + 0x9E3779B9) & word, (k[1] + 0xBB67AE85) & word]
+    bits = torch.stack([half for w in c for half in (w & 0xFFFF, w >> 16)], 1).reshape(-1)
+    return bits[first % 8:first % 8 + count] >= threshold(p)
 
 
 def keep_scale(p: float) -> float:

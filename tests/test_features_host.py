@@ -19,6 +19,14 @@ def test_generator_known_answers():
         0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
 
 
+def test_masks_are_made_of_the_generators_words():
+    seed, layer = 0xFEDCBA9876543210, 5
+    for block in (0, 1, 77, (1 << 32) + 3):
+        words = philox4x32_10((block & 0xFFFFFFFF, block >> 32, layer, 0), (seed & 0xFFFFFFFF, seed >> 32))
+        want = [half >= threshold(0.3) for w in words for half in (w & 0xFFFF, w >> 16)]
+        assert keep_mask(8, 0.3, seed, layer, first=8 * block).tolist() == want
+
+
 def test_mask_of_a_range_is_a_range_of_the_mask():
     whole = keep_mask(64, 0.5, 12345, layer=2)
     assert torch.equal(keep_mask(21, 0.5, 12345, layer=2, first=13), whole[13:34])

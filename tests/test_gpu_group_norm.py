@@ -145,6 +145,43 @@ def test_matches_64_bits(shape, groups, dtype):
     compare(features(shape, dtype, 1), groups, w, b, activation="silu")
 
 
+# Above one megabyte images are taken in two passes: whole vectors, folded pixels, rows that start
+# anywhere, groups wider than 32 channels, more views than processors.
+LARGE = [
+    ((2, 90, 100, 64), 32), ((1, 300, 400, 5), 5), ((3, 97, 101, 30), 5), ((2, 301, 303, 7), 1),
+    ((2, 63, 65, 100), 5), ((1, 61, 47, 512), 2), ((2, 40, 41, 520), 1), ((5, 75, 75, 33), 33),
+    ((150, 33, 37, 4), 1), ((2, 33, 35, 260), 4), ((1, 3, 3, 60000), 3),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape, groups", LARGE)
+def test_two_passes_match_64_bits(shape, groups, dtype):
+    w, b = params(shape[-1], 60)
+    compare(features(shape, dtype, 61), groups, w, b, activation="silu")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape, groups", [((2, 90, 100, 64), 8), ((3, 97, 101, 30), 5), ((2, 301, 303, 7), 1)])
+def test_two_passes_with_dropout_and_parameters_of_each_view(shape, groups, dtype):
+    w, b = params(shape[-1], 62, batch=shape[0])
+    compare(features(shape, dtype, 63), groups, w, b, activation="silu", dropout=0.2, seed=9, layer=1)
+    compare(features(shape, dtype, 64), groups)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("extra", [1, 2, 4, 8])
+def test_two_passes_over_channel_slices(extra, dtype):
+    shape = (2, 120, 130, 32)
+
+    def in_wide(t):
+        wide = torch.full((*shape[:-1], 32 + extra), float("nan"), dtype=t.dtype, device=CUDA)
+        wide[..., extra:] = t.to(CUDA)
+        return wide[..., extra:]
+
+    compare(features(shape, dtype, 65), 4, *params(32, 66), activation="silu", on_gpu=in_wide)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("activation", ["none", "relu", "silu"])
 @pytest.mark.parametrize("shape, groups", [((2, 9, 11, 24), 4), ((2, 10, 12, 6), 2), ((1, 7, 5, 3), 1)])
@@ -214,6 +251,9 @@ def test_offset_far_above_the_spread():
     compare(x, 2, *params(16, 13), activation="silu")
     x[:, 0, 0] = 0.0
     compare(x, 2, *params(16, 13), activation="silu")
+    x = 1000 + torch.randint(-200, 200, (1, 150, 151, 16), generator=gen) / 1024.0
+    x[:, 0, 0] = 0.0
+    compare(x, 2, *params(16, 13), activation="silu")
 
 
 def test_constant_groups_and_large_values():
@@ -228,7 +268,7 @@ def test_constant_groups_and_large_values():
 
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("shape, groups", [((2, 8, 8, 16), 4), ((2, 80, 80, 12), 3)])
+@pytest.mark.parametrize("shape, groups", [((2, 8, 8, 16), 4), ((2, 80, 80, 12), 3), ((2, 203, 207, 12), 3)])
 def test_non_finite_values_stay_in_their_group(value, dtype, shape, groups):
     x = features(shape, dtype, 16).to(CUDA)
     w, b = (t.to(CUDA) for t in params(shape[-1], 17))
@@ -281,12 +321,13 @@ def test_gradients_against_differences():
         assert abs(got - slope) < 1e-3 * float(grads[k].double().norm()) * float(direction.norm())
 
 
-def test_runs_agree_bit_for_bit():
-    x = features((3, 100, 90, 40), torch.bfloat16, 22).to(CUDA).requires_grad_(True)
-    w, b = (t.to(CUDA).requires_grad_(True) for t in params(40, 23))
+@pytest.mark.parametrize("shape", [(3, 20, 30, 40), (3, 100, 90, 40), (3, 101, 103, 42)])
+def test_runs_agree_bit_for_bit(shape):
+    x = features(shape, torch.bfloat16, 22).to(CUDA).requires_grad_(True)
+    w, b = (t.to(CUDA).requires_grad_(True) for t in params(shape[-1], 23))
 
     def run():
-        y = dr.group_norm(x, 5, w, b, activation="silu", dropout=0.1, seed=1)
+        y = dr.group_norm(x, 2, w, b, activation="silu", dropout=0.1, seed=1)
         return [y, *torch.autograd.grad(y, (x, w, b), torch.ones_like(y))]
 
     first = run()
@@ -294,8 +335,9 @@ def test_runs_agree_bit_for_bit():
         assert all(torch.equal(p, q) for p, q in zip(run(), first))
 
 
-def test_only_the_gradients_asked_for():
-    x = features((2, 9, 9, 16), torch.float32, 24).to(CUDA)
+@pytest.mark.parametrize("side", [9, 151])
+def test_only_the_gradients_asked_for(side):
+    x = features((2, side, side, 16), torch.float32, 24).to(CUDA)
     w, b = (t.to(CUDA) for t in params(16, 25))
     g = torch.randn_like(x)
 
@@ -341,13 +383,13 @@ def training_step(x, w, b, seed, g):
     return [y.detach(), *torch.autograd.grad(y, (x, w, b), g)]
 
 
-@pytest.mark.parametrize("shape", [(2, 9, 9, 32), (2, 200, 180, 32)])
+@pytest.mark.parametrize("shape", [(2, 9, 9, 32), (2, 200, 180, 32), (3, 101, 103, 36)])
 def test_two_streams_and_two_graphs_at_once(shape):
     """Steps on two streams, and two captured steps replayed on two streams, do not share state."""
     sets, want = [], []
     for k in range(2):
         x = features(shape, torch.bfloat16, 30 + k).to(CUDA).requires_grad_(True)
-        w, b = (t.to(CUDA).requires_grad_(True) for t in params(32, 32 + k))
+        w, b = (t.to(CUDA).requires_grad_(True) for t in params(shape[-1], 32 + k))
         g = torch.randn(shape, device=CUDA).bfloat16()
         sets.append((x, w, b, torch.tensor([k], device=CUDA), g))
         want.append(training_step(*sets[k]))
