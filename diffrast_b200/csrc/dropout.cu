@@ -119,7 +119,10 @@ extern "C" int dr_dropout(const void* x, const void* residual, int64_t count, in
   if (count < 0 || !known_dtype(dtype) || bad_drop(threshold, layer))
     return DR_ERR_INVALID_ARGUMENT;
   if (count == 0) return DR_OK;
-  if (x == nullptr || y == nullptr) return DR_ERR_INVALID_ARGUMENT;
+  const size_t size = dtype_bytes(dtype);
+  if (x == nullptr || y == nullptr || !aligned_to(x, size) || !aligned_to(y, size) ||
+      !aligned_to(residual, size) || !aligned_to(seed, sizeof(int64_t)))
+    return DR_ERR_INVALID_ARGUMENT;
   // At most 2^31 - 1 blocks.
   if (count > 8LL * kThreads * kCounters * 0x7FFFFFFF) return DR_ERR_TOO_LARGE;
   const DropKey key = drop_key(seed, seed_value, layer, threshold);

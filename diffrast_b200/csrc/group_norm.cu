@@ -409,7 +409,8 @@ extern "C" size_t dr_group_norm_state_floats(int64_t batch, int32_t channels, in
 
 extern "C" size_t dr_group_norm_workspace_bytes(int64_t batch, int64_t pixels, int32_t channels,
                                                 int32_t groups, int32_t dtype, int32_t backward) {
-  if (bad_norm_sizes(batch, pixels, channels, groups, dtype) || too_large(batch, pixels)) return 0;
+  if (bad_norm_sizes(batch, pixels, channels, groups, dtype) || too_large(batch, pixels, channels))
+    return 0;
   return norm_workspace_bytes(batch, pixels, channels, groups, dtype, backward != 0);
 }
 
@@ -427,9 +428,12 @@ extern "C" int dr_group_norm_fwd(const void* x, int64_t x_stride, int32_t dtype,
       activation > DR_ACTIVATION_SILU || bad_drop(drop_threshold, layer))
     return DR_ERR_INVALID_ARGUMENT;
   if (batch == 0 || pixels == 0) return DR_OK;
-  if (x == nullptr || y == nullptr || state == nullptr || !aligned_to(state, 16))
+  const size_t size = dtype_bytes(dtype);
+  if (x == nullptr || y == nullptr || state == nullptr || !aligned_to(state, 16) ||
+      !aligned_to(workspace, 16) || !aligned_to(seed, sizeof(int64_t)) || !aligned_to(x, size) ||
+      !aligned_to(y, size))
     return DR_ERR_INVALID_ARGUMENT;
-  if (too_large(batch, pixels)) return DR_ERR_TOO_LARGE;
+  if (too_large(batch, pixels, x_stride)) return DR_ERR_TOO_LARGE;
   NormShape s;
   ClusterPlan t;
   NormVector v = choose_vector(pixels, channels, dtype, x_stride, channels, {x, y}, false);

@@ -645,7 +645,8 @@ inline bool bad_norm_sizes(int64_t batch, int64_t pixels, int32_t channels, int3
 }
 
 inline bool bad_norm_param(const void* data, int32_t dtype, int64_t rows, int64_t batch) {
-  return data != nullptr && (!known_dtype(dtype) || (rows != 1 && rows != batch));
+  return data != nullptr && (!known_dtype(dtype) || (rows != 1 && rows != batch) ||
+                             !aligned_to(data, dtype_bytes(dtype)));
 }
 
 inline float norm_bound(int activation) {
@@ -727,9 +728,12 @@ inline void cut_norm(NormShape& s, const NormVector& v, long long batch, long lo
   s.chunks = static_cast<int>((s.rows + s.chunk_rows - 1) / s.chunk_rows);
 }
 
-// Views, and pixels of a view, that still leave blocks and rows countable in 32 bits.
-inline bool too_large(long long batch, long long pixels) {
-  return batch > 0x7FFFFFFFLL || pixels > 0x7FFFFFFFLL;
+// Views, and pixels of a view, that leave blocks and rows countable in 32 bits, and at most 2^48
+// elements (more than any device holds), so that no offset or byte count passes 64.
+inline bool too_large(long long batch, long long pixels, long long stride) {
+  constexpr long long kMost = 1LL << 48;
+  return batch > 0x7FFFFFFFLL || pixels > 0x7FFFFFFFLL ||
+         (batch > 0 && pixels > 0 && stride > kMost / batch / pixels);
 }
 
 // Blocks for each view of the kernels that join the blocks' sums (see JoinPlace).

@@ -276,17 +276,23 @@ __global__ void __launch_bounds__(kNormThreads, Drop ? 2 : 3) norm_grad_kernel(
   });
 }
 
-// Gradients of weight and bias: sums over the views (or each view's own), 32 channels a block.
+// Gradients of weight and bias: sums over the views (or each view's own), 8 channels a block. The
+// sums are held in 64 bits: a lane may add thousands of views one after the other, which in 32 bits
+// left 131077 equal views 1e-4 off.
+constexpr int kParamChannels = 8;
+
 __global__ void __launch_bounds__(kNormThreads) norm_params_kernel(
     const float2* sums, long long batch, int channels, void* grad_weight,
     int weight_dtype, bool weight_views, void* grad_bias, int bias_dtype, bool bias_views) {
-  constexpr int kLanes = kNormThreads / 32;
-  __shared__ float2 entry[kLanes][32];
+  constexpr int kLanes = kNormThreads / kParamChannels;
+  __shared__ double2 entry[kLanes][kParamChannels];
   let_next_kernel_start();
   wait_for_kernel_before();
-  const int c = blockIdx.x * 32 + threadIdx.x % 32, lane = threadIdx.x / 32;
-  float2 total = make_float2(0.0f, 0.0f);
+  const int x = threadIdx.x % kParamChannels, lane = threadIdx.x / kParamChannels;
+  const int c = blockIdx.x * kParamChannels + x;
+  double2 total = make_double2(0.0, 0.0);
   if (c < channels) {
+#pragma unroll 4
     for (long long n = lane; n < batch; n += kLanes) {
       const float2 v = sums[n * channels + c];
       if (grad_weight != nullptr && weight_views)
@@ -297,15 +303,18 @@ __global__ void __launch_bounds__(kNormThreads) norm_params_kernel(
       total.y += v.y;
     }
   }
-  entry[lane][threadIdx.x % 32] = total;
+  entry[lane][x] = total;
   __syncthreads();
   if (lane != 0 || c >= channels) return;
-  for (int i = 1; i < kLanes; ++i) {
-    total.x += entry[i][threadIdx.x].x;
-    total.y += entry[i][threadIdx.x].y;
+  const int lanes = static_cast<int>(min(batch, static_cast<long long>(kLanes)));
+  for (int i = 1; i < lanes; ++i) {
+    total.x += entry[i][x].x;
+    total.y += entry[i][x].y;
   }
-  if (grad_weight != nullptr && !weight_views) store_param(grad_weight, weight_dtype, c, total.y);
-  if (grad_bias != nullptr && !bias_views) store_param(grad_bias, bias_dtype, c, total.x);
+  if (grad_weight != nullptr && !weight_views)
+    store_param(grad_weight, weight_dtype, c, static_cast<float>(total.y));
+  if (grad_bias != nullptr && !bias_views)
+    store_param(grad_bias, bias_dtype, c, static_cast<float>(total.x));
 }
 
 struct Gradients {
@@ -446,7 +455,7 @@ int params(const NormShape& s, const float2* sums, const Gradients& out, cudaStr
            bool after) {
   if (out.weight == nullptr && out.bias == nullptr) return DR_OK;
   return static_cast<int>(launch_kernel(
-      norm_params_kernel, blocks_for(s.channels, 32), kNormThreads, 0, stream, after, sums,
+      norm_params_kernel, blocks_for(s.channels, kParamChannels), kNormThreads, 0, stream, after, sums,
       s.batch, s.channels, out.weight, out.weight_dtype, out.weight_views, out.bias,
       out.bias_dtype, out.bias_views));
 }
@@ -517,9 +526,12 @@ extern "C" int dr_group_norm_bwd(const void* x, int64_t x_stride, const void* gr
       bad_drop(drop_threshold, layer))
     return DR_ERR_INVALID_ARGUMENT;
   if (batch == 0 || pixels == 0) return DR_OK;
-  if (x == nullptr || grad_y == nullptr || state == nullptr || !aligned_to(state, 16))
+  const size_t size = dtype_bytes(dtype);
+  if (x == nullptr || grad_y == nullptr || state == nullptr || !aligned_to(state, 16) ||
+      !aligned_to(workspace, 16) || !aligned_to(seed, sizeof(int64_t)) || !aligned_to(x, size) ||
+      !aligned_to(grad_y, size) || !aligned_to(grad_x, size))
     return DR_ERR_INVALID_ARGUMENT;
-  if (too_large(batch, pixels)) return DR_ERR_TOO_LARGE;
+  if (too_large(batch, pixels, std::max(x_stride, grad_stride))) return DR_ERR_TOO_LARGE;
   NormShape s;
   ClusterPlan t;
   NormVector v = choose_vector(pixels, channels, dtype, x_stride, grad_stride,

@@ -491,7 +491,8 @@ int dr_lambert_bwd(const float* color, const float* normal, int64_t normal_strid
  * counter (e / 8 low, e / 8 high, layer, 0): bits 16 (e % 2) and up of word (e % 8) / 2. It is
  * dropped (0, whatever its value) when they are below drop_threshold (0..65535; 0 drops nothing)
  * and scaled by 65536 / (65536 - drop_threshold) otherwise. The seed is read from the device
- * word `seed`, or is seed_value when seed is NULL; the layer is below 2^32.
+ * word `seed`, or is seed_value when seed is NULL; the layer is below 2^32. Images and parameters
+ * are aligned to their element type, workspaces to 16 bytes.
  * ------------------------------------------------------------------------------------------- */
 
 /* y = (residual, or 0 if NULL) + dropout(x), `count` contiguous elements each; y overlaps

@@ -118,11 +118,12 @@ def test_c_abi_refuses_before_any_cuda_call():
     common = [dict(dtype=3), dict(dtype=-1), dict(batch=-1), dict(pixels=-1), dict(channels=0),
               dict(groups=0), dict(groups=3), dict(x_stride=7), dict(act=3), dict(act=-1),
               dict(drop=-1), dict(drop=65536), dict(layer=-1), dict(layer=1 << 32), dict(w=16, wb=3), dict(b=16, bd=4), dict(x=None),
+              dict(x=18), dict(dtype=1, x=17), dict(w=18), dict(w=17, wd=1), dict(b=18), dict(ws=24), dict(seed=20),
               dict(state=None), dict(state=8), dict(channels=1 << 17, x_stride=1 << 17, gy_stride=1 << 17)]
-    for change in common + [dict(y=None)]:
+    for change in common + [dict(y=None), dict(y=18)]:
         change.pop("gy_stride", None)
         assert fwd(lib, **change) == bad, change
-    for change in common + [dict(gy=None), dict(gy_stride=7)]:
+    for change in common + [dict(gy=None), dict(gy_stride=7), dict(gy=18), dict(gx=18)]:
         assert bwd(lib, **change) == bad, change
     for call in (fwd, bwd):
         # An image too large for shared memory needs scratch in both directions.
@@ -130,17 +131,22 @@ def test_c_abi_refuses_before_any_cuda_call():
         assert call(lib, pixels=1 << 24, ws=None) == small
         assert call(lib, batch=0) == 0 and call(lib, pixels=0) == 0
         assert call(lib, batch=1 << 31) == 10003 and call(lib, pixels=1 << 31) == 10003
+        # Sizes whose products would pass 64 bits.
+        assert call(lib, batch=(1 << 31) - 1, pixels=(1 << 31) - 1) == 10003
+        assert call(lib, x_stride=1 << 62) == 10003
+    assert bwd(lib, gy_stride=1 << 62) == 10003
+    assert lib.dr_group_norm_workspace_bytes((1 << 31) - 1, (1 << 31) - 1, 1 << 16, 2, 0, 1) == 0
     assert lib.dr_group_norm_workspace_bytes(2, 9, 8, 3, 0, 0) == 0
     assert lib.dr_group_norm_state_floats(2, 8, 4) == 2 * (3 * 8 + 4)
     for backward in (0, 1):
         assert lib.dr_group_norm_workspace_bytes(2, 1 << 24, 8, 2, 0, backward) > 0
     assert lib.dr_group_norm_workspace_bytes(2, 9, 8, 2, 0, 0) == 0
 
-    def drop(x=16, res=None, count=8, dtype=0, thr=1, y=16):
-        return lib.dr_dropout(x, res, count, dtype, thr, None, 0, 0, y, None)
+    def drop(x=16, res=None, count=8, dtype=0, thr=1, seed=None, y=16):
+        return lib.dr_dropout(x, res, count, dtype, thr, seed, 0, 0, y, None)
 
     for change in (dict(count=-1), dict(dtype=3), dict(thr=-1), dict(thr=65536), dict(x=None),
-                   dict(y=None)):
+                   dict(y=None), dict(x=18), dict(y=18), dict(res=18), dict(dtype=2, x=17), dict(seed=20)):
         assert drop(**change) == bad, change
     assert drop(count=1 << 44) == 10003
     assert drop(count=0) == 0

@@ -169,6 +169,40 @@ def test_two_passes_with_dropout_and_parameters_of_each_view(shape, groups, dtyp
     compare(features(shape, dtype, 64), groups)
 
 
+@pytest.mark.parametrize("shape, groups, dropout", [
+    ((70001, 5, 6), 2, 0.0), ((131077, 7, 7), 1, 0.3), ((66000, 1, 8), 2, 0.3)])
+def test_more_views_than_one_launch_takes(shape, groups, dropout):
+    """A launch takes 65535 views; gradients of shared parameters are sums over all of them."""
+    x = features(shape, torch.float16, 5)
+    compare(x, groups, *params(shape[-1], 6), activation="silu", dropout=dropout, seed=4)
+
+
+@pytest.mark.parametrize("dtype, pixels, channels, copies, groups, views, long", [
+    (torch.float16, 1 << 16, 64, 1025, 8, True, 1), (torch.bfloat16, 100003, 33, 1310, 11, False, 70)])
+def test_element_indices_pass_32_bits(dtype, pixels, channels, copies, groups, views, long):
+    """Copies of one image, as views or as the pixels of one view, have the image's statistics and
+    gradients. In the long view a thread of the join takes 1030 chunks in a row, each with up to
+    four roundings: 64 u + 4 * 1030 u are at most 70 times the 64 u and more of the bounds."""
+    image = features((1, pixels, channels), dtype, 8)
+    grad = torch.randn(1, pixels, channels, generator=torch.Generator().manual_seed(9)).to(dtype)
+    weight, bias = params(channels, 10)
+    shape = (copies, pixels, channels) if views else (1, copies * pixels, channels)
+    x, dy = (t.to(CUDA).expand(copies, -1, -1).reshape(shape) for t in (image, grad))
+    x.requires_grad_(True)
+    y = dr.group_norm(x, groups, weight.to(CUDA), bias.to(CUDA), activation="silu")
+    grad_x, = torch.autograd.grad(y, x, dy)
+    leaf = image.double().requires_grad_(True)
+    want = ref.group_norm(leaf, groups, weight, bias, activation="silu")
+    want_x, = torch.autograd.grad(want, leaf, grad.double())
+    bounds = Bounds(image, groups, weight, bias, 1e-5, "silu", None, grad)
+    for at in (0, copies - 1):
+        part = slice(at, at + 1)
+        within(y.view(copies, pixels, channels)[part], want.detach(), long * bounds.y, dtype)
+        within(grad_x.view(copies, pixels, channels)[part], want_x, long * bounds.x, dtype)
+    del x, dy, y, grad_x
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("extra", [1, 2, 4, 8])
 def test_two_passes_over_channel_slices(extra, dtype):
