@@ -14,25 +14,29 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// A thread has kCounters counters of eight elements each: all their loads are issued first, and the
-// rounds of the generator run while they are under way (with one counter too few bytes are: the
-// gradient of eight 512 x 512 x 64 bfloat16 images took 111 us, with two 98 us). `Wide` tensors
-// are read and written in 16-byte words; the others, whose address is not a multiple of 16, and the
-// last elements one by one.
-constexpr int kCounters = 2;
+// A thread has Counters counters of eight elements each: all their loads are issued first, and the
+// rounds of the generator run while they are under way. Bound by memory: with a residual eight 512 x
+// 512 x 64 bfloat16 images take 122 us, 6.6 TB/s. `Wide` tensors are read and written in 16-byte
+// words; the others, whose address is not a multiple of 16, and the last elements one by one.
+//
+// With two counters bytes enough are under way but for large tensors of 2 bytes an element and no
+// residual, which take four: the images' gradient takes 111, 98 and 93 us with one, two and four.
+// At 32 MB two and four are even (14.6 us), at 8 MB four are slower (6.4 us instead of 5.6), and
+// float32 is slower with four at every size (48 MB: 20.2 us instead of 17.9).
+constexpr long long kManyBytes = 64LL << 20;
 
-template <typename T, bool Wide, bool Residual>
+template <typename T, bool Wide, bool Residual, int Counters>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(
     const T* __restrict__ x, const T* __restrict__ residual, long long count, DropKey key,
     T* __restrict__ y) {
   constexpr int kPer = 16 / static_cast<int>(sizeof(T));  // elements of a 16-byte word
   constexpr int kWords = 8 / kPer;
   const long long base =
-      (blockIdx.x * static_cast<long long>(kThreads * kCounters) + threadIdx.x) * 8;
+      (blockIdx.x * static_cast<long long>(kThreads * Counters) + threadIdx.x) * 8;
   const unsigned long long seed = load_seed(key);
-  uint4 a[kCounters][kWords], b[kCounters][kWords];
+  uint4 a[Counters][kWords], b[Counters][kWords];
 #pragma unroll
-  for (int n = 0; n < kCounters; ++n) {
+  for (int n = 0; n < Counters; ++n) {
     const long long first = base + n * kThreads * 8;
     if constexpr (Wide) {
       if (first + 8 <= count) {
@@ -45,7 +49,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(
     }
   }
 #pragma unroll
-  for (int n = 0; n < kCounters; ++n) {
+  for (int n = 0; n < Counters; ++n) {
     const long long first = base + n * kThreads * 8;
     if (first >= count) return;
     const bool whole = Wide && first + 8 <= count;
@@ -95,16 +99,21 @@ int run(const void* x, const void* residual, long long count, const DropKey& key
         cudaStream_t stream) {
   const bool wide = aligned_to(x, 16) && aligned_to(y, 16) &&
                     (residual == nullptr || aligned_to(residual, 16));
-  const unsigned int blocks = blocks_for((count + 7) / 8, kThreads * kCounters);
-  auto launch = [&](auto kernel) {
-    kernel<<<blocks, kThreads, 0, stream>>>(static_cast<const T*>(x),
-                                            static_cast<const T*>(residual), count, key,
-                                            static_cast<T*>(y));
+  auto launch = [&](auto kernel, int counters) {
+    kernel<<<blocks_for((count + 7) / 8, kThreads * counters), kThreads, 0, stream>>>(
+        static_cast<const T*>(x), static_cast<const T*>(residual), count, key, static_cast<T*>(y));
   };
-  if (residual != nullptr)
-    wide ? launch(dropout_kernel<T, true, true>) : launch(dropout_kernel<T, false, true>);
-  else
-    wide ? launch(dropout_kernel<T, true, false>) : launch(dropout_kernel<T, false, false>);
+  if (residual != nullptr) {
+    wide ? launch(dropout_kernel<T, true, true, 2>, 2) : launch(dropout_kernel<T, false, true, 2>, 2);
+    return launch_status();
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (wide && count * 2 >= kManyBytes) {
+      launch(dropout_kernel<T, true, false, 4>, 4);
+      return launch_status();
+    }
+  }
+  wide ? launch(dropout_kernel<T, true, false, 2>, 2) : launch(dropout_kernel<T, false, false, 2>, 2);
   return launch_status();
 }
 
@@ -124,7 +133,7 @@ extern "C" int dr_dropout(const void* x, const void* residual, int64_t count, in
       !aligned_to(residual, size) || !aligned_to(seed, sizeof(int64_t)))
     return DR_ERR_INVALID_ARGUMENT;
   // At most 2^31 - 1 blocks.
-  if (count > 8LL * kThreads * kCounters * 0x7FFFFFFF) return DR_ERR_TOO_LARGE;
+  if (count > 8LL * kThreads * 2 * 0x7FFFFFFF) return DR_ERR_TOO_LARGE;
   const DropKey key = drop_key(seed, seed_value, layer, threshold);
   switch (dtype) {
     case DR_FLOAT32:

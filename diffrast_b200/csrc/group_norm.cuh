@@ -335,7 +335,7 @@ __device__ __forceinline__ P load_slot(unsigned int at) {
 // A thread's rows on their way to it: it copies its own vectors (of Images images) into its own
 // slots of shared memory, Stages rows ahead of the one it works on. No slot is shared, so the
 // copies need no barriers, and they hold no registers: with batches of loads in registers instead,
-// the sums of the backward pass read memory at 1.9 TB/s, for want of bytes under way.
+// the sums of the backward pass read memory at 1.9 TB/s, for want of bytes under way; so, at 5.0.
 template <typename T, int V, int Images, int Stages>
 struct RowRing {
   using P = Packed<T, V>;
@@ -452,9 +452,10 @@ struct Affine {
 
 // The kernels that join the blocks' sums: a block has a run of whole groups of at most 8 channels
 // together, or one group of at most 32, by as many lanes as it has threads for (with 32 channels to
-// every block, two blocks read all the parts of 64 channels, in 10 us; they are the only work
-// between the two passes). Of wider groups it has 32 channels, and a second kernel joins the
-// channels of each group (one block for a group of 256 channels took 45 us).
+// every block, two blocks read all the parts of 64 channels, in 10 us instead of 7; they are the
+// only work between the two passes). Of wider groups it has 32 channels, and a second kernel joins the
+// channels of each group (the norm of 301 x 301 x 256 in one group takes 61 us so, 116 us with one
+// block for the group).
 constexpr int kJoinThreads = 1024;
 constexpr int kJoinChannels = 32;
 
@@ -462,6 +463,9 @@ __host__ __device__ inline int join_channels(int group_channels) {
   if (group_channels > kJoinChannels) return kJoinChannels;
   return group_channels > 8 ? group_channels : 8 / group_channels * group_channels;
 }
+
+// log2 of the threads in a row of such a block, at least one for each of its `run` channels.
+__host__ __device__ inline int join_shift(int run) { return run > 16 ? 5 : run > 8 ? 4 : 3; }
 
 struct JoinPlace {
   int view, channel, channels;     // first channel, and channels
@@ -472,9 +476,9 @@ struct JoinPlace {
     view = view0 + blockIdx.y;
     channel = blockIdx.x * run;
     channels = min(run, s.channels - channel);
-    const int shift = run > 16 ? 5 : run > 8 ? 4 : 3;
+    const int shift = join_shift(run);
     width = 1 << shift;
-    lanes = kJoinThreads >> shift;
+    lanes = blockDim.x >> shift;
     x = threadIdx.x & (width - 1);
     y = threadIdx.x >> shift;
   }
@@ -487,7 +491,7 @@ struct JoinPlace {
 // each channel from their shared memory, and finishes its rows from its own: one launch, and the
 // image is read once and written once. (Larger teams, over all processors and through memory, had
 // some 18 us from one slab's copies to its results, and too little shared memory to cover that with
-// other slabs: 171 us for the 78 us of the two passes on four images of 512 x 512 x 64.)
+// other slabs: 171 us for the 74 us of the two passes on four images of 512 x 512 x 64.)
 
 constexpr int kMostCluster = 16;
 
@@ -736,10 +740,16 @@ inline bool too_large(long long batch, long long pixels, long long stride) {
          (batch > 0 && pixels > 0 && stride > kMost / batch / pixels);
 }
 
-// Blocks for each view of the kernels that join the blocks' sums (see JoinPlace).
+// Blocks for each view of the kernels that join the blocks' sums (see JoinPlace), and their
+// threads: all or, where a view has few chunks, a warp for each channel (of 64 views of 512 KB each
+// the forward pass takes 26 us so and 37 us with 1024 threads to every block).
 inline unsigned int join_runs(const NormShape& s) {
   const int run = join_channels(s.group_channels);
   return static_cast<unsigned int>((s.channels + run - 1) / run);
+}
+inline unsigned int join_threads(const NormShape& s) {
+  const int width = 1 << join_shift(join_channels(s.group_channels));
+  return static_cast<long long>(s.chunks) * width <= kJoinThreads ? 32 * width : kJoinThreads;
 }
 
 constexpr int kMostShared = 220 * 1024;  // dynamic shared memory of a block
@@ -747,15 +757,19 @@ constexpr int kMostShared = 220 * 1024;  // dynamic shared memory of a block
 // Blocks of a processor that the kernels' registers allow, forward and backward.
 constexpr int kResident[2] = {4, 3};
 
-// Largest image that is taken in clusters. With the two passes, an image of 32 KB takes 8.0 us
-// forward and 6.9 us backward, in clusters 6.4 and 4.4 us, and two launches less; at 2 MB both
-// take 11 and 10 us, and at 8 MB the passes are a third faster.
-constexpr long long kClusterBytes = 1LL << 20;
+// Largest view that is taken in clusters. One view of 32 KB (16 x 16 x 64 bfloat16) takes 5.2 us
+// forward and 4.6 us backward in clusters, 6.2 and 7.0 us in two passes, and 1024 of them 24 and 37
+// us against 48 and 58 us; four of 256 KB 7.3 and 8.1 us against 7.8 and 9.3 us, and 256 of them 42
+// and 69 us against 46 and 70 us. At 512 KB neither is ahead (four: 8.7 and 10.2 us against 8.3 and
+// 10.6 us; 256: 78 and 132 us against 78 and 118 us).
+constexpr long long kClusterBytes = 1LL << 18;
 
 // The plan of a call in clusters, or false where none fits: tiles of whole groups, and blocks to a
 // cluster, by the estimated time in microseconds. A block's own is what is fixed (2, or 3 with a
-// cluster), its bytes at a processor's share of the memory, and its rows' instructions; the blocks
-// of a processor overlap, as many as its registers and shared memory hold.
+// cluster, and with clusters the start of all blocks of a wave: sixteen views of 128 KB take 10.7 us
+// in 512 blocks of clusters and 6.5 us in 128 without), its bytes at a processor's share of the
+// memory, and its rows' instructions, or the cache lines that its warps' copies touch if those are
+// slower; the blocks of a processor overlap, as many as its registers and shared memory hold.
 inline bool plan_clusters(NormShape& s, ClusterPlan& t, const NormVector& v, long long batch,
                           long long pixels, int channels, int groups, int dtype,
                           long long x_stride, long long grad_stride, int images, int processors) {
@@ -765,7 +779,7 @@ inline bool plan_clusters(NormShape& s, ClusterPlan& t, const NormVector& v, lon
   const int unit = v.fold > 1 ? row_cols : d / greatest_divisor(d, v.vec);
   const long long rows = pixels / v.fold;
   double best = 1e30;
-  if (unit > most_cols || batch * pixels * channels * size > kClusterBytes) return false;
+  if (unit > most_cols || pixels * channels * size > kClusterBytes) return false;
   for (int cols = unit; cols <= std::min(row_cols, most_cols); cols *= 2) {
     const long long tiles = (row_cols + cols - 1) / cols;
     const long long slabs = batch * tiles;
@@ -784,9 +798,14 @@ inline bool plan_clusters(NormShape& s, ClusterPlan& t, const NormVector& v, lon
       const double narrow = tiles == 1 || width * size >= 64 ? 1.0 : width * size >= 32 ? 1.3 : 2.0;
       const double move =
           static_cast<double>(block_rows) * width * size * (images + 1) * narrow / 43.5e3;
-      const double work = static_cast<double>(lane_rows) * (images == 1 ? 0.16 : 0.31) + 1.0;
-      const double fixed = team == 1 ? 2.0 : team <= 8 ? 3.0 : 3.5;
-      const double each = static_cast<double>(slabs * team) / processors;
+      const double lines = 8.0 * (cols < 8 ? 32.0 / cols : 4.0) * (images + 1) / 1.9e3;
+      const double row = std::max(images == 1 ? 0.16 : 0.31, lines);
+      const double work = static_cast<double>(lane_rows) * row + 1.0;
+      const double blocks = static_cast<double>(slabs * team);
+      const double fixed =
+          team == 1 ? 2.0
+                    : (team <= 8 ? 3.0 : 3.5) + 0.01 * std::min(blocks, processors * here);
+      const double each = blocks / processors;
       const double waves = std::ceil(each / here);
       const double together = std::min(here, std::ceil(each));
       const double time =
@@ -861,19 +880,18 @@ inline int views_at_once(long long batch) {
 }
 
 // The plan of a call in passes over memory. A block's start and the join of its sums cost as much
-// as 16 rows of its threads, so a block has 16 rows of them (64 KB of 16-byte vectors), in the
-// forward pass 32 where the blocks fill the processors many times over; blocks fill the processors
-// evenly, up to `resident` to each, or several times over. Four images of 512 x 512 x 64 bfloat16
-// take 91, 82 and 78 us forward with 8, 16 and 32 rows, and 116, 114 and 122 us backward; eight of
-// 128 x 128 x 256 take 83, 76 and 82 us forward.
+// as 16 rows of its threads, and with long blocks the last ones run alone, so a block has about 24
+// rows of them (96 KB of 16-byte vectors); blocks fill the processors evenly, up to `resident` to
+// each, or several times over. Four images of 512 x 512 x 64 bfloat16 take 76, 74, 78 and 91 us
+// forward with 16, 24, 48 and 112 rows, and 114, 115, 120 and 126 us backward; eight of 128 x 128 x
+// 256 with dropout take 65, 65, 70 and 112 us, and 96, 96, 92 and 148 us.
 inline void plan_passes(NormShape& s, const NormVector& v, long long batch, long long pixels,
                         int channels, int groups, int dtype, long long x_stride,
                         long long grad_stride, int images, int processors) {
   const int size = dtype_bytes(dtype), resident = kResident[images - 1];
   const long long bytes = pixels * channels * size * views_at_once(batch);
   const long long row = static_cast<long long>(kNormThreads) * v.vec * size;
-  const long long waves = bytes / (16 * row * resident * processors);
-  const long long chunk = (waves >= 3 && images == 1 ? 32 : 16) * row;
+  const long long chunk = 24 * row;
   const long long each = (bytes + processors * chunk / 2) / (processors * chunk);
   const long long blocks =
       processors * (each <= resident ? std::max(1LL, each)

@@ -170,9 +170,11 @@ def test_two_passes_with_dropout_and_parameters_of_each_view(shape, groups, dtyp
 
 
 @pytest.mark.parametrize("shape, groups, dropout", [
-    ((70001, 5, 6), 2, 0.0), ((131077, 7, 7), 1, 0.3), ((66000, 1, 8), 2, 0.3)])
-def test_more_views_than_one_launch_takes(shape, groups, dropout):
-    """A launch takes 65535 views; gradients of shared parameters are sums over all of them."""
+    ((70001, 5, 6), 2, 0.0), ((131077, 7, 7), 1, 0.3), ((66000, 1, 8), 2, 0.3), ((66000, 1, 258), 1, 0.3),
+    ((300, 32, 32, 32), 4, 0.0), ((90, 40, 50, 64), 2, 0.3), ((1000, 4, 4, 256), 32, 0.0)])
+def test_many_views(shape, groups, dropout):
+    """A launch takes 65535 views (of 258 channels in one group, too wide for clusters of blocks);
+    gradients of shared parameters are sums over all views."""
     x = features(shape, torch.float16, 5)
     compare(x, groups, *params(shape[-1], 6), activation="silu", dropout=dropout, seed=4)
 
