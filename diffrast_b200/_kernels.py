@@ -804,7 +804,7 @@ def _contiguous_like(t: Tensor) -> Tensor:
 
 
 @functools.lru_cache(maxsize=256)
-def _norm_workspace_bytes(batch, pixels, channels, groups, dtype, backward) -> int:
+def _norm_workspace_bytes(device, batch, pixels, channels, groups, dtype, backward) -> int:
     return N.lib().dr_group_norm_workspace_bytes(batch, pixels, channels, groups, dtype, backward)
 
 
@@ -827,7 +827,7 @@ def group_norm_fwd(x: Tensor, groups: int, weight: Tensor | None, bias: Tensor |
     dtype = N.FEATURE_DTYPES[x.dtype]
     y = _contiguous_like(x)
     state = x.new_empty(batch * (3 * channels + groups), dtype=torch.float32)
-    nbytes = _norm_workspace_bytes(batch, pixels, channels, groups, dtype, 0)
+    nbytes = _norm_workspace_bytes(x.device.index, batch, pixels, channels, groups, dtype, 0)
     work = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     N.check(
         N.lib().dr_group_norm_fwd(x.data_ptr(), stride, dtype, batch, pixels, channels, groups,
@@ -855,7 +855,7 @@ def group_norm_bwd(x: Tensor, grad_y: Tensor, groups: int, weight: Tensor | None
     grad_x = _contiguous_like(x) if need_x else None
     grad_w = None if weight is None else torch.empty_like(weight)
     grad_b = None if bias is None else torch.empty_like(bias)
-    nbytes = _norm_workspace_bytes(batch, pixels, channels, groups, dtype, 1)
+    nbytes = _norm_workspace_bytes(x.device.index, batch, pixels, channels, groups, dtype, 1)
     work = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     N.check(
         N.lib().dr_group_norm_bwd(x.data_ptr(), stride, grad_y.data_ptr(), grad_stride, dtype,
