@@ -14,6 +14,8 @@ Bounds, with u = 2^-24 and everything per group, in units that the reference sup
 - the result is rounded once: half a unit in the last place of its type.
 """
 
+import concurrent.futures
+
 import pytest
 import torch
 
@@ -417,6 +419,56 @@ def test_inference_tensors_pass_and_give_the_same():
 def training_step(x, w, b, seed, g):
     y = dr.group_norm(x, 4, w, b, activation="silu", dropout=0.2, seed=seed)
     return [y.detach(), *torch.autograd.grad(y, (x, w, b), g)]
+
+
+@pytest.mark.parametrize("dtype, width", [(torch.float32, 16), (torch.float32, 17), (torch.bfloat16, 32),
+                                          (torch.bfloat16, 33)])
+def test_views_at_the_size_where_the_passes_change(dtype, width):
+    """Views of 256 KB and just above."""
+    x = features((5, 64, width, 64), dtype, 31)
+    compare(x, 8, *params(64, 32), activation="silu", dropout=0.2, seed=33)
+
+
+def test_one_tensor_in_two_places():
+    x = features((2, 9, 11, 16), torch.float32, 41)
+    p = params(16, 42)[0]
+    gx, gp = x.to(CUDA).requires_grad_(True), p.to(CUDA).requires_grad_(True)
+    y = dr.group_norm(gx, 4, gp, gp, activation="relu")
+    grads = torch.autograd.grad(y.square().sum(), (gx, gp))
+    two = [p.to(CUDA).requires_grad_(True) for _ in range(2)]
+    want = dr.group_norm(gx, 4, *two, activation="relu")
+    apart = torch.autograd.grad(want.square().sum(), (gx, *two))
+    assert torch.equal(y, want) and torch.equal(grads[0], apart[0])
+    assert torch.equal(grads[1], apart[1] + apart[2])
+    z = dr.dropout(gx, 0.5, 7, residual=gx)
+    keep = ref.keep_mask(x.numel(), 0.5, 7).view(x.shape).to(CUDA)
+    assert torch.equal(z, gx + 2 * gx * keep)
+    assert torch.equal(torch.autograd.grad(z.sum(), gx)[0], 1 + 2.0 * keep)
+
+
+def test_threads_with_streams_of_their_own():
+    """Calls of four threads at once, in clusters and in passes, give what one thread gets."""
+    inputs = [features(shape, torch.bfloat16, i).to(CUDA) for i, shape in
+              enumerate([(2, 16, 16, 64), (2, 130, 100, 64), (3, 101, 103, 36), (40, 32, 32, 24)])]
+    grads = [torch.randn_like(x) for x in inputs]
+
+    def step(x, grad):
+        leaf = x.clone().requires_grad_(True)
+        y = dr.group_norm(leaf, 4, activation="silu", dropout=0.1, seed=5)
+        return y.detach(), torch.autograd.grad(y, leaf, grad)[0]
+
+    want = [step(x, g) for x, g in zip(inputs, grads)]
+    torch.cuda.synchronize()
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got = [step(inputs[i], grads[i]) for _ in range(10)]
+        stream.synchronize()
+        return all(torch.equal(a, b) for pair in got for a, b in zip(pair, want[i]))
+
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, range(4)))
 
 
 @pytest.mark.parametrize("shape", [(2, 9, 9, 32), (2, 200, 180, 32), (3, 101, 103, 36)])
