@@ -16,6 +16,7 @@ from typing import Literal, SupportsFloat, get_args
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from diffrast_b200 import _functions as F
 from diffrast_b200 import _kernels as K
@@ -685,8 +686,8 @@ def group_norm(
     same bits, gradients included.
 
     Differentiable in ``x``, ``weight`` and ``bias``; the backward pass computes activation and
-    mask again from ``x``. A group with NaN or infinite values is NaN throughout. Not part of
-    diffrast's API.
+    mask again from ``x``. Forward-mode derivatives raise ``NotImplementedError``. A group with NaN
+    or infinite values is NaN throughout. Not part of diffrast's API.
     """
     channels = _check_features(x, "x")
     if isinstance(groups, bool) or not isinstance(groups, int):
@@ -734,7 +735,8 @@ def dropout(
     Calls of one step are told apart by ``layer`` (below 2**32). ``p`` in ``[0, 1)`` is rounded to
     a multiple of 2**-16 (at most 65535 of them), and the scale is that of the rounded
     probability. A dropped element is 0 whatever its value. Differentiable in ``x`` and
-    ``residual``. Not part of diffrast's API.
+    ``residual`` (forward-mode derivatives raise ``NotImplementedError``). Not part of diffrast's
+    API.
     """
     _check_features(x, "x", ndim=0)
     if seed is None:
@@ -770,10 +772,17 @@ def _on_device(t: Tensor):
 
 
 def _wants_grad(*tensors) -> bool:
-    if not torch.is_grad_enabled():
-        return False
+    """Whether a call has to go through autograd: an input requires a gradient, or carries a
+    forward-mode tangent, which the autograd functions refuse and a direct call would drop."""
+    grad = torch.is_grad_enabled()
+    # Without an open level, the usual case, no tensor carries a tangent.
+    forward = getattr(forward_ad, "_current_level", 0) >= 0
     for t in tensors:
-        if t is not None and t.requires_grad:
+        if t is None:
+            continue
+        if grad and t.requires_grad:
+            return True
+        if forward and forward_ad.unpack_dual(t).tangent is not None:
             return True
     return False
 
