@@ -13,6 +13,7 @@ from typing import NamedTuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from diffrast_b200 import _kernels as K
 
@@ -31,6 +32,15 @@ def first_order(op: str):
         return guarded
 
     return decorate
+
+
+def _refuse_tangent(op: str, grad: Tensor) -> None:
+    """Refuses an upstream gradient with a forward-mode tangent, which a kernel would drop."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(grad).tangent is not None:
+        raise NotImplementedError(
+            f"{op} in diffrast_b200 has no forward-mode derivatives, but the gradient given to its "
+            "backward pass carries a tangent."
+        )
 
 
 def _saveable(t: Tensor | None) -> Tensor | None:
@@ -723,6 +733,7 @@ class GroupNorm(torch.autograd.Function):
     @staticmethod
     @first_order("group_norm")
     def backward(ctx, grad_out):
+        _refuse_tangent("group_norm", grad_out)
         x, weight, bias, seed, state = ctx.saved_tensors
         groups, _, activation, drop = ctx.options
         need_x, need_w, need_b, _, _ = ctx.needs_input_grad
@@ -745,7 +756,10 @@ class Dropout(torch.autograd.Function):
     def backward(ctx, grad_out):
         (seed,) = ctx.saved_tensors
         need_x, need_residual, _, _ = ctx.needs_input_grad
-        grad_x = K.dropout(grad_out.contiguous(), None, ctx.drop, seed) if need_x else None
+        grad_x = None
+        if need_x:
+            _refuse_tangent("dropout", grad_out)
+            grad_x = K.dropout(grad_out.contiguous(), None, ctx.drop, seed)
         return grad_x, grad_out if need_residual else None, None, None
 
 

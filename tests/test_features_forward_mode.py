@@ -53,3 +53,25 @@ def test_calls_without_tangents_pass_beside_them(stand_ins, name):
         leaf = primal.clone().requires_grad_(True)
         assert call(leaf).requires_grad
     assert call(primal).shape == X.shape
+
+
+def gradient(monkeypatch, name):
+    """The gradient, for an upstream gradient that carries a tangent."""
+    monkeypatch.setattr(K, "group_norm_bwd", lambda x, g, *rest: (g.detach().clone(), None, None))
+    primal, call = CALLS[name]
+    leaf = primal.clone().requires_grad_(True)
+    y = call(leaf)
+    return torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))[0]
+
+
+@pytest.mark.parametrize("name", ["norm x", "norm x alone", "dropout x", "dropout x beside residual"])
+def test_tangents_of_the_upstream_gradient_are_refused(stand_ins, monkeypatch, name):
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        gradient(monkeypatch, name)
+
+
+def test_the_residuals_gradient_keeps_its_tangent(stand_ins, monkeypatch):
+    """It is the upstream gradient itself."""
+    with forward_ad.dual_level():
+        tangent = forward_ad.unpack_dual(gradient(monkeypatch, "dropout residual")).tangent
+    assert torch.equal(tangent, torch.ones_like(X))
