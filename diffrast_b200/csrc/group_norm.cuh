@@ -127,12 +127,12 @@ __device__ __forceinline__ float2 exponentials(float2 z) {
   return e;
 }
 
-// q / (1 + exp(-z)).
+// q / (1 + exp(-z)). The reciprocal comes first: q times a neighbour's exponential could overflow.
 __device__ __forceinline__ float2 times_sigmoid(float2 q, float2 z) {
   const float2 e = add2(exponentials(z), both(1.0f));
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e.x * e.y));
-  return mul2(make_float2(q.x * e.y, q.y * e.x), both(r));
+  return mul2(q, mul2(make_float2(e.y, e.x), both(r)));
 }
 
 // The activations: SiLU, or a clamp from below that is the identity with bound -infinity and ReLU

@@ -82,3 +82,18 @@ def test_slope_is_exact_to_rounding_at_any_size(layout, seed):
         want, want_slope = silu_and_slope(z[:slope.numel()])
         within(y[:, want > 0], want[want > 0], 8 * U * want[want > 0] + 2 * U)
         within(slope, want_slope, 12 * U)
+
+
+FAR = torch.logspace(19, 38, 32, dtype=torch.float64)
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("seed", range(3))
+def test_large_values_beside_very_negative_ones(layout, seed):
+    """Neighbours share a reciprocal, and no product of theirs may pass float32's range."""
+    z = torch.cat([FAR, -torch.logspace(1.5, 2, 32, dtype=torch.float64)]).float()
+    z = z[torch.randperm(64, generator=torch.Generator().manual_seed(seed))]
+    y, slope = run(layout, z)
+    want, want_slope = silu_and_slope(z[:slope.numel()])
+    within(y[:, want > 0], want[want > 0], 8 * U * want[want > 0])
+    within(slope, want_slope, 12 * U)
