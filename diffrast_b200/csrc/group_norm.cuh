@@ -113,47 +113,54 @@ __device__ __forceinline__ void store_param(void* data, int dtype, long long i, 
     static_cast<__nv_bfloat16*>(data)[i] = __float2bfloat16_rn(v);
 }
 
-// exp(-z) of a pair, for 1 / (1 + exp(-z)). The special-function unit gives 16 results a clock and processor,
-// and with an exponential and a reciprocal for each value it was the busiest unit (74% of its rate
-// in the second pass), so the two values share one reciprocal: 1 / a = b / (a b). Exponents are cut
-// at 2^63, so that the product stays finite: below z = -43.7 the result is 2^-63 instead of less.
-// Exponential and reciprocal are within two units in the last place of float32. A NaN gives 2^-63
-// (the cut drops it), and its product with z is NaN again.
-__device__ __forceinline__ float2 exponentials(float2 z) {
-  const float2 t = mul2(z, both(-1.4426950408889634f));
-  float2 e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(fminf(t.x, 63.0f)));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(fminf(t.y, 63.0f)));
+__device__ __forceinline__ float power_of_two(float t) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
   return e;
 }
-
-// q / (1 + exp(-z)). The reciprocal comes first: q times a neighbour's exponential could overflow.
-__device__ __forceinline__ float2 times_sigmoid(float2 q, float2 z) {
-  const float2 e = add2(exponentials(z), both(1.0f));
+__device__ __forceinline__ float reciprocal(float v) {
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e.x * e.y));
-  return mul2(q, mul2(make_float2(e.y, e.x), both(r)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
 
-// The activations: SiLU, or a clamp from below that is the identity with bound -infinity and ReLU
-// with bound 0. The comparisons are written so that NaN passes, as it does through both.
+// exp(-z) of a pair. Off by (1.23 |z| + 4) u relative (u = 2^-24), mostly from rounding z / ln 2, which
+// moves a function of z like a change of z by as much. Below 2^-126 it is 0.
+__device__ __forceinline__ float2 exp_minus(float2 z) {
+  const float2 t = mul2(z, both(-1.4426950408889634f));
+  return make_float2(power_of_two(t.x), power_of_two(t.y));
+}
+
+// 1 / d of a pair. The special-function unit gives 16 results a clock and processor, and with an
+// exponential and a reciprocal for each value it is the busiest unit of the second pass (74% of its
+// rate). One reciprocal for both values, 1 / a = b / (a b), takes four images of 512 x 512 x 64
+// bfloat16 from 73 to 70 us forward and nothing off the backward pass, but their product leaves the
+// range of float32 with exp(-z) above 2^63, a NaN spoils its neighbour, and what it takes to tell
+// (a test of each pair: 79 us; of each vector: 74; all rows again after a test at their end: 72, in
+// registers that the passes do not have) gives the time back.
+__device__ __forceinline__ float2 reciprocals(float2 d) {
+  return make_float2(reciprocal(d.x), reciprocal(d.y));
+}
+
+// The activations: SiLU, z / (1 + exp(-z)), or a clamp from below that is the identity with bound
+// -infinity and ReLU with bound 0. The comparisons are written so that NaN passes, as it does
+// through all three.
 template <bool Silu>
 __device__ __forceinline__ float2 activate(float2 z, float bound) {
-  if (Silu) return times_sigmoid(z, z);
+  if (Silu) return mul2(z, reciprocals(add2(exp_minus(z), both(1.0f))));
   return make_float2(z.x <= bound ? bound : z.x, z.y <= bound ? bound : z.y);
 }
 
-// q times the derivative at z: s (1 + z (1 - s)) for SiLU. ReLU's is 0 at 0. The part 1 - s is formed
-// from the exponential, as exp(-z) s: the difference from an s that is a few units off is wrong by as
-// many, and z multiplies them (with z = 1000 the slope came out 6e-5 from 1).
+// q times the derivative at z: s (1 + z (1 - s)) for SiLU, s the sigmoid. ReLU's is 0 at 0.
+//
+// 1 - s is formed as exp(-z) s: the difference from an s that is a few units off is wrong by as many,
+// and z multiplies them (with z = 1000 the slope came out 6e-5 from 1). Where exp(-z) passes 2^126, s
+// is 0 or next to it; the cut keeps 0 times infinity out of the product.
 template <bool Silu>
 __device__ __forceinline__ float2 activate_grad(float2 q, float2 z, float bound) {
   if (Silu) {
-    const float2 e = exponentials(z), d = add2(e, both(1.0f));
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d.x * d.y));
-    const float2 s = mul2(make_float2(d.y, d.x), both(r));
-    const float2 rest = mul2(e, s);
+    const float2 e = exp_minus(z), s = reciprocals(add2(e, both(1.0f)));
+    const float2 rest = mul2(make_float2(fminf(e.x, 0x1p126f), fminf(e.y, 0x1p126f)), s);
     return mul2(q, mul2(s, fma2(z, rest, both(1.0f))));
   }
   return make_float2(z.x <= bound ? 0.0f : q.x, z.y <= bound ? 0.0f : q.y);

@@ -97,3 +97,22 @@ def test_large_values_beside_very_negative_ones(layout, seed):
     want, want_slope = silu_and_slope(z[:slope.numel()])
     within(y[:, want > 0], want[want > 0], 8 * U * want[want > 0])
     within(slope, want_slope, 12 * U)
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("seed", range(3))
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_very_negative_values_go_to_zero(layout, seed, dtype):
+    """SiLU and its slope below zero to the digits of their own size, down to the smallest float32,
+    whatever the neighbours; the slope's factor 1 + z (1 - s) adds 7 u there."""
+    below = [torch.linspace(20, 90, 32, dtype=torch.float64), torch.logspace(1.9, 38.5, 32, dtype=torch.float64)]
+    for magnitudes in below:
+        z = torch.cat([-magnitudes, MODERATE if seed == 0 else -below[0] if seed == 1 else FAR]).float()
+        z = z[torch.randperm(64, generator=torch.Generator().manual_seed(seed))]
+        y, slope = run(layout, z, dtype)
+        z = z[:slope.numel()].double()
+        want, want_slope = silu_and_slope(z)
+        near = z.abs().clamp(max=128)
+        rounded = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+        within(y[:, z < 0], want[z < 0], ((10 + 1.25 * near) * U * want.abs() + rounded * want.abs() + FLUSH)[z < 0])
+        within(slope[z < -20], want_slope[z < -20], ((20 + 1.25 * near) * U * want_slope.abs() + FLUSH)[z < -20])
