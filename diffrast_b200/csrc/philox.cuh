@@ -38,8 +38,20 @@ inline DropKey drop_key(const int64_t* seed, int64_t seed_value, int64_t layer,
           static_cast<float>(65536.0 / (65536 - threshold))};
 }
 
+// The load carries its test with it as one instruction's predicate: written as a load under an if,
+// it could be moved before the test, and `seed` is NULL with every seed that is a number.
 __device__ __forceinline__ unsigned long long load_seed(const DropKey& key) {
-  return key.seed != nullptr ? static_cast<unsigned long long>(*key.seed) : key.value;
+  unsigned long long seed = key.value;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred given;\n\t"
+      "setp.ne.u64 given, %1, 0;\n\t"
+      "@given ld.global.u64 %0, [%1];\n\t"
+      "}"
+      : "+l"(seed)
+      : "l"(key.seed)
+      : "memory");
+  return seed;
 }
 
 __device__ __forceinline__ uint4 philox(unsigned long long block, unsigned int layer,
