@@ -169,7 +169,7 @@ __device__ __forceinline__ float2 activate_grad(float2 q, float2 z, float bound)
 // Running moments of V channels. Values are summed as differences from the thread's first value
 // k: with n values, sum (x - k)^2 is at most n times their sum of squared deviations from their
 // mean (k is one of them), so rounding grows by no more than n, whatever the offset of the data.
-// Blocks give a thread at most kThreadRows rows.
+// Plans give a thread at most kThreadRows rows.
 constexpr int kThreadRows = 128;
 
 template <int V>
@@ -804,7 +804,7 @@ inline bool plan_clusters(NormShape& s, ClusterPlan& t, const NormVector& v, lon
       const long long block_rows = (rows + team - 1) / team;
       const long long lane_rows = (block_rows + lanes - 1) / lanes;
       const long long shared = lane_rows * slot + extra;
-      if (shared > kMostShared || slabs * team > 0x7FFFFFFF) continue;
+      if (shared > kMostShared || slabs * team > 0x7FFFFFFF || lane_rows > kThreadRows) continue;
       const double here = static_cast<double>(
           std::min<long long>(kResident[images - 1], 228 * 1024 / (shared + 2048)));
       const double narrow = tiles == 1 || width * size >= 64 ? 1.0 : width * size >= 32 ? 1.3 : 2.0;
