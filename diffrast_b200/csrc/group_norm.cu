@@ -143,19 +143,17 @@ __global__ void __launch_bounds__(kJoinThreads) norm_join_kernel(
            (chunk == 0 ? static_cast<float>(s.leftover) : 0.0f);
   };
   // This lane's chunks of channel x.
-  Moment m = {0.0f, 0.0f, 0.0f};
+  LongMoment own;
   if (p.x < p.channels) {
 #pragma unroll 8
-    for (int i = p.y; i < s.chunks; i += p.lanes) {
-      const float2 v = parts[static_cast<long long>(i) * s.channels + p.x];
-      m.join({count_of(i), v.x, v.y});
-    }
+    for (int i = p.y; i < s.chunks; i += p.lanes)
+      own.join(count_of(i), parts[static_cast<long long>(i) * s.channels + p.x]);
   }
-  entry[p.y * (p.width + 1) + p.x] = make_float2(m.mean, m.squares);
+  entry[p.y * (p.width + 1) + p.x] = make_float2(own.mean.sum, own.squares.sum);
   __syncthreads();
   // A warp a channel, from its lanes; lane i has ceil((chunks - i) / lanes) chunks.
   for (int c = warp; c < p.channels; c += blockDim.x / 32) {
-    m = {0.0f, 0.0f, 0.0f};
+    Moment m = {0.0f, 0.0f, 0.0f};
     for (int i = lane; i < p.lanes; i += 32) {
       const float2 v = entry[i * (p.width + 1) + c];
       const int own = i < s.chunks ? (s.chunks - i + p.lanes - 1) / p.lanes : 0;

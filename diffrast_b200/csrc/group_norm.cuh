@@ -253,6 +253,35 @@ struct Moment {
   }
 };
 
+// A sum with what its roundings have left out (Kahan's compensated summation), for the lanes of the
+// joins, which may add thousands of chunks one after the other: in plain 32 bits a sum of equal terms
+// over 1.5 GB was 250 units in the last place off. (Sums in 64 bits cost the join of a view of 268 MB
+// 3 us, most of it for the conversions.)
+struct LongSum {
+  float sum = 0.0f, lost = 0.0f;
+
+  __device__ __forceinline__ void add(float v) {
+    const float term = v - lost, total = sum + term;
+    // An infinite sum stays infinite.
+    lost = fabsf(total) < __int_as_float(0x7f800000) ? (total - sum) - term : 0.0f;
+    sum = total;
+  }
+};
+
+// The moments of a lane's chunks: Moment::join with long sums.
+struct LongMoment {
+  float n = 0.0f;
+  LongSum mean, squares;
+
+  __device__ __forceinline__ void join(float count, float2 chunk) {
+    const float share = count > 0.0f ? __fdividef(count, n + count) : 0.0f;
+    const float d = chunk.x - mean.sum;
+    mean.add(d * share);
+    squares.add(fmaf(d * (n * share), d, chunk.y));
+    n += count;
+  }
+};
+
 // NaN or infinite data give NaN statistics (their mean is NaN or infinite).
 __device__ __forceinline__ float rstd_of(const Moment& m, float eps) {
   return isfinite(m.mean) ? rsqrtf(m.squares / m.n + eps) : __int_as_float(0x7fc00000);

@@ -176,17 +176,21 @@ __global__ void __launch_bounds__(kJoinThreads) norm_means_kernel(
   parts += static_cast<long long>(p.view) * s.chunks * s.channels + p.channel;
   sums += static_cast<long long>(p.view) * s.channels + p.channel;
   wait_for_kernel_before();
-  float2 total = make_float2(0.0f, 0.0f);
+  // This lane's chunks of channel x.
+  LongSum sum, dot;
   if (p.x < p.channels) {
 #pragma unroll 8
-    for (int i = p.y; i < s.chunks; i += p.lanes)
-      total = add2(total, parts[static_cast<long long>(i) * s.channels + p.x]);
+    for (int i = p.y; i < s.chunks; i += p.lanes) {
+      const float2 v = parts[static_cast<long long>(i) * s.channels + p.x];
+      sum.add(v.x);
+      dot.add(v.y);
+    }
   }
-  entry[p.y * (p.width + 1) + p.x] = total;
+  entry[p.y * (p.width + 1) + p.x] = make_float2(sum.sum, dot.sum);
   __syncthreads();
   // A warp a channel, from its lanes.
   for (int c = warp; c < p.channels; c += blockDim.x / 32) {
-    total = make_float2(0.0f, 0.0f);
+    float2 total = make_float2(0.0f, 0.0f);
     for (int i = lane; i < p.lanes; i += 32) total = add2(total, entry[i * (p.width + 1) + c]);
     total.x = warp_sum(total.x);
     total.y = warp_sum(total.y);
