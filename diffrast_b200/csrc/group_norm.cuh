@@ -21,11 +21,9 @@
 // passes joins the blocks' sums of each channel and the channels of each group, and leaves the
 // constants of each view's channels for the second pass as it reads them.
 //
-// What a block does once costs as much as many of its rows: with the statistics joined per group in
-// every block, divisions for the threads' places and the channels' constants formed by every
-// thread, 1000 instructions of a warp were spent beside 35 for each row of vectors, and a view of
-// 8 MB took 17 us with all its data in L2. Hence the block's shape, the sums by channel and the
-// tables of constants.
+// A row of vectors costs a warp 53 instructions in the first pass, so what a block does once is kept
+// small: its shape gives the threads their places without a division, it sums by channel whatever
+// the groups, and it reads the channels' constants from tables.
 #pragma once
 
 #include <algorithm>
@@ -131,13 +129,14 @@ __device__ __forceinline__ float2 exp_minus(float2 z) {
   return make_float2(power_of_two(t.x), power_of_two(t.y));
 }
 
-// 1 / d of a pair. The special-function unit gives 16 results a clock and processor, and with an
-// exponential and a reciprocal for each value it is the busiest unit of the second pass (74% of its
-// rate). One reciprocal for both values, 1 / a = b / (a b), takes four images of 512 x 512 x 64
-// bfloat16 from 73 to 70 us forward and nothing off the backward pass, but their product leaves the
-// range of float32 with exp(-z) above 2^63, a NaN spoils its neighbour, and what it takes to tell
-// (a test of each pair: 79 us; of each vector: 74; all rows again after a test at their end: 72, in
-// registers that the passes do not have) gives the time back.
+// 1 / d of a pair. The special-function unit gives 16 results a clock and processor, and an
+// exponential and a reciprocal for each value keep it busy for 29 of the 43 us of the second pass over
+// four images of 512 x 512 x 64 bfloat16. One reciprocal for both values, 1 / a = b / (a b), takes
+// their forward pass from 74 to 70 us and 2 us off the backward pass, but the product leaves the
+// range of float32 with exp(-z) above 2^63, and a NaN spoils its neighbour. What it takes to tell
+// gives the time back: 79 us with a test of each pair, 74 of each vector, 72 with all rows again after
+// a test at their end (in registers that the passes do not have), 73 with exp(-|z|), at most 1, and
+// selects.
 __device__ __forceinline__ float2 reciprocals(float2 d) {
   return make_float2(reciprocal(d.x), reciprocal(d.y));
 }
@@ -493,10 +492,10 @@ struct Affine {
 
 // The kernels that join the blocks' sums: a block has a run of whole groups of at most 8 channels
 // together, or one group of at most 32, by as many lanes as it has threads for (with 32 channels to
-// every block, two blocks read all the parts of 64 channels, in 10 us instead of 7; they are the
+// every block, two blocks read all the parts of 64 channels, 3 us longer; they are the
 // only work between the two passes). Of wider groups it has 32 channels, and a second kernel joins the
-// channels of each group (the norm of 301 x 301 x 256 in one group takes 61 us so, 116 us with one
-// block for the group).
+// channels of each group (the norm of 301 x 301 x 256 float32 in one group takes 61 us so, 116
+// us with one block for the group).
 constexpr int kJoinThreads = 1024;
 constexpr int kJoinChannels = 32;
 
@@ -532,7 +531,7 @@ struct JoinPlace {
 // each channel from their shared memory, and finishes its rows from its own: one launch, and the
 // image is read once and written once. (Larger teams, over all processors and through memory, had
 // some 18 us from one slab's copies to its results, and too little shared memory to cover that with
-// other slabs: 171 us for the 74 us of the two passes on four images of 512 x 512 x 64.)
+// other slabs: 171 us where the two passes took 74, on four images of 512 x 512 x 64.)
 
 constexpr int kMostCluster = 16;
 
@@ -783,7 +782,7 @@ inline bool too_large(long long batch, long long pixels, long long stride) {
 
 // Blocks for each view of the kernels that join the blocks' sums (see JoinPlace), and their
 // threads: all or, where a view has few chunks, a warp for each channel (of 64 views of 512 KB each
-// the forward pass takes 26 us so and 37 us with 1024 threads to every block).
+// the forward pass takes 26 us so and 33 us with 1024 threads to every block).
 inline unsigned int join_runs(const NormShape& s) {
   const int run = join_channels(s.group_channels);
   return static_cast<unsigned int>((s.channels + run - 1) / run);
@@ -798,19 +797,28 @@ constexpr int kMostShared = 220 * 1024;  // dynamic shared memory of a block
 // Blocks of a processor that the kernels' registers allow, forward and backward.
 constexpr int kResident[2] = {4, 3};
 
-// Largest view that is taken in clusters. One view of 32 KB (16 x 16 x 64 bfloat16) takes 5.2 us
-// forward and 4.6 us backward in clusters, 6.2 and 7.0 us in two passes, and 1024 of them 24 and 37
-// us against 48 and 58 us; four of 256 KB 7.3 and 8.1 us against 7.8 and 9.3 us, and 256 of them 42
-// and 69 us against 46 and 70 us. At 512 KB neither is ahead (four: 8.7 and 10.2 us against 8.3 and
-// 10.6 us; 256: 78 and 132 us against 78 and 118 us).
+// Largest view that is taken in clusters, both ways. One view of 32 KB (16 x 16 x 64 bfloat16) takes
+// 4.8 us forward and 4.5 us backward in clusters, 6.2 and 7.0 us in two passes, and 1024 of them 21
+// and 34 us against 47 and 56 us. Four of 256 KB take 7.4 and 8.1 us against 7.8 and 9.4 us, and 256
+// of them 43 and 71 us against 46 and 68 us: there the backward pass is even, ahead with few views
+// and behind with many. At 512 KB clusters are behind (four: 8.8 and 10.4 us against 8.5 and 10.9 us;
+// 256: 79 and 137 us against 75 and 119 us).
 constexpr long long kClusterBytes = 1LL << 18;
 
 // The plan of a call in clusters, or false where none fits: tiles of whole groups, and blocks to a
 // cluster, by the estimated time in microseconds. A block's own is what is fixed (2, or 3 with a
-// cluster, and with clusters the start of all blocks of a wave: sixteen views of 128 KB take 10.7 us
+// cluster, and with clusters the start of all blocks of a wave: sixteen views of 128 KB took 10.7 us
 // in 512 blocks of clusters and 6.5 us in 128 without), its bytes at a processor's share of the
 // memory, and its rows' instructions, or the cache lines that its warps' copies touch if those are
 // slower; the blocks of a processor overlap, as many as its registers and shared memory hold.
+//
+// The constants: 43.5e3 bytes a microsecond are a processor's share of the measured copy rate (6446
+// GB/s by 148); 1.9e3 clocks are a microsecond, and a clock moves one line of 128 bytes between a
+// processor and L2 (a warp's copy touches 4, or 32 / cols with rows of fewer vectors); 0.16 and 0.31 us
+// are a row of the 8 warps through both loops, some 150 and 290 instructions a warp at four a clock;
+// rows of a tile shorter than 64 and 32 bytes waste parts of their 32-byte sectors (1.3 and 2.0). The
+// fixed times, 1.0 for joins and constants and 0.01 a block, are set by hand to timings of 1 to 1024
+// views of 8 to 512 KB. They choose between plans that are all right, and bound nothing.
 inline bool plan_clusters(NormShape& s, ClusterPlan& t, const NormVector& v, long long batch,
                           long long pixels, int channels, int groups, int dtype,
                           long long x_stride, long long grad_stride, int images, int processors) {
@@ -923,9 +931,9 @@ inline int views_at_once(long long batch) {
 // The plan of a call in passes over memory. A block's start and the join of its sums cost as much
 // as 16 rows of its threads, and with long blocks the last ones run alone, so a block has about 24
 // rows of them (96 KB of 16-byte vectors); blocks fill the processors evenly, up to `resident` to
-// each, or several times over. Four images of 512 x 512 x 64 bfloat16 take 76, 74, 78 and 91 us
-// forward with 16, 24, 48 and 112 rows, and 114, 115, 120 and 126 us backward; eight of 128 x 128 x
-// 256 with dropout take 65, 65, 70 and 112 us, and 96, 96, 92 and 148 us.
+// each, or several times over. Four images of 512 x 512 x 64 bfloat16, called again and again, take
+// 72, 72, 82 and 100 us forward with 16, 24, 48 and 112 rows, and 113, 113, 120 and 135 us backward;
+// eight of 128 x 128 x 256 with dropout take 55, 55, 63 and 79 us, and 97, 97, 94 and 151 us.
 inline void plan_passes(NormShape& s, const NormVector& v, long long batch, long long pixels,
                         int channels, int groups, int dtype, long long x_stride,
                         long long grad_stride, int images, int processors) {

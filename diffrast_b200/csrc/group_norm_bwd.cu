@@ -89,9 +89,10 @@ __device__ __forceinline__ Leftover leftover_at(const T* x, const T* grad, long 
 
 // First pass: sums of q and q (x - m) of each channel over one chunk of rows in one tile of columns.
 // parts [batch][chunks][channels]. Bound by memory: 268 MB (x and the gradient of four images of 512
-// x 512 x 64 bfloat16) in 54 us, 5.0 TB/s; a warp has 133 instructions for each of its rows of
-// vectors, 62% of the rate at which it could issue them. With dropout the generator's registers
-// leave room for two blocks.
+// x 512 x 64 bfloat16) in 57 us, 4.7 TB/s; a warp has 117 instructions for each of its rows of
+// vectors, 55% of the rate at which it could issue them, and 16 results of the special-function unit.
+// With dropout the generator's registers leave room for two blocks, and both passes are bound by
+// their instructions (64% of the rate, with 23% of the warps that a processor can hold).
 template <typename T, int V, bool Silu, bool Drop>
 __global__ void __launch_bounds__(kNormThreads, Drop ? 2 : 3) norm_sums_kernel(
     const T* __restrict__ x, const T* __restrict__ grad, NormShape s, int view0,
@@ -160,7 +161,7 @@ __device__ __forceinline__ void write_constants(float* table, const NormShape& s
 
 // Joins the parts of a view's channels into sums [batch][channels] of q and q h, and the channels of
 // its groups where a block has them all; the others are left to norm_group_means_kernel. Bound by
-// latency: 7 us for four views of 64 channels.
+// latency: 8 us for four views of 64 channels.
 __global__ void __launch_bounds__(kJoinThreads) norm_means_kernel(
     const float2* parts, NormShape s, int view0, const float* __restrict__ affine,
     const float* __restrict__ rstd, float2* __restrict__ sums, float* __restrict__ table) {
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_group_means_kernel(
 
 // Second pass: grad x = r (q w - A - h B) over one chunk of rows in one tile of columns, from the
 // end of the views to their start (what the first pass read last is still in L2: of four images of
-// 512 x 512 x 64 bfloat16 a fifth is). Bound by memory: 55 us for those, 403 MB read and written.
+// 512 x 512 x 64 bfloat16 a fifth is). Bound by memory: 60 us for those, 403 MB read and written.
 template <typename T, int V, bool Silu, bool Drop>
 __global__ void __launch_bounds__(kNormThreads, Drop ? 2 : 3) norm_grad_kernel(
     const T* __restrict__ x, const T* __restrict__ grad, NormShape s, int view0,
@@ -334,7 +335,7 @@ struct Gradients {
 
 // The whole pass by clusters of blocks (see "clusters" in group_norm.cuh). The gradients of weight
 // and bias are written here where they are sums of one view (`direct`); otherwise the views' sums
-// are left for norm_params_kernel. Bound by latency: 4.6 us for one 16 x 16 x 64 bfloat16 view.
+// are left for norm_params_kernel. Bound by latency: 4.5 us for one 16 x 16 x 64 bfloat16 view.
 template <typename T, int V, bool Silu, bool Drop>
 __global__ void __launch_bounds__(kNormThreads, Drop ? 2 : 3) norm_cluster_bwd_kernel(
     const T* __restrict__ x, const T* __restrict__ grad, NormShape s, ClusterPlan t,

@@ -1,4 +1,4 @@
-// Vectors of float32, float16 and bfloat16 values: one load or store of up to 32 bytes, arithmetic
+// Vectors of float32, float16 and bfloat16 values: one load or store of up to 16 bytes, arithmetic
 // in float32, one rounding (to nearest even) on the way out.
 #pragma once
 

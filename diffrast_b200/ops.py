@@ -687,7 +687,9 @@ def group_norm(
 
     Differentiable in ``x``, ``weight`` and ``bias``; the backward pass computes activation and
     mask again from ``x``. Forward-mode derivatives raise ``NotImplementedError``. A group with NaN
-    or infinite values is NaN throughout. Not part of diffrast's API.
+    or infinite values is NaN throughout; where a group's sum of squared deviations passes float32's
+    range, its deviation counts as infinite and its values are normalised to 0. Not part of
+    diffrast's API.
     """
     channels = _check_features(x, "x")
     if isinstance(groups, bool) or not isinstance(groups, int):

@@ -116,3 +116,17 @@ def test_very_negative_values_go_to_zero(layout, seed, dtype):
         rounded = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
         within(y[:, z < 0], want[z < 0], ((10 + 1.25 * near) * U * want.abs() + rounded * want.abs() + FLUSH)[z < 0])
         within(slope[z < -20], want_slope[z < -20], ((20 + 1.25 * near) * U * want_slope.abs() + FLUSH)[z < -20])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_groups_whose_squares_pass_the_range_are_normalised_to_zero(layout, dtype):
+    batch, height, width, channels, extra = LAYOUTS[layout]
+    gen = torch.Generator(device=CUDA).manual_seed(4)
+    x = 1e20 * torch.randn(batch, height, width, channels + extra, generator=gen, device=CUDA)
+    x = x.to(dtype)[..., extra:].requires_grad_(True)
+    bias = torch.linspace(-3, 3, channels, device=CUDA, requires_grad=True)
+    y = dr.group_norm(x, 1, None, bias)
+    assert torch.equal(y.float(), bias.to(dtype).float().expand_as(y))
+    grad_x, grad_bias = torch.autograd.grad(y, (x, bias), torch.ones_like(y))
+    assert bool((grad_x == 0).all()) and bool((grad_bias == batch * height * width).all())
