@@ -3,8 +3,7 @@
 With weights of zero, z is the channel's bias exactly, so that the activation's own error is all
 there is. With u = 2^-24, t = z / ln 2 rounded and its power of two are off by 1.23 |z| u + 4 u
 relative (a product, its constant, 2^-22 for the power), which counts as an error of z of that size.
-1 / (1 + exp) and the products around it add 5 u to s and 6 u to 1 - s (a sum, a product, a
-reciprocal within 2 u, a product each). So
+The sum, the reciprocal (within 2 u) and the products add at most 5 u to s and 6 u to 1 - s. So
 
 - y = z s is off by (10 + 1.25 |z|) u |y| below zero, 8 u |y| + 2 u above it (|z s (1 - s)| < 0.23
   and z^2 s (1 - s) < 0.45 multiply the error of z);
@@ -90,7 +89,7 @@ FAR = torch.logspace(19, 38, 32, dtype=torch.float64)
 @pytest.mark.parametrize("layout", LAYOUTS)
 @pytest.mark.parametrize("seed", range(3))
 def test_large_values_beside_very_negative_ones(layout, seed):
-    """Neighbours share a reciprocal, and no product of theirs may pass float32's range."""
+    """No value passes float32's range, or changes, because of what its neighbour is."""
     z = torch.cat([FAR, -torch.logspace(1.5, 2, 32, dtype=torch.float64)]).float()
     z = z[torch.randperm(64, generator=torch.Generator().manual_seed(seed))]
     y, slope = run(layout, z)
